@@ -274,6 +274,106 @@ typedef struct tgcb_segment {
 int tgcb_peer_allreduce_avg_f32(const tgcb_peer_group* g, const tgcb_segment* segs, int n_segs, int slot,
                                 uint32_t epoch, int ctas, void* stream);
 
+/* ---- Token generation: heads, an int8 cache of keys and values, attention over it ----
+ * The reference has one float32 attention head (tgc/analysis/attention.py:97-137), a row norm
+ * (normalisation.py:61-70) and a per-row int8 quantiser (quantize.py:90-128); these entry points
+ * are the same functions in the form a program that generates tokens calls them in. */
+#define TGCB_F32 0
+#define TGCB_BF16 1
+#define TGCB_F16 2
+
+/* Rows [tokens, heads, width] with unit stride along width; strides in elements. */
+typedef struct tgcb_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} tgcb_heads;
+
+/* RMS norm of every query and key head and the rotation of its first `rotary` columns:
+ * y = x / sqrt(mean(x^2) + epsilon) * gain, then column pairs (i, i + rotary/2), or with
+ * interleaved != 0 (2i, 2i + 1), turned by positions[token] * frequencies[i] radians.
+ * Forward: out = rotate(norm(in)). Backward: given `grad`, the gradients of the forward's outputs,
+ * `out` receives the gradients of its inputs and gain_grad those of the gains (summed over tokens and heads
+ * in a fixed order). Index 0 of each pair is the queries, 1 the keys. `out` may be `in` or `grad`
+ * itself (same data and strides) but must not overlap them otherwise. */
+typedef struct tgcb_rotary_desc {
+  int32_t dtype;          /* TGCB_F32, TGCB_BF16 or TGCB_F16: in, grad, out */
+  int32_t gain_dtype;     /* TGCB_F32 or dtype: gain, gain_grad */
+  int32_t position_bytes; /* 4 or 8: signed integers */
+  int32_t interleaved;
+  int64_t tokens;         /* 0: nothing to do (the backward writes zero gain gradients) */
+  int32_t heads[2];       /* >= 1 */
+  int32_t width;          /* 2 .. 1024 */
+  int32_t rotary;         /* even, 2 .. width */
+  double epsilon;         /* > 0 */
+  const void* positions;  /* [tokens] */
+  const double* frequencies; /* [rotary / 2], radians per position */
+  const void* gain[2];    /* [width] */
+  tgcb_heads in[2];
+  tgcb_heads grad[2];     /* backward only */
+  tgcb_heads out[2];
+  void* gain_grad[2];     /* backward only, [width] */
+  void* scratch;          /* backward only: tgcb_norm_rotate_scratch_bytes(width) bytes, 16-byte aligned */
+  uint64_t scratch_bytes;
+} tgcb_rotary_desc;
+
+int tgcb_norm_rotate(const tgcb_rotary_desc* d, void* stream);
+size_t tgcb_norm_rotate_scratch_bytes(int width);
+int tgcb_norm_rotate_backward(const tgcb_rotary_desc* d, void* stream);
+
+/* A paged cache: row (page p, head h, place r) of keys and of values is `width` int8 codes at
+ * ((p * kv_heads + h) * page + r) * width and one float32 scale at (p * kv_heads + h) * page + r; the
+ * row stands for code * scale. Codes are 16-byte aligned. `faults` counts rows that a call refused on the
+ * device (see tgcb_batch). */
+typedef struct tgcb_cache {
+  int8_t* keys;
+  int8_t* values;
+  float* key_scales;
+  float* value_scales;
+  int32_t* faults;
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t page;  /* places in a page: 16, 32, 64 or 128 */
+  int32_t width; /* 32, 64, 128 or 256 */
+} tgcb_cache;
+
+/* Which sequence and place each token row of a call has. Sequence b owns token rows
+ * [offsets[b], offsets[b+1]) (offsets null: [b * each, (b+1) * each), each = tokens / batch); its row i
+ * lies at position starts[b] + i, which is place position % page of page
+ * table[b * table_stride + position / page]. Rows of no sequence are left as they were. A position that is
+ * negative or past the table, and a page outside [0, pages), is never accessed: it counts in
+ * cache->faults, an append skips it, a read gives NaN, and attention leaves its key out. */
+typedef struct tgcb_batch {
+  const int32_t* table;
+  const int32_t* starts;
+  const int32_t* offsets;
+  int64_t table_stride;
+  int64_t tokens;
+  int32_t batch;
+  int32_t max_pages;
+} tgcb_batch;
+
+/* Quantise each token's key and value rows [tokens, kv_heads, width] into the cache by
+ * tgcb_quantise_rows_i8's rule, bit for bit (a 16-bit value is its float32). Where several rows of a
+ * call have one place, the last of them is stored. */
+int tgcb_cache_append(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, const tgcb_heads* keys,
+                      const tgcb_heads* values, void* stream);
+/* The cached rows at each token's position, code * scale rounded to dtype. */
+int tgcb_cache_read(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, const tgcb_heads* keys,
+                    const tgcb_heads* values, void* stream);
+
+/* Attention of every token over its sequence's cached positions: query head h reads key head
+ * h / (q_heads / kv_heads); score = scale * (q . k), with cap > 0 cap * tanh(score / cap); softmax over the
+ * positions the token sees, times the values. Row i of sequence b sees positions 0 .. starts[b] + i;
+ * with `visible` ([tokens] bit sets) it sees positions 0 .. starts[b] - 1 and, of the call's own rows,
+ * starts[b] + j for each set bit j (rows past the 64th are seen by none). The rows' own keys must
+ * have been appended before. A token that sees nothing gets zeros. Scratch as
+ * tgcb_cached_attention_scratch_bytes says, 16-byte aligned, not shared by calls that may overlap. */
+size_t tgcb_cached_attention_scratch_bytes(const tgcb_cache* cache, const tgcb_batch* batch, int q_heads);
+int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, int q_heads,
+                          const tgcb_heads* queries, const int64_t* visible, float scale, float cap,
+                          const tgcb_heads* out, void* scratch, size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

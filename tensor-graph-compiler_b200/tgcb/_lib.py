@@ -80,6 +80,67 @@ class Segment(ctypes.Structure):
     _fields_ = [("offset", ctypes.c_uint64), ("count", ctypes.c_uint64)]
 
 
+class Heads(ctypes.Structure):
+    """tgcb_heads: rows [tokens, heads, width] at a device address, strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """tgcb_rotary_desc."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("gain_dtype", ctypes.c_int32),
+        ("position_bytes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32 * 2),
+        ("width", ctypes.c_int32),
+        ("rotary", ctypes.c_int32),
+        ("epsilon", ctypes.c_double),
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("gain", ctypes.c_void_p * 2),
+        ("rows_in", Heads * 2),
+        ("grad", Heads * 2),
+        ("rows_out", Heads * 2),
+        ("gain_grad", ctypes.c_void_p * 2),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_uint64),
+    ]
+
+
+class CacheDesc(ctypes.Structure):
+    """tgcb_cache."""
+
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+        ("faults", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+    ]
+
+
+class BatchDesc(ctypes.Structure):
+    """tgcb_batch."""
+
+    _fields_ = [
+        ("table", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
 SIGNATURES = {
     "tgcb_version": (ctypes.c_char_p, []),
     "tgcb_last_error": (ctypes.c_char_p, []),
@@ -144,6 +205,28 @@ SIGNATURES = {
     "tgcb_peer_allreduce_avg_f32": (
         ctypes.c_int,
         [ctypes.POINTER(PeerGroupDesc), ctypes.POINTER(Segment), ctypes.c_int, ctypes.c_int, ctypes.c_uint32, ctypes.c_int,
+         ctypes.c_void_p],
+    ),
+    "tgcb_norm_rotate": (ctypes.c_int, [ctypes.POINTER(RotaryDesc), ctypes.c_void_p]),
+    "tgcb_norm_rotate_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int]),
+    "tgcb_norm_rotate_backward": (ctypes.c_int, [ctypes.POINTER(RotaryDesc), ctypes.c_void_p]),
+    "tgcb_cache_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.c_int, ctypes.POINTER(Heads), ctypes.POINTER(Heads),
+         ctypes.c_void_p],
+    ),
+    "tgcb_cache_read": (
+        ctypes.c_int,
+        [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.c_int, ctypes.POINTER(Heads), ctypes.POINTER(Heads),
+         ctypes.c_void_p],
+    ),
+    "tgcb_cached_attention_scratch_bytes": (
+        ctypes.c_size_t, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.c_int]
+    ),
+    "tgcb_cached_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.c_int, ctypes.c_int, ctypes.POINTER(Heads),
+         ctypes.c_void_p, ctypes.c_float, ctypes.c_float, ctypes.POINTER(Heads), ctypes.c_void_p, ctypes.c_size_t,
          ctypes.c_void_p],
     ),
     "tgcb_quantise_rows_i8": (

@@ -6,16 +6,21 @@ one pass over the keys with the running maximum and sum rescaled as blocks arriv
 matrix never written to memory. ``block`` is checked as tgc checks it; the kernel's own key
 block is 64, which moves rounding, not the result. ``AttentionShape`` mirrors tgc's
 (attention.py:44-77).
+
+``cached_attention`` is the same function over a ``tgcb.kv_cache.QuantisedCache``, for the tokens a
+program generates: all heads of a batch of sequences in one call, query heads sharing key heads, single tokens,
+pieces of prompts and trees of drafted tokens.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
 
-from tgcb import _lib
+from tgcb import _lib, heads, kv_cache
 from tgcb.errors import ConfigError
 
 WIDTHS = (16, 32, 64, 128)
@@ -79,4 +84,58 @@ def streaming_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch
     q, k, v = (t.contiguous() for t in (queries, keys, values))
     out = torch.empty_like(q)
     streaming_attention_into(q, k, v, out)
+    return out
+
+
+def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, table: torch.Tensor, starts: torch.Tensor,
+                     offsets: torch.Tensor | None = None, *, visible: torch.Tensor | None = None, scale: float | None = None,
+                     cap: float | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of each token of a call over its sequence's cached positions.
+
+    ``queries`` [tokens, q_heads, width] with q_heads a multiple of the cache's heads (query head h
+    reads key head h // (q_heads // kv_heads)); ``table``, ``starts`` and ``offsets`` as for
+    ``QuantisedCache.append``, which must have stored the call's own keys and values before. Row i of
+    a sequence sees positions 0 .. starts + i. With ``visible`` (int64 [tokens]) it sees positions 0 .. starts - 1
+    and, among the call's own rows of its sequence, row j where bit j is set: a tree's ancestors
+    and the token itself. At most 64 rows a sequence can be named so.
+
+    score = scale * q.k (``scale`` None: 1 / sqrt(width)), then with ``cap`` cap * tanh(score / cap).
+    A token that sees nothing gets zeros. ``out`` (not the queries) receives the result; rows of no sequence are not written.
+    """
+    if not isinstance(cache, kv_cache.QuantisedCache):
+        raise ConfigError("cached_attention reads a QuantisedCache")
+    heads.check_rows("queries", queries)
+    device = cache.device
+    if queries.device != device:
+        raise ConfigError(f"queries must be on {device}, where the cache is")
+    tokens, q_heads, width = queries.shape
+    if width != cache.width or q_heads < 1 or q_heads % cache.kv_heads:
+        raise ConfigError(f"queries must be [tokens, a multiple of {cache.kv_heads} heads, {cache.width}], got {tuple(queries.shape)}")
+    b = kv_cache.batch_of(table, starts, offsets, tokens, device)
+    if visible is not None:
+        heads.check_vector("visible", visible, tokens, (torch.int64,), device)
+        if offsets is None and tokens > 64 * table.shape[0]:
+            raise ConfigError(f"a tree has at most 64 tokens, got {tokens // table.shape[0]} a sequence")
+    scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
+    cap = 0.0 if cap is None else float(cap)
+    if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
+        raise ConfigError(f"the scale has to be finite and the cap finite and not negative, got {scale} and {cap}")
+    if out is not None:
+        heads.check_rows("out", out, queries)
+        if out.shape != queries.shape:
+            raise ConfigError(f"out must have the shape {tuple(queries.shape)}, got {tuple(out.shape)}")
+        heads.check_written("out", out)
+        heads.check_apart("out", out, "queries", queries)
+    lib = _lib.load()
+    need = lib.tgcb_cached_attention_scratch_bytes(cache.desc, b, q_heads)
+    with heads.on_stream(device, stream):
+        if out is None:
+            out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with heads.on_device(device):
+        rc = lib.tgcb_cached_attention(
+            cache.desc, b, heads.DTYPES[queries.dtype], q_heads, heads.rows(queries), visible.data_ptr() if visible is not None else None,
+            scale, cap, heads.rows(out), scratch.data_ptr() if need else None, need, heads.raw(device, stream),
+        )
+    _lib.check(rc, "tgcb_cached_attention")
     return out

@@ -1,0 +1,99 @@
+"""The token-generation entry points without a GPU: calls that are refused before anything is launched."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from tgcb import _lib, attention, kv_cache, rotary
+from tgcb.errors import ConfigError
+
+memory = (ctypes.c_char * 4096)()  # never read: every call here is refused for its arguments
+HERE = (ctypes.addressof(memory) + 255) & ~255
+
+
+def rotary_desc(**change):
+    d = _lib.RotaryDesc(dtype=0, gain_dtype=0, position_bytes=4, tokens=3, heads=(2, 1), width=64, rotary=64, epsilon=1e-5, positions=HERE,
+                        frequencies=HERE, gain=(HERE, HERE), gain_grad=(HERE, HERE), scratch=HERE, scratch_bytes=1 << 40)
+    for i in range(2):
+        d.rows_in[i] = d.grad[i] = d.rows_out[i] = _lib.Heads(HERE, 64, 64)
+    for name, value in change.items():
+        setattr(d, name, value)
+    return d
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(dtype=3), "element type"), (dict(dtype=-1), "element type"), (dict(gain_dtype=1), "gains"), (dict(position_bytes=2), "positions"),
+    (dict(tokens=-1), "negative"), (dict(heads=(0, 1)), "head"), (dict(width=1), "width"), (dict(width=1025), "width"), (dict(rotary=0), "rotary"),
+    (dict(rotary=63), "rotary"), (dict(rotary=66), "rotary"), (dict(epsilon=0.0), "epsilon"), (dict(epsilon=float("nan")), "epsilon"),
+    (dict(positions=None), "null"), (dict(frequencies=None), "null"), (dict(gain=(HERE, None)), "null"), (dict(heads=(1 << 21, 1)), "2\\^20"),
+])
+def test_norm_rotate_refuses(change, why):
+    lib = _lib.load()
+    for entry in (lib.tgcb_norm_rotate, lib.tgcb_norm_rotate_backward):
+        assert entry(rotary_desc(**change), None) == _lib.TGCB_E_INVALID
+        with pytest.raises(Exception, match=why):
+            _lib.check(_lib.TGCB_E_INVALID, "norm_rotate")
+
+
+def test_norm_rotate_backward_refuses_its_scratch():
+    lib = _lib.load()
+    need = lib.tgcb_norm_rotate_scratch_bytes(64)
+    for change in (dict(scratch=None), dict(scratch_bytes=need - 1), dict(scratch=HERE + 4), dict(gain_grad=(HERE, None))):
+        assert lib.tgcb_norm_rotate_backward(rotary_desc(**change), None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_norm_rotate(None, None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_norm_rotate_scratch_bytes(0) == 0
+
+
+def cache_desc(**change):
+    return _lib.CacheDesc(**{**dict(keys=HERE, values=HERE, key_scales=HERE, value_scales=HERE, faults=HERE, pages=4, kv_heads=2, page=16,
+                                    width=64), **change})
+
+
+def batch_desc(**change):
+    return _lib.BatchDesc(**{**dict(table=HERE, starts=HERE, offsets=None, table_stride=2, tokens=6, batch=3, max_pages=2), **change})
+
+
+@pytest.mark.parametrize("cache,batch,dtype", [
+    (dict(keys=None), {}, 0), (dict(value_scales=None), {}, 0), (dict(faults=None), {}, 0), (dict(values=HERE + 8), {}, 0), (dict(width=48), {}, 0),
+    (dict(page=24), {}, 0), (dict(page=0), {}, 0), (dict(kv_heads=0), {}, 0), (dict(pages=0), {}, 0), (dict(pages=1 << 31), {}, 0),
+    ({}, dict(table=None), 0), ({}, dict(starts=None), 0), ({}, dict(batch=0), 0), ({}, dict(batch=4097), 0), ({}, dict(max_pages=0), 0),
+    ({}, dict(tokens=-1), 0), ({}, dict(tokens=7), 0), ({}, dict(tokens=1 << 32), 0), ({}, {}, 3), ({}, {}, -1),
+])
+def test_cache_calls_refuse(cache, batch, dtype):
+    lib, rows = _lib.load(), _lib.Heads(HERE, 128, 64)
+    c, b = cache_desc(**cache), batch_desc(**batch)
+    assert lib.tgcb_cache_append(c, b, dtype, rows, rows, None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_cache_read(c, b, dtype, rows, rows, None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_cached_attention(c, b, dtype, 4, rows, None, 1.0, 0.0, rows, HERE, 1 << 40, None) == _lib.TGCB_E_INVALID
+
+
+def test_null_rows_and_descriptors_are_refused():
+    lib, rows, nothing = _lib.load(), _lib.Heads(HERE, 128, 64), _lib.Heads(None, 128, 64)
+    c, b = cache_desc(), batch_desc()
+    for k, v in ((None, rows), (rows, None), (nothing, rows), (rows, nothing)):
+        assert lib.tgcb_cache_append(c, b, 0, k, v, None) == _lib.TGCB_E_INVALID
+        assert lib.tgcb_cache_read(c, b, 0, k, v, None) == _lib.TGCB_E_INVALID
+        assert lib.tgcb_cached_attention(c, b, 0, 4, k, None, 1.0, 0.0, v, HERE, 1 << 40, None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_cache_append(None, b, 0, rows, rows, None) == _lib.TGCB_E_INVALID
+    assert lib.tgcb_cache_append(c, None, 0, rows, rows, None) == _lib.TGCB_E_INVALID
+
+
+@pytest.mark.parametrize("q_heads,scale,cap", [(3, 1.0, 0.0), (0, 1.0, 0.0), (4, float("nan"), 0.0), (4, float("inf"), 0.0), (4, 1.0, -1.0),
+                                               (4, 1.0, float("nan")), (4, 1.0, float("inf"))])
+def test_attention_refuses(q_heads, scale, cap):
+    lib, rows = _lib.load(), _lib.Heads(HERE, 256, 64)
+    rc = lib.tgcb_cached_attention(cache_desc(), batch_desc(), 0, q_heads, rows, None, scale, cap, rows, HERE, 1 << 40, None)
+    assert rc == _lib.TGCB_E_INVALID
+
+
+def test_host_tensors_are_refused():
+    rows, gain = torch.randn(2, 2, 64), torch.ones(64)
+    with pytest.raises(ConfigError):
+        rotary.norm_rotate(rows, rows, gain, gain, torch.zeros(2, dtype=torch.int32), torch.ones(32, dtype=torch.float64))
+    with pytest.raises(ConfigError):
+        kv_cache.QuantisedCache(4, 2, 64, device="cpu")
+    with pytest.raises(ConfigError):
+        attention.cached_attention(rows, None, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
