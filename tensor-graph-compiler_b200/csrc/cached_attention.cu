@@ -4,8 +4,25 @@
 // capped to cap tanh(s_j / cap) on request, over the positions j the token sees; out = sum_j e^(s_j - m) v_j
 // / sum_j e^(s_j - m) with m the largest s_j, found in one pass by rescaling what has been added
 // whenever a larger score arrives.
+//
+// A unit is one sequence, one key head and up to ROWS = 8 RN query rows (tokens x the heads that
+// share the key head, token by token). Both products run on mma.sync with the cache as the left
+// operand: S^T [16 keys x 8 rows] = K Q^T and O^T [16 columns x 8 rows] += V^T P^T. With the rows as the narrow
+// side a single token's few query heads fill an 8-wide tile instead of a 16-wide one, and a
+// warp's codes are converted once for all its rows. The codes are exact in bfloat16; what
+// multiplies them is split into bfloat16 parts: the queries exactly (1 part from bfloat16, 2 from
+// float16, 3 from float32), the weights p_j * value scale into 2 parts (16 bits) for 16-bit rows, below their
+// own rounding, and 3 (24 bits) for float32 rows.
+//
+// What bounds it with few rows is reading the cache, 2 W + 8 bytes a position and head. Each
+// warp streams its own 32-key steps through a private ring in shared memory (cp.async), with no
+// barrier between warps until a unit ends. The work is the list of all units' steps, cut into
+// equal pieces, one per CTA, whatever the sequences' lengths are (they are known on the device alone):
+// a unit that lies in one piece is finished there, one that is cut leaves its parts in scratch and
+// `combine` joins them in order, so results do not depend on timing.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -19,84 +36,752 @@ namespace {
 using namespace tgcb_elem;
 using tgcb_kv::Batch;
 using tgcb_kv::Cache;
-using tgcb_kv::Place;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStep = 32;       // keys a warp takes at once; pages hold 16 or more, so a step touches at most two
+constexpr int kMaxCtas = 444;   // three per SM
+constexpr int kMinSteps = 8;    // steps a CTA takes at least: two per warp
+constexpr int kWholeBelow = 512;  // positions up to which units are not cut
 
 struct Args {
   const char* q;
   char* out;
   long long q_t, q_h, out_t, out_h;
   const long long* visible;
-  int q_heads;
+  float* parts;   // [2 * CTAs][ROWS * (W + 2)]: weighted sums, then each row's maximum and sum of weights
+  int4* cuts;     // [CTAs]: sequence (-1: none), head, row tile and last CTA of the unit that is cut at this CTA's end
+  int q_heads, group;
   float scale, cap;
+  int capacity;   // positions a table row holds
+  int whole;      // units are not cut
 };
 
-constexpr int kWarps = 4;
+template <typename T>
+struct Parts;
+template <>
+struct Parts<__nv_bfloat16> {
+  static constexpr int Q = 1, P = 2;
+};
+template <>
+struct Parts<__half> {
+  static constexpr int Q = 2, P = 2;
+};
+template <>
+struct Parts<float> {
+  static constexpr int Q = 3, P = 3;
+};
 
-// One warp per token and query head, one key at a time.
-template <typename T, int W>
-__global__ void __launch_bounds__(32 * kWarps) attend_rows(const Cache c, const Batch b, const Args a) {
-  __shared__ Place place;
-  const long long token = blockIdx.x;
-  if (threadIdx.x == 0) place.sequence = -1;
+// Shared memory. Row pitches keep a warp's reads of key rows (W / 4 bytes of row lane / 4 at column
+// lane % 4) and value rows (W / 8 bytes of rows 2 (lane % 4) .. at column lane / 4) on different banks
+// for widths up to 128 (two ways at 256).
+template <typename T, int W, int RN>
+struct Shape {
+  static constexpr int ROWS = 8 * RN;
+  static constexpr int KP = W == 128 || W == 256 ? W + 16 : W;
+  static constexpr int VP = W + 16;
+  static constexpr int STAGE = kStep * (KP + VP + 8);
+  static constexpr int STAGES = 2;
+  static constexpr int RING = kWarps * STAGES * STAGE;
+  static constexpr int OP = W + 4;  // pitch of a warp's sums in floats when the warps are joined
+  static constexpr int JOIN = kWarps * ROWS * (OP + 2) * 4;
+  static constexpr int QUERIES = RN * Parts<T>::Q * (W / 16) * 32 * 8;
+  static constexpr int BYTES = QUERIES + (RING > JOIN ? RING : JOIN);
+};
+
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(unsigned dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+
+// Bytes 0 and 2 of a word of int8 codes as two bfloat16: 128 + (x & 127) and 128 + (x & 128) are
+// both bfloat16 bit patterns (7 bits of mantissa count ones there), and their difference is x.
+__device__ __forceinline__ unsigned codes(unsigned w) {
+  const unsigned low = (w & 0x007f007fu) | 0x43004300u, sign = (w & 0x00800080u) | 0x43004300u;
+  unsigned r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(low), "r"(sign));
+  return r;
+}
+
+__device__ __forceinline__ void mma(float* d, const unsigned* a, unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ unsigned transposed(unsigned x) {
+  unsigned r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two floats as N pairs of bfloat16 whose sums they are: the leading 8 bits cut off N - 1 times (exact
+// remainders), the rest rounded.
+template <int N>
+__device__ __forceinline__ void split(float x, float y, unsigned* parts) {
+#pragma unroll
+  for (int i = 0; i < N - 1; ++i) {
+    parts[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+  }
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(parts[N - 1]) : "f"(y), "f"(x));
+}
+
+// A sequence's rows, units and steps.
+struct Sequence {
+  long long first;  // its first token row
+  int rows, tiles;  // token rows; tiles of ROWS query rows
+  long long start;
+  int end;    // positions that its last row may see
+  int steps;  // of one unit
+};
+
+template <int ROWS>
+__device__ __forceinline__ Sequence sequence_of(const Batch& b, const Args& a, int s) {
+  Sequence q;
+  long long last;
+  tgcb_kv::range_of(b, s, &q.first, &last);
+  q.rows = (int)(last - q.first);
+  q.tiles = (int)(((long long)q.rows * a.group + ROWS - 1) / ROWS);
+  q.start = __ldg(b.starts + s);
+  const long long end = q.start + q.rows;
+  q.end = (int)(end < 0 ? 0 : end > a.capacity ? a.capacity : end);
+  q.steps = max(1, (q.end + kStep - 1) / kStep);
+  return q;
+}
+
+template <int ROWS>
+__device__ __forceinline__ long long work_of(const Cache& c, const Batch& b, const Args& a, int s) {
+  const Sequence q = sequence_of<ROWS>(b, a, s);
+  return (long long)c.heads * q.tiles * (a.whole ? 1 : q.steps);
+}
+
+struct Begin {
+  long long total, offset;  // all work; this CTA's first piece within its first sequence
+  int sequence;
+};
+
+// Where this CTA's share of the work begins: the threads add up consecutive sequences, the CTA
+// scans the sums, and the thread in whose sequences the share begins walks to it.
+template <int ROWS>
+__device__ __forceinline__ void begin_at(const Cache& c, const Batch& b, const Args& a, long long* chunk, Begin* out) {
+  __shared__ long long warp_sums[kWarps];
+  const int per = (b.batch + kThreads - 1) / kThreads;
+  const int s0 = min(threadIdx.x * per, b.batch), s1 = min(s0 + per, b.batch);
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += work_of<ROWS>(c, b, a, s);
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if ((threadIdx.x & 31) >= o) upto += v;
+  }
+  if ((threadIdx.x & 31) == 31) warp_sums[threadIdx.x >> 5] = upto;
   __syncthreads();
-  tgcb_kv::find(c, b, token, &place);
-  __syncthreads();
-  if (place.sequence < 0) return;
-  const int lane = threadIdx.x & 31;
-  constexpr int E = W / 32;
-  long long first, last;
-  tgcb_kv::range_of(b, place.sequence, &first, &last);
-  const long long start = place.position - (token - first);
-  const long long end = a.visible ? start + (last - first) : place.position + 1;
-  const unsigned long long bits = a.visible ? (unsigned long long)a.visible[token] : 0ull;
-  for (int head = threadIdx.x >> 5; head < a.q_heads; head += kWarps) {
-    const T* q = reinterpret_cast<const T*>(a.q) + token * a.q_t + head * a.q_h;
-    T* out = reinterpret_cast<T*>(a.out) + token * a.out_t + head * a.out_h;
-    const int h = head / (a.q_heads / c.heads);
-    float x[E], o[E], m = -INFINITY, sum = 0.f;
-    bool any = false;
+  long long total = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = to_float(q[lane * E + i]), o[i] = 0.f;
-    for (long long j = 0; j < end; ++j) {
-      if (a.visible && j >= start && (j - start >= 64 || !((bits >> (j - start)) & 1))) continue;
-      const int page = tgcb_kv::page_of(c, b, place.sequence, j);
-      if (page < 0) continue;
-      any = true;
-      const long long at = ((long long)page * c.heads + h) * c.page + (j & (c.page - 1));
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(x[i], (float)c.keys[at * W + lane * E + i], s);
-#pragma unroll
-      for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-      s = s * c.key_scales[at] * a.scale;
-      if (a.cap > 0) s = a.cap * tanhf(s / a.cap);
-      const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-      const float keep = expf(m - base), p = expf(s - base);
-      m = mn;
-      sum = sum * keep + p;
-#pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = o[i] * keep + p * c.value_scales[at] * (float)c.values[at * W + lane * E + i];
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < (int)(threadIdx.x >> 5)) upto += warp_sums[w];
+    total += warp_sums[w];
+  }
+  const long long least = a.whole ? 1 : kMinSteps;
+  long long share = (total + gridDim.x - 1) / gridDim.x;
+  share = share < least ? least : share;
+  *chunk = share;
+  const long long target = blockIdx.x * share;
+  if (threadIdx.x == 0) out->total = total;
+  if (target >= upto - mine && target < upto) {
+    long long left = target - (upto - mine);
+    int s = s0;
+    for (;; ++s) {
+      const long long w = work_of<ROWS>(c, b, a, s);
+      if (left < w) break;
+      left -= w;
     }
+    out->sequence = s;
+    out->offset = left;
+  }
+  __syncthreads();
+}
+
+// Sums of weights of parts, where -1 marks a part whose scores were all -infinity: its factor is 0 beside
+// any other part, and a row with nothing else has no answer (NaN, as 0 / 0).
+__device__ __forceinline__ void add_sum(float* all, float sum, float factor) {
+  if (sum < 0.f)
+    *all = *all == 0.f ? -1.f : *all;
+  else if (sum != 0.f)
+    *all = fmaf(sum, factor, *all < 0.f ? 0.f : *all);
+}
+__device__ __forceinline__ float answer(float v, float sum) {
+  return sum == 0.f ? 0.f : sum < 0.f ? __int_as_float(0x7fffffff) : v / sum;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* v, bool wide) {
+  if (wide) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      union {
+        uint2 raw;
+        T e[4];
+      } x;
 #pragma unroll
-    for (int i = 0; i < E; ++i) out[lane * E + i] = from_float<T>(any ? o[i] / sum : 0.f);
+      for (int i = 0; i < 4; ++i) x.e[i] = from_float<T>(v[i]);
+      *reinterpret_cast<uint2*>(p) = x.raw;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = from_float<T>(v[i]);
   }
 }
 
-template <typename T, int W>
+template <typename T>
+__device__ __forceinline__ T* out_row(const Args& a, const Sequence& q, int head, int row) {
+  const int token = row / a.group, in_group = row - token * a.group;
+  return reinterpret_cast<T*>(a.out) + (q.first + token) * a.out_t + (long long)(head * a.group + in_group) * a.out_h;
+}
+
+template <typename T>
+__device__ __forceinline__ bool out_wide(const Args& a) {
+  return ((reinterpret_cast<uintptr_t>(a.out) | (unsigned long long)(a.out_t * sizeof(T)) | (unsigned long long)(a.out_h * sizeof(T))) &
+          (4 * sizeof(T) - 1)) == 0;
+}
+
+template <typename T, int W, int RN>
+__global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(const Cache c, const Batch b, const Args a) {
+  using S = Shape<T, W, RN>;
+  constexpr int NQ = Parts<T>::Q, NP = Parts<T>::P, ROWS = S::ROWS, TILES = W / 16;
+  constexpr float kLog2e = 1.4426950408889634f;
+  extern __shared__ __align__(16) unsigned char memory[];
+  __shared__ Begin begin;
+  asm volatile("griddepcontrol.launch_dependents;");
+  long long chunk;
+  begin_at<ROWS>(c, b, a, &chunk, &begin);
+  const long long total = begin.total;
+  long long at = blockIdx.x * chunk;
+  const long long stop = at + chunk < total ? at + chunk : total;
+  if (!a.whole && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (at >= stop) return;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, l4 = lane & 3;
+  uint2* queries = reinterpret_cast<uint2*>(memory);
+  unsigned char* ring = memory + S::QUERIES + warp * S::STAGES * S::STAGE;
+  const unsigned ring_at = static_cast<unsigned>(__cvta_generic_to_shared(ring));
+  const bool wide = out_wide<T>(a);
+  const float scale2 = a.scale * kLog2e, cap2 = a.cap * kLog2e, by_cap = a.cap > 0 ? a.scale / a.cap : 0.f;
+
+  int s = begin.sequence;
+  Sequence q = sequence_of<ROWS>(b, a, s);
+  const int per_unit0 = a.whole ? 1 : q.steps;
+  long long unit = begin.offset / per_unit0;
+  int from = (int)(begin.offset - unit * per_unit0);
+
+  while (at < stop) {
+    while (unit >= (long long)c.heads * q.tiles) {  // on to the next sequence that has rows
+      q = sequence_of<ROWS>(b, a, ++s);
+      unit = 0;
+    }
+    const int head = (int)(unit / q.tiles), tile = (int)(unit - (long long)head * q.tiles);
+    int to = q.steps;
+    if (!a.whole) to = stop - at < to - from ? from + (int)(stop - at) : to;
+    const int rows = min(ROWS, q.rows * a.group - tile * ROWS);
+
+    // The unit's queries as right-hand fragments: word pair (part, k, lane) holds row lane / 4's columns
+    // (lane % 4) W / 4 + 4 k + {0, 2} and {1, 3}, as `codes` delivers the keys' columns.
+    __syncthreads();
+    for (int i = threadIdx.x; i < RN * TILES * 32; i += kThreads) {
+      const int ln = i & 31, k = (i >> 5) % TILES, rn = (i >> 5) / TILES;
+      const int r = rn * 8 + (ln >> 2);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < rows) {
+        const int row = tile * ROWS + r, token = row / a.group, in_group = row - token * a.group;
+        const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h +
+                     (ln & 3) * (W / 4) + 4 * k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = to_float(p[j]);
+      }
+      unsigned even[NQ], odd[NQ];
+      split<NQ>(v[0], v[2], even);
+      split<NQ>(v[1], v[3], odd);
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) queries[((rn * NQ + j) * TILES + k) * 32 + ln] = make_uint2(even[j], odd[j]);
+    }
+    __syncthreads();
+
+    // What this lane's rows 2 l4 + {0, 1} of each row tile see: positions below `limit`, and with
+    // `visible` those whose bit is set. Positions below `all` are seen by every row.
+    int limit[RN][2];
+    unsigned long long bits[RN][2];
+    int all;
+    {
+      const int token0 = tile * ROWS / a.group;
+      const long long seen = a.visible ? q.start : q.start + token0 + 1;
+      all = (int)(seen < 0 ? 0 : seen > a.capacity ? a.capacity : seen);
+#pragma unroll
+      for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = tile * ROWS + min(rn * 8 + 2 * l4 + j, rows - 1), token = row / a.group;
+          const long long sees = a.visible ? q.start : q.start + token + 1;
+          limit[rn][j] = (int)(sees < 0 ? 0 : sees > a.capacity ? a.capacity : sees);
+          bits[rn][j] = a.visible ? (unsigned long long)__ldg(a.visible + q.first + token) : 0ull;
+        }
+    }
+    const int in_tree = a.visible ? min(q.rows, 64) : 0;
+    // a tile's rows need no step behind the last position that one of them sees
+    int end = to;
+    if (!a.visible) {
+      const long long sees = q.start + (tile * ROWS + rows - 1) / a.group + 1;
+      end = min(to, (int)(((sees < 0 ? 0 : sees > q.end ? q.end : sees) + kStep - 1) / kStep));
+    }
+
+    float m[RN][2], sum[RN][2], o[RN][TILES][4];
+    unsigned seen_rows = 0;
+#pragma unroll
+    for (int rn = 0; rn < RN; ++rn) {
+      m[rn][0] = m[rn][1] = -INFINITY, sum[rn][0] = sum[rn][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) o[rn][t][0] = o[rn][t][1] = o[rn][t][2] = o[rn][t][3] = 0.f;
+    }
+
+    // pages of a step's two halves, -1: none of it is read
+    auto pages_of = [&](int step) {
+      int2 p = make_int2(-1, -1);
+      if (step < end) {
+        const int position = step * kStep;
+        p.x = tgcb_kv::page_of(c, b, s, position);
+        if (p.x < 0 && lane == 0 && position < q.end) atomicAdd(c.faults, 1);
+        if (position + 16 < q.end) {
+          p.y = c.page_bits >= 5 ? p.x : tgcb_kv::page_of(c, b, s, position + 16);
+          if (p.y < 0 && lane == 0) atomicAdd(c.faults, 1);
+        }
+      }
+      return p;
+    };
+    auto issue = [&](int step, int stage, int2 p) {
+      const unsigned base = ring_at + stage * S::STAGE;
+      constexpr int CH = W / 16;       // 16-byte pieces of a row
+      constexpr int LANES = CH < 16 ? 32 / CH : 2;  // rows a warp copies at once
+      if (step < end) {
+        const int place = (step * kStep) & (c.page - 1);
+        const long long row0 = ((long long)max(p.x, 0) * c.heads + head) * c.page + place;
+        const long long row1 = ((long long)max(p.y, 0) * c.heads + head) * c.page + ((place + 16) & (c.page - 1)) - 16;
+#pragma unroll
+        for (int r0 = 0; r0 < kStep; r0 += LANES) {
+          const int r = r0 + lane / CH, piece = lane % CH;
+          const bool low = r0 < 16;  // LANES divides 16
+          const long long from_row = (low ? row0 : row1) + r;
+          const bool valid = (low ? p.x : p.y) >= 0;
+          copy16(base + r * S::KP + 16 * piece, c.keys + from_row * W + 16 * piece, valid);
+          copy16(base + kStep * S::KP + r * S::VP + 16 * piece, c.values + from_row * W + 16 * piece, valid);
+        }
+        const long long from_row = (lane < 16 ? row0 : row1) + lane;
+        const bool valid = (lane < 16 ? p.x : p.y) >= 0;
+        const unsigned scales = base + kStep * (S::KP + S::VP) + 4 * lane;
+        copy4(scales, c.key_scales + from_row, valid);
+        copy4(scales + 4 * kStep, c.value_scales + from_row, valid);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    int2 held[S::STAGES];
+    const int first = from + warp;
+#pragma unroll
+    for (int i = 0; i < S::STAGES; ++i) {
+      held[i] = pages_of(first + i * kWarps);
+      issue(first + i * kWarps, i, held[i]);
+    }
+    int2 next = pages_of(first + S::STAGES * kWarps);
+    int stage = 0;
+    for (int step = first; step < end; step += kWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
+      __syncwarp();
+      const unsigned char* K = ring + stage * S::STAGE;
+      const unsigned char* V = K + kStep * S::KP;
+      const float* key_scale = reinterpret_cast<const float*>(V + kStep * S::VP);
+      const float* value_scale = key_scale + kStep;
+      const int position = step * kStep;
+      const bool inside = position + kStep <= all && held[0].x >= 0 && held[0].y >= 0;
+
+      // scores: [half of the step][row tile]{key g row 2 l4, same row 2 l4 + 1, key g + 8 ..}
+      float sc[2][RN][4], low[2][RN][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[h][rn][j] = low[h][rn][j] = 0.f;
+      constexpr int WORDS = W / 16 < 4 ? W / 16 : 4;  // words of a key row a lane reads at once
+#pragma unroll
+      for (int i = 0; i < TILES / WORDS; ++i) {
+        unsigned raw[2][2][WORDS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const unsigned char* p = K + (16 * h + 8 * j + g) * S::KP + l4 * (W / 4) + 4 * WORDS * i;
+            if constexpr (WORDS == 4) {
+              const uint4 x = *reinterpret_cast<const uint4*>(p);
+              raw[h][j][0] = x.x, raw[h][j][1] = x.y, raw[h][j][2] = x.z, raw[h][j][3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(p);
+              raw[h][j][0] = x.x, raw[h][j][1] = x.y;
+            }
+          }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          unsigned ka[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ka[h][0] = codes(raw[h][0][w]), ka[h][1] = codes(raw[h][1][w]);
+            ka[h][2] = codes(raw[h][0][w] >> 8), ka[h][3] = codes(raw[h][1][w] >> 8);
+          }
+#pragma unroll
+          for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+            for (int part = 0; part < NQ; ++part) {
+              const uint2 qb = queries[((rn * NQ + part) * TILES + i * WORDS + w) * 32 + lane];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) mma(part == 0 ? sc[h][rn] : low[h][rn], ka[h], qb.x, qb.y);
+            }
+        }
+      }
+
+      // scores in units of log2 e, masks
+      float vs[2][2];
+      unsigned seen = 0xffffffffu;  // bit (h RN + rn) 4 + j
+      float top[RN][2];
+#pragma unroll
+      for (int rn = 0; rn < RN; ++rn) top[rn][0] = top[rn][1] = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int key = 16 * h + 8 * k + g;
+          const float ks = key_scale[key];
+          vs[h][k] = value_scale[key];
+          const bool there = (h ? held[0].y : held[0].x) >= 0;
+          const int since = (int)min((long long)position + key - q.start, 1ll << 30);
+#pragma unroll
+          for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x = sc[h][rn][2 * k + j];
+              if (NQ > 1) x += low[h][rn][2 * k + j];
+              x *= ks;
+              x = a.cap > 0 ? cap2 * tanhf(x * by_cap) : x * scale2;
+              if (!inside) {
+                bool sees = position + key < limit[rn][j];
+                if (a.visible && since >= 0 && since < in_tree) sees = sees || ((bits[rn][j] >> since) & 1);
+                if (!(sees && there)) {
+                  x = -INFINITY;
+                  seen &= ~(1u << ((h * RN + rn) * 4 + 2 * k + j));
+                }
+              }
+              sc[h][rn][2 * k + j] = x;
+              top[rn][j] = fmaxf(top[rn][j], x);
+            }
+        }
+      float keep[RN][2];
+      bool moved = false;
+#pragma unroll
+      for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float t = top[rn][j];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+          const float mn = fmaxf(m[rn][j], t);
+          keep[rn][j] = mn == m[rn][j] ? 1.f : exp2_fast(m[rn][j] - mn);
+          moved |= mn != m[rn][j];
+          m[rn][j] = mn;
+          sum[rn][j] *= keep[rn][j];
+        }
+      constexpr bool FRESH = NP == 3;  // float32 rows: each step's products in accumulators of their own, added in float32
+      if (!FRESH && __any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+          for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[rn][t][j] *= keep[rn][j & 1];
+      }
+
+      // weights, and the products with the values
+      unsigned pb[2][RN][NP][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int rn = 0; rn < RN; ++rn) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float base = m[rn][j & 1] == -INFINITY ? 0.f : m[rn][j & 1];
+            const float p = exp2_fast(sc[h][rn][j] - base);
+            sum[rn][j & 1] += p;
+            w[j] = p * vs[h][j >> 1];
+            const unsigned bit = (seen >> ((h * RN + rn) * 4 + j)) & 1u;
+            if (!inside && !bit) w[j] = 0.f;  // whatever lies there
+            seen_rows |= bit << (rn * 2 + (j & 1));
+          }
+          unsigned lo[NP], hi[NP];
+          split<NP>(w[0], w[1], lo);
+          split<NP>(w[2], w[3], hi);
+#pragma unroll
+          for (int part = 0; part < NP; ++part) {
+            pb[h][rn][part][0] = transposed(lo[part]);
+            pb[h][rn][part][1] = transposed(hi[part]);
+          }
+        }
+      constexpr int VB = W / 8;                        // bytes of a value row a lane reads
+      constexpr int VW = VB / 4 < 4 ? VB / 4 : 4;      // words at once
+#pragma unroll
+      for (int i = 0; i < VB / 4 / VW; ++i) {
+        unsigned raw[2][4][VW];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const unsigned char* p = V + (16 * h + 2 * l4 + (j & 1) + 8 * (j >> 1)) * S::VP + g * VB + 4 * VW * i;
+            if constexpr (VW == 4) {
+              const uint4 x = *reinterpret_cast<const uint4*>(p);
+              raw[h][j][0] = x.x, raw[h][j][1] = x.y, raw[h][j][2] = x.z, raw[h][j][3] = x.w;
+            } else if constexpr (VW == 2) {
+              const uint2 x = *reinterpret_cast<const uint2*>(p);
+              raw[h][j][0] = x.x, raw[h][j][1] = x.y;
+            } else {
+              raw[h][j][0] = *reinterpret_cast<const unsigned*>(p);
+            }
+          }
+#pragma unroll
+        for (int t = 0; t < 2 * VW; ++t) {
+          const int word = t / 2, byte = (t & 1) * 2;
+          const unsigned pick0 = byte * 0x11 + (byte + 4) * 0x1100, pick1 = pick0 + 0x1111;
+          float fresh[RN][4];
+#pragma unroll
+          for (int rn = 0; rn < RN; ++rn) fresh[rn][0] = fresh[rn][1] = fresh[rn][2] = fresh[rn][3] = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned va[4];
+            va[0] = codes(__byte_perm(raw[h][0][word], raw[h][1][word], pick0));
+            va[1] = codes(__byte_perm(raw[h][0][word], raw[h][1][word], pick1));
+            va[2] = codes(__byte_perm(raw[h][2][word], raw[h][3][word], pick0));
+            va[3] = codes(__byte_perm(raw[h][2][word], raw[h][3][word], pick1));
+#pragma unroll
+            for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+              for (int part = 0; part < NP; ++part)
+                mma(FRESH ? fresh[rn] : o[rn][2 * VW * i + t], va, pb[h][rn][part][0], pb[h][rn][part][1]);
+          }
+          if (FRESH) {
+#pragma unroll
+            for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                o[rn][2 * VW * i + t][j] = fmaf(o[rn][2 * VW * i + t][j], keep[rn][j & 1], fresh[rn][j]);
+          }
+        }
+      }
+      __syncwarp();
+      issue(step + S::STAGES * kWarps, stage, next);
+#pragma unroll
+      for (int i = 0; i + 1 < S::STAGES; ++i) held[i] = held[i + 1];
+      held[S::STAGES - 1] = next;
+      next = pages_of(step + (S::STAGES + 1) * kWarps);
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // join the warps: maxima and sums, then the weighted sums of each row
+#pragma unroll
+    for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum[rn][j] += __shfl_xor_sync(0xffffffffu, sum[rn][j], x);
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) seen_rows |= __shfl_xor_sync(0xffffffffu, seen_rows, x);
+    __syncthreads();  // the rings are free
+    float* joined = reinterpret_cast<float*>(memory + S::QUERIES);
+    float* own = joined + warp * ROWS * (S::OP + 2);
+#pragma unroll
+    for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = rn * 8 + 2 * l4 + j;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)  // columns g W / 8 + 2 t + {0, 1}, at 16 t + 2 g
+          *reinterpret_cast<float2*>(own + r * S::OP + 16 * t + 2 * g) = make_float2(o[rn][t][j], o[rn][t][2 + j]);
+        if (g == 0) {
+          // a row that saw nothing has sum 0, one that saw scores of -infinity alone is marked with -1
+          const bool lowest = ((seen_rows >> (rn * 2 + j)) & 1) && m[rn][j] == -INFINITY;
+          own[ROWS * S::OP + 2 * r] = m[rn][j];
+          own[ROWS * S::OP + 2 * r + 1] = lowest ? -1.f : sum[rn][j];
+        }
+      }
+    __syncthreads();
+    const bool complete = from == 0 && to == q.steps;
+    // a piece that began in an earlier CTA goes to slot 0 of this CTA, one that ends in a later to slot 1
+    float* part = complete ? nullptr : a.parts + (2ll * blockIdx.x + (from == 0)) * ROWS * (W + 2);
+    constexpr int QUADS = W / 4;
+    for (int i = threadIdx.x; i < rows * QUADS; i += kThreads) {
+      const int r = i / QUADS, quad = i - r * QUADS;
+      const float* ml = joined + ROWS * S::OP + 2 * r;
+      float mm = -INFINITY, f[kWarps], all_sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[w * ROWS * (S::OP + 2)]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        f[w] = exp2_fast(ml[w * ROWS * (S::OP + 2)] - base);
+        add_sum(&all_sum, ml[w * ROWS * (S::OP + 2) + 1], f[w]);
+      }
+      const int col = 4 * quad, lane_of = col / (W / 8), t0 = (col % (W / 8)) / 2;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* from_w = joined + w * ROWS * (S::OP + 2) + r * S::OP + 2 * lane_of;
+        const float2 x = *reinterpret_cast<const float2*>(from_w + 16 * t0);
+        const float2 y = *reinterpret_cast<const float2*>(from_w + 16 * (t0 + 1));
+        v[0] = fmaf(x.x, f[w], v[0]), v[1] = fmaf(x.y, f[w], v[1]);
+        v[2] = fmaf(y.x, f[w], v[2]), v[3] = fmaf(y.y, f[w], v[3]);
+      }
+      if (complete) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = answer(v[j], all_sum);
+        store4<T>(out_row<T>(a, q, head, tile * ROWS + r) + col, v, wide);
+      } else {
+        *reinterpret_cast<float4*>(part + r * W + col) = make_float4(v[0], v[1], v[2], v[3]);
+        if (quad == 0) *reinterpret_cast<float2*>(part + ROWS * W + 2 * r) = make_float2(mm, all_sum);
+      }
+    }
+    if (!complete && from == 0 && threadIdx.x == 0) {
+      const long long last = (at + q.steps - 1) / chunk;
+      a.cuts[blockIdx.x] = make_int4(s, head, tile, (int)last);
+    }
+    at += a.whole ? 1 : to - from;
+    ++unit;
+    from = 0;
+  }
+}
+
+// Joins the parts of the unit that begins in CTA blockIdx.x of `attend` and was cut at its end, in the
+// order of the keys.
+template <typename T, int W, int RN>
+__global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, const Args a) {
+  constexpr int ROWS = 8 * RN, QUADS = W / 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.x < 0) return;
+  const Sequence q = sequence_of<ROWS>(b, a, cut.x);
+  const int rows = min(ROWS, q.rows * a.group - cut.z * ROWS);
+  const bool wide = out_wide<T>(a);
+  const int n = cut.w - blockIdx.x + 1;
+  auto part = [&](int i) { return a.parts + (i == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + i)) * ROWS * (W + 2); };
+  for (int i = threadIdx.x; i < rows * QUADS; i += 256) {
+    const int r = i / QUADS, col = 4 * (i - r * QUADS);
+    float mm = -INFINITY, all_sum = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) mm = fmaxf(mm, part(k)[ROWS * W + 2 * r]);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float* p = part(k);
+      const float2 ml = *reinterpret_cast<const float2*>(p + ROWS * W + 2 * r);
+      const float4 x = *reinterpret_cast<const float4*>(p + r * W + col);
+      const float f = exp2_fast(ml.x - base);
+      add_sum(&all_sum, ml.y, f);
+      v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = answer(v[j], all_sum);
+    store4<T>(out_row<T>(a, q, cut.y, cut.z * ROWS + r) + col, v, wide);
+  }
+}
+
+// Row tiles of 8 a unit takes: as many as the call's sequences have rows on average, since a unit
+// reads and converts its keys once for all its rows.
+int row_tiles(const Batch& b, int group, int width) {
+  const long long rows = (b.tokens + b.batch - 1) / b.batch * group;
+  if (rows <= 8) return 1;
+  if (rows <= 16 || width > 128) return 2;
+  return 4;
+}
+
+size_t cuts_bytes() { return kMaxCtas * sizeof(int4); }
+
+size_t scratch_bytes(const Cache& c, const Batch& b, int q_heads) {
+  if (b.tokens == 0 || (long long)b.max_pages * c.page <= kWholeBelow) return 0;
+  const size_t rows = 8 * row_tiles(b, q_heads / c.heads, c.width);
+  return cuts_bytes() + 2ull * kMaxCtas * rows * (c.width + 2) * sizeof(float);
+}
+
+template <typename T, int W, int RN>
 int launch(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
-  attend_rows<T, W><<<(unsigned)b.tokens, 32 * kWarps, 0, s>>>(c, b, a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "cached_attention", cudaGetErrorString(e));
+  using S = Shape<T, W, RN>;
+  const char* what = "tgcb_cached_attention";
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+  static std::atomic<unsigned long long> configured{0};
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    e = cudaFuncSetAttribute(attend<T, W, RN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+    configured.fetch_or(bit);
+  }
+  // no more CTAs than there can be pieces of work
+  const long long tiles = (b.tokens * a.group + S::ROWS - 1) / S::ROWS + b.batch;
+  const long long steps = a.whole ? 1 : (a.capacity + kStep - 1) / kStep;
+  const long long pieces = (tiles * c.heads * steps + (a.whole ? 0 : kMinSteps - 1)) / (a.whole ? 1 : kMinSteps);
+  const unsigned grid = (unsigned)(pieces < kMaxCtas ? pieces : kMaxCtas);
+  attend<T, W, RN><<<grid, kThreads, S::BYTES, s>>>(c, b, a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+  if (a.whole) return TGCB_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, combine<T, W, RN>, c, b, a);
+  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
   return TGCB_OK;
+}
+
+template <typename T, int W>
+int by_rows(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
+  switch (row_tiles(b, a.group, W)) {
+    case 1: return launch<T, W, 1>(c, b, a, s);
+    case 2: return launch<T, W, 2>(c, b, a, s);
+    default:
+      if constexpr (W <= 128) return launch<T, W, 4>(c, b, a, s);
+      return launch<T, W, 2>(c, b, a, s);
+  }
 }
 
 template <typename T>
 int run(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
   switch (c.width) {
-    case 32: return launch<T, 32>(c, b, a, s);
-    case 64: return launch<T, 64>(c, b, a, s);
-    case 128: return launch<T, 128>(c, b, a, s);
-    default: return launch<T, 256>(c, b, a, s);
+    case 32: return by_rows<T, 32>(c, b, a, s);
+    case 64: return by_rows<T, 64>(c, b, a, s);
+    case 128: return by_rows<T, 128>(c, b, a, s);
+    default: return by_rows<T, 256>(c, b, a, s);
   }
 }
 
@@ -105,13 +790,15 @@ int run(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
 extern "C" {
 
 size_t tgcb_cached_attention_scratch_bytes(const tgcb_cache* cache, const tgcb_batch* batch, int q_heads) {
-  (void)cache, (void)batch, (void)q_heads;
-  return 0;
+  Cache c;
+  Batch b;
+  if (tgcb_kv::checked(cache, batch, TGCB_F32, &c, &b, "tgcb_cached_attention_scratch_bytes") != TGCB_OK) return 0;
+  return q_heads < 1 || q_heads % c.heads ? 0 : scratch_bytes(c, b, q_heads);
 }
 
 int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, int q_heads,
                           const tgcb_heads* queries, const int64_t* visible, float scale, float cap,
-                          const tgcb_heads* out, void* scratch, size_t scratch_bytes, void* stream) {
+                          const tgcb_heads* out, void* scratch, size_t scratch_size, void* stream) {
   const char* what = "tgcb_cached_attention";
   Cache c;
   Batch b;
@@ -121,13 +808,21 @@ int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int 
   if (queries == nullptr || out == nullptr || (b.tokens > 0 && (queries->data == nullptr || out->data == nullptr)))
     return bad("null pointer");
   if (q_heads < 1 || q_heads % c.heads) return bad("the query heads must be a multiple of the cache's heads");
+  if (b.tokens * q_heads > 0x7fffffffll) return bad("too many tokens");
   if (!std::isfinite(scale)) return bad("the scale must be finite");
   if (!(cap >= 0) || std::isinf(cap)) return bad("the cap must be finite and not negative");
   if (b.tokens == 0) return TGCB_OK;
-  (void)scratch, (void)scratch_bytes;
-  const Args a = {static_cast<const char*>(queries->data), static_cast<char*>(out->data), queries->token_stride,
-                  queries->head_stride, out->token_stride, out->head_stride,
-                  reinterpret_cast<const long long*>(visible), q_heads, scale, cap};
+  const size_t need = scratch_bytes(c, b, q_heads);
+  if (need && (scratch == nullptr || scratch_size < need || (reinterpret_cast<uintptr_t>(scratch) & 15u)))
+    return bad("scratch must be 16-byte aligned and hold tgcb_cached_attention_scratch_bytes");
+  Args a = {};
+  a.q = static_cast<const char*>(queries->data), a.q_t = queries->token_stride, a.q_h = queries->head_stride;
+  a.out = static_cast<char*>(out->data), a.out_t = out->token_stride, a.out_h = out->head_stride;
+  a.visible = reinterpret_cast<const long long*>(visible);
+  a.cuts = static_cast<int4*>(scratch);
+  a.parts = need ? reinterpret_cast<float*>(static_cast<char*>(scratch) + cuts_bytes()) : nullptr;
+  a.q_heads = q_heads, a.group = q_heads / c.heads, a.scale = scale, a.cap = cap;
+  a.capacity = b.max_pages * c.page, a.whole = need == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case TGCB_F32: return run<float>(c, b, a, s);

@@ -135,7 +135,7 @@ int checked(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, Cache* 
   if (cache->pages < 1 || cache->pages > 0x7fffffffll) return bad("a cache has 1 to 2^31 - 1 pages");
   if (batch->tokens < 0 || batch->tokens > 0x7fffffffll) return bad("too many tokens");
   if (batch->batch < 1 || batch->batch > kMaxBatch) return bad("a call has 1 to 4096 sequences");
-  if (batch->max_pages < 1 || batch->max_pages > (1 << 24)) return bad("a page table has 1 to 2^24 pages a sequence");
+  if (batch->max_pages < 1 || (long long)batch->max_pages * cache->page > (1ll << 30)) return bad("a page table holds 1 to 2^30 positions a sequence");
   if (batch->table == nullptr || batch->starts == nullptr) return bad("null pointer in the batch");
   if (batch->offsets == nullptr && batch->tokens % batch->batch != 0)
     return bad("without offsets every sequence has the same number of tokens");

@@ -26,6 +26,8 @@ def nvcc_command(output: str = LIBRARY) -> list[str]:
         *ARCH,
         "-lineinfo",
         "-O3",
+        "--threads",
+        "0",
         "-std=c++17",
         "-Xcompiler",
         "-fPIC",
