@@ -72,15 +72,10 @@ struct Parts<float> {
   static constexpr int Q = 3, P = 3;
 };
 
-// Shared memory. Row pitches keep a warp's reads of key rows (W / 4 bytes of row lane / 4 at column
-// lane % 4) and value rows (W / 8 bytes of rows 2 (lane % 4) .. at column lane / 4) on different banks
-// for widths up to 128 (two ways at 256).
 template <typename T, int W, int RN>
 struct Shape {
   static constexpr int ROWS = 8 * RN;
-  static constexpr int KP = W == 128 || W == 256 ? W + 16 : W;
-  static constexpr int VP = W + 16;
-  static constexpr int STAGE = kStep * (KP + VP + 8);
+  static constexpr int STAGE = kStep * (2 * W + 8);
   static constexpr int STAGES = 2;
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int OP = W + 4;  // pitch of a warp's sums in floats when the warps are joined
@@ -89,6 +84,29 @@ struct Shape {
   static constexpr int BYTES = QUERIES + (RING > JOIN ? RING : JOIN);
 };
 
+// Where 16-byte piece `piece` of row `row` of a step lies in its row: permuted so that one piece of eight
+// consecutive rows, which ldmatrix reads at once, lies on all banks.
+template <int W>
+__device__ __forceinline__ int piece_at(int row, int piece) {
+  return piece ^ (W >= 128 ? row & 7 : W == 64 ? (row >> 1) & 3 : (row >> 2) & 1);
+}
+
+// One 16-byte piece of 32 rows of bytes, whose addresses the lanes give. Plain: word i is bytes
+// 4 (lane % 4) .. + 3 of row 8 i + lane / 4. Transposed: bytes 2 (lane / 4) and + 1 of row 8 i + 2 (lane % 4), then
+// the same two of the next row.
+__device__ __forceinline__ void load_rows(unsigned address, unsigned* w) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(address)
+               : "memory");
+}
+__device__ __forceinline__ void load_rows_transposed(unsigned address, unsigned* w) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(address)
+               : "memory");
+}
+
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
@@ -96,12 +114,17 @@ __device__ __forceinline__ void copy4(unsigned dst, const void* src, bool valid)
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
 
-// Bytes 0 and 2 of a word of int8 codes as two bfloat16: 128 + (x & 127) and 128 + (x & 128) are
-// both bfloat16 bit patterns (7 bits of mantissa count ones there), and their difference is x.
-__device__ __forceinline__ unsigned codes(unsigned w) {
-  const unsigned low = (w & 0x007f007fu) | 0x43004300u, sign = (w & 0x00800080u) | 0x43004300u;
-  unsigned r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(low), "r"(sign));
+// Bytes 0 and 2 of a word of int8 codes as two bfloat16, each x / 64. With the sign bit flipped a byte is x + 128,
+// and the bfloat16 whose low byte it is and whose high byte is zero has the value (x + 128) 2^-133, subnormal
+// below 128 and normal from there; times 2^127, minus 2, is x 2^-6, exactly. `flip` and `mask` are
+// 0x00800080 and 0x00ff00ff in registers, for with two constants in it the logic operation is issued twice.
+// Against cutting the byte into its sign and its other bits and subtracting the two as
+// bfloat16 numbers around 128: 1.5 arithmetic-logic instructions fewer for every two codes.
+constexpr float kCodeScale = 64.f;
+__device__ __forceinline__ unsigned codes(unsigned w, unsigned mask, unsigned flip) {
+  unsigned u, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x78;" : "=r"(u) : "r"(flip), "r"(w), "r"(mask));  // flip ^ (w & mask)
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x7f007f00u), "r"(0xc000c000u));
   return r;
 }
 
@@ -278,7 +301,11 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
   unsigned char* ring = memory + S::QUERIES + warp * S::STAGES * S::STAGE;
   const unsigned ring_at = static_cast<unsigned>(__cvta_generic_to_shared(ring));
   const bool wide = out_wide<T>(a);
-  const float scale2 = a.scale * kLog2e, cap2 = a.cap * kLog2e, by_cap = a.cap > 0 ? a.scale / a.cap : 0.f;
+  // a score's factor beside its key's scale: for the hyperbolic tangent of the cap, or in units of log2 e
+  const float factor = kCodeScale * (a.cap > 0 ? a.scale / a.cap : a.scale * kLog2e), cap2 = a.cap * kLog2e;
+  unsigned mask, flip;
+  asm volatile("mov.u32 %0, 0x00ff00ff;" : "=r"(mask));
+  asm volatile("mov.u32 %0, 0x00800080;" : "=r"(flip));
 
   int s = begin.sequence;
   Sequence q = sequence_of<ROWS>(b, a, s);
@@ -297,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
     const int rows = min(ROWS, q.rows * a.group - tile * ROWS);
 
     // The unit's queries as right-hand fragments: word pair (part, k, lane) holds row lane / 4's columns
-    // (lane % 4) W / 4 + 4 k + {0, 2} and {1, 3}, as `codes` delivers the keys' columns.
+    // 16 k + 4 (lane % 4) + {0, 2} and {1, 3}, as `codes` delivers the keys' columns.
     __syncthreads();
     for (int i = threadIdx.x; i < RN * TILES * 32; i += kThreads) {
       const int ln = i & 31, k = (i >> 5) % TILES, rn = (i >> 5) / TILES;
@@ -306,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
       if (r < rows) {
         const int row = tile * ROWS + r, token = row / a.group, in_group = row - token * a.group;
         const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h +
-                     (ln & 3) * (W / 4) + 4 * k;
+                     16 * k + 4 * (ln & 3);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = to_float(p[j]);
       }
@@ -368,28 +395,41 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
       }
       return p;
     };
+    constexpr int CH = W / 16;                    // 16-byte pieces of a row
+    constexpr int LANES = CH < 16 ? 32 / CH : 2;  // rows a warp copies at once; divides 16
+    // the permutation goes by a row's last three bits, so copies 8 rows apart share their offsets
+    constexpr int KINDS = LANES < 8 ? 8 / LANES : 1;
+    unsigned copy_to[KINDS];
+#pragma unroll
+    for (int i = 0; i < KINDS; ++i) {
+      const int r = i * LANES + lane / CH;
+      copy_to[i] = ring_at + r * W + 16 * piece_at<W>(r, lane % CH);
+    }
+    const unsigned scale_to = ring_at + 2 * kStep * W + 4 * lane;
+    const int lane_from = lane * 16;
     auto issue = [&](int step, int stage, int2 p) {
-      const unsigned base = ring_at + stage * S::STAGE;
-      constexpr int CH = W / 16;       // 16-byte pieces of a row
-      constexpr int LANES = CH < 16 ? 32 / CH : 2;  // rows a warp copies at once
       if (step < end) {
         const int place = (step * kStep) & (c.page - 1);
         const long long row0 = ((long long)max(p.x, 0) * c.heads + head) * c.page + place;
-        const long long row1 = ((long long)max(p.y, 0) * c.heads + head) * c.page + ((place + 16) & (c.page - 1)) - 16;
+        const long long row1 = ((long long)max(p.y, 0) * c.heads + head) * c.page + ((place + 16) & (c.page - 1));
+        const unsigned at_stage = stage * S::STAGE;
 #pragma unroll
-        for (int r0 = 0; r0 < kStep; r0 += LANES) {
-          const int r = r0 + lane / CH, piece = lane % CH;
-          const bool low = r0 < 16;  // LANES divides 16
-          const long long from_row = (low ? row0 : row1) + r;
-          const bool valid = (low ? p.x : p.y) >= 0;
-          copy16(base + r * S::KP + 16 * piece, c.keys + from_row * W + 16 * piece, valid);
-          copy16(base + kStep * S::KP + r * S::VP + 16 * piece, c.values + from_row * W + 16 * piece, valid);
+        for (int half = 0; half < 2; ++half) {
+          const long long row = half ? row1 : row0;
+          const bool valid = (half ? p.y : p.x) >= 0;
+          const int8_t* k = c.keys + row * W + lane_from;
+          const int8_t* v = c.values + row * W + lane_from;
+#pragma unroll
+          for (int r0 = 0; r0 < 16; r0 += LANES) {
+            const int kind = r0 / LANES % KINDS, group = r0 / LANES / KINDS * KINDS * LANES + 16 * half;
+            copy16(copy_to[kind] + at_stage + group * W, k + r0 * W, valid);
+            copy16(copy_to[kind] + at_stage + (kStep + group) * W, v + r0 * W, valid);
+          }
         }
-        const long long from_row = (lane < 16 ? row0 : row1) + lane;
+        const long long row = lane < 16 ? row0 + lane : row1 + (lane - 16);
         const bool valid = (lane < 16 ? p.x : p.y) >= 0;
-        const unsigned scales = base + kStep * (S::KP + S::VP) + 4 * lane;
-        copy4(scales, c.key_scales + from_row, valid);
-        copy4(scales + 4 * kStep, c.value_scales + from_row, valid);
+        copy4(scale_to + at_stage, c.key_scales + row, valid);
+        copy4(scale_to + at_stage + 4 * kStep, c.value_scales + row, valid);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -406,9 +446,8 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
     for (int step = first; step < end; step += kWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
       __syncwarp();
-      const unsigned char* K = ring + stage * S::STAGE;
-      const unsigned char* V = K + kStep * S::KP;
-      const float* key_scale = reinterpret_cast<const float*>(V + kStep * S::VP);
+      const unsigned rows_at = ring_at + stage * S::STAGE + lane * W;  // of the keys; the values follow
+      const float* key_scale = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * kStep * W);
       const float* value_scale = key_scale + kStep;
       const int position = step * kStep;
       const bool inside = position + kStep <= all && held[0].x >= 0 && held[0].y >= 0;
@@ -421,90 +460,89 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
         for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
           for (int j = 0; j < 4; ++j) sc[h][rn][j] = low[h][rn][j] = 0.f;
-      constexpr int WORDS = W / 16 < 4 ? W / 16 : 4;  // words of a key row a lane reads at once
 #pragma unroll
-      for (int i = 0; i < TILES / WORDS; ++i) {
-        unsigned raw[2][2][WORDS];
+      for (int k = 0; k < TILES; ++k) {
+        unsigned raw[4], ka[2][4];
+        load_rows(rows_at + 16 * piece_at<W>(lane, k), raw);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const unsigned char* p = K + (16 * h + 8 * j + g) * S::KP + l4 * (W / 4) + 4 * WORDS * i;
-            if constexpr (WORDS == 4) {
-              const uint4 x = *reinterpret_cast<const uint4*>(p);
-              raw[h][j][0] = x.x, raw[h][j][1] = x.y, raw[h][j][2] = x.z, raw[h][j][3] = x.w;
-            } else {
-              const uint2 x = *reinterpret_cast<const uint2*>(p);
-              raw[h][j][0] = x.x, raw[h][j][1] = x.y;
-            }
-          }
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-          unsigned ka[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ka[h][0] = codes(raw[h][0][w]), ka[h][1] = codes(raw[h][1][w]);
-            ka[h][2] = codes(raw[h][0][w] >> 8), ka[h][3] = codes(raw[h][1][w] >> 8);
-          }
-#pragma unroll
-          for (int rn = 0; rn < RN; ++rn)
-#pragma unroll
-            for (int part = 0; part < NQ; ++part) {
-              const uint2 qb = queries[((rn * NQ + part) * TILES + i * WORDS + w) * 32 + lane];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) mma(part == 0 ? sc[h][rn] : low[h][rn], ka[h], qb.x, qb.y);
-            }
+        for (int h = 0; h < 2; ++h) {
+          ka[h][0] = codes(raw[2 * h], mask, flip), ka[h][1] = codes(raw[2 * h + 1], mask, flip);
+          ka[h][2] = codes(raw[2 * h] >> 8, mask, flip), ka[h][3] = codes(raw[2 * h + 1] >> 8, mask, flip);
         }
+#pragma unroll
+        for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+          for (int part = 0; part < NQ; ++part) {
+            const uint2 qb = queries[((rn * NQ + part) * TILES + k) * 32 + lane];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mma(part == 0 ? sc[h][rn] : low[h][rn], ka[h], qb.x, qb.y);
+          }
       }
 
-      // scores in units of log2 e, masks
+      // scores in units of log2 e
       float vs[2][2];
-      unsigned seen = 0xffffffffu;  // bit (h RN + rn) 4 + j
-      float top[RN][2];
-#pragma unroll
-      for (int rn = 0; rn < RN; ++rn) top[rn][0] = top[rn][1] = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int key = 16 * h + 8 * k + g;
-          const float ks = key_scale[key];
-          vs[h][k] = value_scale[key];
-          const bool there = (h ? held[0].y : held[0].x) >= 0;
-          const int since = (int)min((long long)position + key - q.start, 1ll << 30);
+          const float ks = key_scale[16 * h + 8 * k + g] * factor;
+          vs[h][k] = value_scale[16 * h + 8 * k + g] * kCodeScale;
 #pragma unroll
           for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float x = sc[h][rn][2 * k + j];
-              if (NQ > 1) x += low[h][rn][2 * k + j];
-              x *= ks;
-              x = a.cap > 0 ? cap2 * tanhf(x * by_cap) : x * scale2;
-              if (!inside) {
-                bool sees = position + key < limit[rn][j];
-                if (a.visible && since >= 0 && since < in_tree) sees = sees || ((bits[rn][j] >> since) & 1);
-                if (!(sees && there)) {
-                  x = -INFINITY;
-                  seen &= ~(1u << ((h * RN + rn) * 4 + 2 * k + j));
-                }
-              }
-              sc[h][rn][2 * k + j] = x;
-              top[rn][j] = fmaxf(top[rn][j], x);
+            for (int j = 2 * k; j < 2 * k + 2; ++j) {
+              if (NQ > 1) sc[h][rn][j] += low[h][rn][j];
+              sc[h][rn][j] *= ks;
             }
         }
-      float keep[RN][2];
+      if (a.cap > 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[h][rn][j] = cap2 * tanhf(sc[h][rn][j]);
+      }
+      unsigned hidden = 0;  // bit (h RN + rn) 4 + j: a score that its row does not see
+      if (!inside) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int key = position + 16 * h + 8 * k + g;
+            const bool there = (h ? held[0].y : held[0].x) >= 0;
+            const int since = (int)min((long long)key - q.start, 1ll << 30);
+            const bool in_call = since >= 0 && since < in_tree;
+#pragma unroll
+            for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const bool sees = key < limit[rn][j] || (in_call && ((bits[rn][j] >> since) & 1));
+                if (sees && there) {
+                  seen_rows |= 1u << (rn * 2 + j);
+                } else {
+                  sc[h][rn][2 * k + j] = -INFINITY;
+                  hidden |= 1u << ((h * RN + rn) * 4 + 2 * k + j);
+                }
+              }
+          }
+      } else {
+        seen_rows = ~0u;
+      }
+      float keep[RN][2], base[RN][2];
       bool moved = false;
 #pragma unroll
       for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float t = top[rn][j];
+          float t = fmaxf(fmaxf(sc[0][rn][j], sc[0][rn][2 + j]), fmaxf(sc[1][rn][j], sc[1][rn][2 + j]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
           const float mn = fmaxf(m[rn][j], t);
           keep[rn][j] = mn == m[rn][j] ? 1.f : exp2_fast(m[rn][j] - mn);
           moved |= mn != m[rn][j];
           m[rn][j] = mn;
+          base[rn][j] = mn == -INFINITY ? 0.f : mn;
           sum[rn][j] *= keep[rn][j];
         }
       constexpr bool FRESH = NP == 3;  // float32 rows: each step's products in accumulators of their own, added in float32
@@ -518,78 +556,62 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
       }
 
       // weights, and the products with the values
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = exp2_fast(sc[h][rn][j] - base[rn][j & 1]);
+            sum[rn][j & 1] += p;
+            sc[h][rn][j] = p * vs[h][j >> 1];
+          }
+      if (hidden) {  // whatever lies there
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if ((hidden >> ((h * RN + rn) * 4 + j)) & 1) sc[h][rn][j] = 0.f;
+      }
       unsigned pb[2][RN][NP][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int rn = 0; rn < RN; ++rn) {
-          float w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float base = m[rn][j & 1] == -INFINITY ? 0.f : m[rn][j & 1];
-            const float p = exp2_fast(sc[h][rn][j] - base);
-            sum[rn][j & 1] += p;
-            w[j] = p * vs[h][j >> 1];
-            const unsigned bit = (seen >> ((h * RN + rn) * 4 + j)) & 1u;
-            if (!inside && !bit) w[j] = 0.f;  // whatever lies there
-            seen_rows |= bit << (rn * 2 + (j & 1));
-          }
           unsigned lo[NP], hi[NP];
-          split<NP>(w[0], w[1], lo);
-          split<NP>(w[2], w[3], hi);
+          split<NP>(sc[h][rn][0], sc[h][rn][1], lo);
+          split<NP>(sc[h][rn][2], sc[h][rn][3], hi);
 #pragma unroll
           for (int part = 0; part < NP; ++part) {
             pb[h][rn][part][0] = transposed(lo[part]);
             pb[h][rn][part][1] = transposed(hi[part]);
           }
         }
-      constexpr int VB = W / 8;                        // bytes of a value row a lane reads
-      constexpr int VW = VB / 4 < 4 ? VB / 4 : 4;      // words at once
 #pragma unroll
-      for (int i = 0; i < VB / 4 / VW; ++i) {
-        unsigned raw[2][4][VW];
+      for (int t = 0; t < TILES; ++t) {
+        unsigned raw[4];
+        float fresh[RN][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int rn = 0; rn < RN; ++rn) fresh[rn][0] = fresh[rn][1] = fresh[rn][2] = fresh[rn][3] = 0.f;
+        load_rows_transposed(rows_at + kStep * W + 16 * piece_at<W>(lane, t), raw);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const unsigned char* p = V + (16 * h + 2 * l4 + (j & 1) + 8 * (j >> 1)) * S::VP + g * VB + 4 * VW * i;
-            if constexpr (VW == 4) {
-              const uint4 x = *reinterpret_cast<const uint4*>(p);
-              raw[h][j][0] = x.x, raw[h][j][1] = x.y, raw[h][j][2] = x.z, raw[h][j][3] = x.w;
-            } else if constexpr (VW == 2) {
-              const uint2 x = *reinterpret_cast<const uint2*>(p);
-              raw[h][j][0] = x.x, raw[h][j][1] = x.y;
-            } else {
-              raw[h][j][0] = *reinterpret_cast<const unsigned*>(p);
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          unsigned va[4];  // tile rows lane / 4 and + 8: columns 16 t + 2 (lane / 4) and the next
+          va[0] = codes(raw[2 * h], mask, flip), va[1] = codes(raw[2 * h] >> 8, mask, flip);
+          va[2] = codes(raw[2 * h + 1], mask, flip), va[3] = codes(raw[2 * h + 1] >> 8, mask, flip);
 #pragma unroll
-        for (int t = 0; t < 2 * VW; ++t) {
-          const int word = t / 2, byte = (t & 1) * 2;
-          const unsigned pick0 = byte * 0x11 + (byte + 4) * 0x1100, pick1 = pick0 + 0x1111;
-          float fresh[RN][4];
+          for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
-          for (int rn = 0; rn < RN; ++rn) fresh[rn][0] = fresh[rn][1] = fresh[rn][2] = fresh[rn][3] = 0.f;
+            for (int part = 0; part < NP; ++part)
+              mma(FRESH ? fresh[rn] : o[rn][t], va, pb[h][rn][part][0], pb[h][rn][part][1]);
+        }
+        if (FRESH) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            unsigned va[4];
-            va[0] = codes(__byte_perm(raw[h][0][word], raw[h][1][word], pick0));
-            va[1] = codes(__byte_perm(raw[h][0][word], raw[h][1][word], pick1));
-            va[2] = codes(__byte_perm(raw[h][2][word], raw[h][3][word], pick0));
-            va[3] = codes(__byte_perm(raw[h][2][word], raw[h][3][word], pick1));
+          for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
-            for (int rn = 0; rn < RN; ++rn)
-#pragma unroll
-              for (int part = 0; part < NP; ++part)
-                mma(FRESH ? fresh[rn] : o[rn][2 * VW * i + t], va, pb[h][rn][part][0], pb[h][rn][part][1]);
-          }
-          if (FRESH) {
-#pragma unroll
-            for (int rn = 0; rn < RN; ++rn)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                o[rn][2 * VW * i + t][j] = fmaf(o[rn][2 * VW * i + t][j], keep[rn][j & 1], fresh[rn][j]);
-          }
+            for (int j = 0; j < 4; ++j) o[rn][t][j] = fmaf(o[rn][t][j], keep[rn][j & 1], fresh[rn][j]);
         }
       }
       __syncwarp();
@@ -620,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
       for (int j = 0; j < 2; ++j) {
         const int r = rn * 8 + 2 * l4 + j;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)  // columns g W / 8 + 2 t + {0, 1}, at 16 t + 2 g
+        for (int t = 0; t < TILES; ++t)
           *reinterpret_cast<float2*>(own + r * S::OP + 16 * t + 2 * g) = make_float2(o[rn][t][j], o[rn][t][2 + j]);
         if (g == 0) {
           // a row that saw nothing has sum 0, one that saw scores of -infinity alone is marked with -1
@@ -646,15 +668,12 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
         f[w] = exp2_fast(ml[w * ROWS * (S::OP + 2)] - base);
         add_sum(&all_sum, ml[w * ROWS * (S::OP + 2) + 1], f[w]);
       }
-      const int col = 4 * quad, lane_of = col / (W / 8), t0 = (col % (W / 8)) / 2;
+      const int col = 4 * quad;
       float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float* from_w = joined + w * ROWS * (S::OP + 2) + r * S::OP + 2 * lane_of;
-        const float2 x = *reinterpret_cast<const float2*>(from_w + 16 * t0);
-        const float2 y = *reinterpret_cast<const float2*>(from_w + 16 * (t0 + 1));
-        v[0] = fmaf(x.x, f[w], v[0]), v[1] = fmaf(x.y, f[w], v[1]);
-        v[2] = fmaf(y.x, f[w], v[2]), v[3] = fmaf(y.y, f[w], v[3]);
+        const float4 x = *reinterpret_cast<const float4*>(joined + w * ROWS * (S::OP + 2) + r * S::OP + col);
+        v[0] = fmaf(x.x, f[w], v[0]), v[1] = fmaf(x.y, f[w], v[1]), v[2] = fmaf(x.z, f[w], v[2]), v[3] = fmaf(x.w, f[w], v[3]);
       }
       if (complete) {
 #pragma unroll
