@@ -146,6 +146,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// float32 rows take CUDA's tanh (a few units in the last place). For 16-bit rows 1 - 2 / (1 + e^2x) is near enough: off
+// by 2^-22 of the cap, where a row's own rounding is 2^-9 or 2^-12 of its value, and a
+// third of the instructions.
+template <typename T>
+__device__ __forceinline__ float tanh_of(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  return 1.f - __fdividef(2.f, 1.f + exp2_fast(2.885390081777927f * x));
+}
+
 // Two floats as N pairs of bfloat16 whose sums they are: the leading 8 bits cut off N - 1 times (exact
 // remainders), the rest rounded.
 template <int N>
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
 #pragma unroll
           for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[h][rn][j] = cap2 * tanhf(sc[h][rn][j]);
+            for (int j = 0; j < 4; ++j) sc[h][rn][j] = cap2 * tanh_of<T>(sc[h][rn][j]);
       }
       unsigned hidden = 0;  // bit (h RN + rn) 4 + j: a score that its row does not see
       if (!inside) {
@@ -695,38 +704,57 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
 }
 
 // Joins the parts of the unit that begins in CTA blockIdx.x of `attend` and was cut at its end, in the
-// order of the keys.
+// order of the keys: a warp per row, first the parts' maxima and sums (a lane per part), then the
+// weighted sums (a lane per four columns), eight parts' loads in flight. One thread per four columns that
+// walked all parts twice took 22 us for 28 parts of 8 units; this takes 4.
 template <typename T, int W, int RN>
 __global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, const Args a) {
-  constexpr int ROWS = 8 * RN, QUADS = W / 4;
+  constexpr int ROWS = 8 * RN, QUADS = W / 4, PER = (QUADS + 31) / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 cut = a.cuts[blockIdx.x];
   if (cut.x < 0) return;
   const Sequence q = sequence_of<ROWS>(b, a, cut.x);
-  const int rows = min(ROWS, q.rows * a.group - cut.z * ROWS);
-  const bool wide = out_wide<T>(a);
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= q.rows * a.group - cut.z * ROWS) return;
   const int n = cut.w - blockIdx.x + 1;
   auto part = [&](int i) { return a.parts + (i == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + i)) * ROWS * (W + 2); };
-  for (int i = threadIdx.x; i < rows * QUADS; i += 256) {
-    const int r = i / QUADS, col = 4 * (i - r * QUADS);
-    float mm = -INFINITY, all_sum = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) mm = fmaxf(mm, part(k)[ROWS * W + 2 * r]);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float* p = part(k);
-      const float2 ml = *reinterpret_cast<const float2*>(p + ROWS * W + 2 * r);
-      const float4 x = *reinterpret_cast<const float4*>(p + r * W + col);
-      const float f = exp2_fast(ml.x - base);
-      add_sum(&all_sum, ml.y, f);
-      v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
-    }
+  float mm = -INFINITY;
+  for (int k = lane; k < n; k += 32) mm = fmaxf(mm, part(k)[ROWS * W + 2 * r]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = answer(v[j], all_sum);
-    store4<T>(out_row<T>(a, q, cut.y, cut.z * ROWS + r) + col, v, wide);
+  for (int x = 1; x < 32; x <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float all_sum = 0.f, v[PER][4];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    float mine = 0.f, weights = 0.f;
+    if (k0 + lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(k0 + lane) + ROWS * W + 2 * r);
+      mine = exp2_fast(ml.x - base), weights = ml.y;
+    }
+    const int some = min(32, n - k0);
+#pragma unroll 8
+    for (int k = 0; k < some; ++k) {
+      const float f = __shfl_sync(0xffffffffu, mine, k);
+      add_sum(&all_sum, __shfl_sync(0xffffffffu, weights, k), f);
+      const float* p = part(k0 + k) + r * W;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (QUADS >= 32 || lane < QUADS) {
+          const float4 x = *reinterpret_cast<const float4*>(p + 4 * (lane + 32 * i));
+          v[i][0] = fmaf(x.x, f, v[i][0]), v[i][1] = fmaf(x.y, f, v[i][1]);
+          v[i][2] = fmaf(x.z, f, v[i][2]), v[i][3] = fmaf(x.w, f, v[i][3]);
+        }
+    }
   }
+  const bool wide = out_wide<T>(a);
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (QUADS >= 32 || lane < QUADS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = answer(v[i][j], all_sum);
+      store4<T>(out_row<T>(a, q, cut.y, cut.z * ROWS + r) + 4 * (lane + 32 * i), v[i], wide);
+    }
 }
 
 // Row tiles of 8 a unit takes: as many as the call's sequences have rows on average, since a unit
@@ -770,7 +798,7 @@ int launch(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
   if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
   if (a.whole) return TGCB_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(grid, RN);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

@@ -143,6 +143,218 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
   }
 }
 
+// Rows of 16-byte vectors. A group of `lanes` threads has one row: thread i of it holds two vectors, which in the turned
+// columns are the two halves of its pairs (or, interleaved, two neighbouring vectors), so that a
+// pair never leaves its thread. A CTA takes `tokens_each` tokens with `groups[side]` groups a side for each, every
+// group always on the same side and columns; the cosines of its tokens are computed once for all
+// heads, into shared memory, while the rows are on their way.
+//
+// Bound by HBM: each row is read and written once (backward: two read, one written). 8192
+// tokens of 32 + 8 bfloat16 heads of 128: forward 168 MB, backward 252 MB.
+constexpr int kVecThreads = 512;
+
+struct Layout {
+  int lanes_log, groups[2], tokens_each, passes, threads;
+  size_t shared;
+};
+
+template <typename T, bool INTERLEAVED, bool BACKWARD>
+__global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vectors(const Params p, const Layout layout) {
+  constexpr int V = Vec<T>::N;
+  // gains [side][width], then cosines and sines [2 buffers][tokens_each][cos, sin][half]; at the end the sums
+  extern __shared__ __align__(16) float shared[];
+  const int half = p.rotary / 2, lanes = 1 << layout.lanes_log, per_token = layout.groups[0] + layout.groups[1];
+  const int group = threadIdx.x >> layout.lanes_log, item = threadIdx.x & (lanes - 1);
+  const int token_in = group / per_token, in_token = group - token_in * per_token;
+  const int which = in_token >= layout.groups[0];
+  const Side& s = p.side[which];
+  const int head0 = which ? in_token - layout.groups[0] : in_token, heads_step = layout.groups[which];
+  const bool working = token_in < layout.tokens_each;
+
+  // this thread's columns a and b, V of each, and the first of the frequencies that turn them (-1: none)
+  int a, b, turn_a, turn_b;
+  if (INTERLEAVED) {
+    a = 2 * item * V, b = a + V;
+    turn_a = a < p.rotary ? a / 2 : -1, turn_b = b < p.rotary ? b / 2 : -1;
+  } else {
+    const int pairs = half / V;
+    const bool paired = item < pairs;
+    a = paired ? item * V : p.rotary + 2 * (item - pairs) * V;
+    b = paired ? half + item * V : a + V;
+    turn_a = turn_b = paired ? item * V : -1;
+  }
+  const bool has_a = working && a < p.width, has_b = working && b < p.width;
+  float sum_a[V], sum_b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum_a[i] = sum_b[i] = 0.f;
+  for (int i = threadIdx.x; i < 2 * p.width; i += blockDim.x)
+    shared[i] = load_any(p.side[i >= p.width].gain, p.gain_dtype, i >= p.width ? i - p.width : i);
+  const float* gain_a = shared + which * p.width + (has_a ? a : 0);
+  const float* gain_b = shared + which * p.width + (has_b ? b : 0);
+  float* all_angles = shared + 2 * p.width;
+
+  int buffer = 0;
+  for (long long tile = blockIdx.x; tile * layout.tokens_each < p.tokens; tile += gridDim.x, buffer ^= 1) {
+    const long long token0 = tile * layout.tokens_each, token = token0 + token_in;
+    float* angles = all_angles + buffer * layout.tokens_each * p.rotary;
+    for (int pass = 0; pass < layout.passes; ++pass) {
+      const int head = head0 + pass * heads_step;
+      const bool row = token < p.tokens && head < s.heads;
+      const T* x = static_cast<const T*>(s.in) + token * s.in_t + head * s.in_h;
+      const T* d = BACKWARD ? static_cast<const T*>(s.grad) + token * s.grad_t + head * s.grad_h : nullptr;
+      T* y = static_cast<T*>(s.out) + token * s.out_t + head * s.out_h;
+      Vec<T> xa, xb, da, db;
+      xa.raw = xb.raw = da.raw = db.raw = make_uint4(0, 0, 0, 0);
+      if (row && has_a) xa.raw = *reinterpret_cast<const uint4*>(x + a);
+      if (row && has_b) xb.raw = *reinterpret_cast<const uint4*>(x + b);
+      if (BACKWARD) {
+        if (row && has_a) da.raw = *reinterpret_cast<const uint4*>(d + a);
+        if (row && has_b) db.raw = *reinterpret_cast<const uint4*>(d + b);
+      }
+      if (pass == 0) {
+        for (int i = threadIdx.x; i < layout.tokens_each * half; i += blockDim.x) {
+          const int t = i / half, f = i - t * half;
+          if (token0 + t < p.tokens) turn(position_of(p, token0 + t), p.frequencies[f], angles + t * p.rotary + f, angles + t * p.rotary + half + f);
+        }
+        __syncthreads();  // the other buffer's readers are past it too, so the next tile may fill that one
+      }
+      // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
+      const float* cs = angles + (working ? token_in : 0) * p.rotary;
+      float fa[V], fb[V], square = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        fa[i] = to_float(xa.e[i]), fb[i] = to_float(xb.e[i]);
+        square = fmaf(fa[i], fa[i], square);
+        square = fmaf(fb[i], fb[i], square);
+      }
+      if (!BACKWARD) {
+        for (int o = lanes >> 1; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+        const float r = 1.f / sqrtf(square / (float)p.width + p.epsilon);
+#pragma unroll
+        for (int i = 0; i < V; ++i) fa[i] = fa[i] * r * gain_a[i], fb[i] = fb[i] * r * gain_b[i];
+        if (!INTERLEAVED) {
+          if (turn_a >= 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = fa[i], v = fb[i];
+              fa[i] = u * c - v * n, fb[i] = u * n + v * c;
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            if (turn_a >= 0) {
+              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = fa[2 * i], v = fa[2 * i + 1];
+              fa[2 * i] = u * c - v * n, fa[2 * i + 1] = u * n + v * c;
+            }
+            if (turn_b >= 0) {
+              const float c = cs[turn_b + i], n = cs[half + turn_b + i], u = fb[2 * i], v = fb[2 * i + 1];
+              fb[2 * i] = u * c - v * n, fb[2 * i + 1] = u * n + v * c;
+            }
+          }
+        }
+        if (row && has_a) store_vec<T>(y + a, fa);
+        if (row && has_b) store_vec<T>(y + b, fb);
+      } else {
+        float ga[V], gb[V], ex = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ga[i] = to_float(da.e[i]), gb[i] = to_float(db.e[i]);
+        if (!INTERLEAVED) {
+          if (turn_a >= 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = ga[i], v = gb[i];
+              ga[i] = u * c + v * n, gb[i] = v * c - u * n;
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            if (turn_a >= 0) {
+              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = ga[2 * i], v = ga[2 * i + 1];
+              ga[2 * i] = u * c + v * n, ga[2 * i + 1] = v * c - u * n;
+            }
+            if (turn_b >= 0) {
+              const float c = cs[turn_b + i], n = cs[half + turn_b + i], u = gb[2 * i], v = gb[2 * i + 1];
+              gb[2 * i] = u * c + v * n, gb[2 * i + 1] = v * c - u * n;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          ex = fmaf(ga[i] * gain_a[i], fa[i], ex);
+          ex = fmaf(gb[i] * gain_b[i], fb[i], ex);
+        }
+        for (int o = lanes >> 1; o > 0; o >>= 1) {
+          square += __shfl_xor_sync(0xffffffffu, square, o);
+          ex += __shfl_xor_sync(0xffffffffu, ex, o);
+        }
+        const float r = 1.f / sqrtf(square / (float)p.width + p.epsilon), m = ex * r * r / (float)p.width;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (row) {
+            sum_a[i] = fmaf(ga[i] * r, fa[i], sum_a[i]);
+            sum_b[i] = fmaf(gb[i] * r, fb[i], sum_b[i]);
+          }
+          fa[i] = r * (ga[i] * gain_a[i] - fa[i] * m);
+          fb[i] = r * (gb[i] * gain_b[i] - fb[i] * m);
+        }
+        if (row && has_a) store_vec<T>(y + a, fa);
+        if (row && has_b) store_vec<T>(y + b, fb);
+      }
+    }
+  }
+  if (BACKWARD) {  // this CTA's gain gradients: the groups of a side added up in order
+    __syncthreads();
+    const int groups = layout.tokens_each * per_token;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (has_a) shared[group * p.width + a + i] = sum_a[i];
+      if (has_b) shared[group * p.width + b + i] = sum_b[i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * p.width; c += blockDim.x) {
+      const int side = c >= p.width, column = c - side * p.width;
+      float v = 0.f;
+      for (int g = 0; g < groups; ++g)
+        if ((g % per_token >= layout.groups[0]) == (side == 1)) v += shared[g * p.width + column];
+      p.partials[(long long)blockIdx.x * 2 * p.width + c] = v;
+    }
+  }
+}
+
+// Whether the vector kernel takes these rows, and how. Other rows (widths that are no multiple of 16 bytes, odd halves,
+// rows off a 16-byte boundary) take norm_rotate_rows: the same 8192 tokens there in 150 us forward and 519 us backward.
+template <typename T>
+bool vectors(const Params& p, bool backward, Layout* out) {
+  constexpr int V = Vec<T>::N;
+  const int half = p.rotary / 2;
+  if (p.width % V || (p.interleaved ? p.rotary % V : half % V)) return false;
+  auto whole = [](const void* data, long long t, long long h) {
+    return ((reinterpret_cast<uintptr_t>(data) | (unsigned long long)(t * (long long)sizeof(T)) | (unsigned long long)(h * (long long)sizeof(T))) & 15u) == 0;
+  };
+  for (const Side& s : p.side)
+    if (!whole(s.in, s.in_t, s.in_h) || !whole(s.out, s.out_t, s.out_h) || (backward && !whole(s.grad, s.grad_t, s.grad_h))) return false;
+  const int single = p.width / V, items = p.interleaved ? (single + 1) / 2 : half / V + (single - p.rotary / V + 1) / 2;
+  Layout l = {};
+  while ((1 << l.lanes_log) < items) ++l.lanes_log;
+  if (l.lanes_log > 5) return false;
+  const int most = kVecThreads >> l.lanes_log;
+  for (l.passes = 1;; ++l.passes) {
+    for (int i = 0; i < 2; ++i) l.groups[i] = (p.side[i].heads + l.passes - 1) / l.passes;
+    if (l.groups[0] + l.groups[1] <= most) break;
+  }
+  // several tokens a CTA where one has few heads and there are CTAs enough
+  const int per_token = l.groups[0] + l.groups[1];
+  l.tokens_each = 1;
+  while (2 * l.tokens_each * per_token <= most / 2 && p.tokens / (2 * l.tokens_each) >= 148 * 8) l.tokens_each *= 2;
+  l.threads = ((l.tokens_each * per_token << l.lanes_log) + 31) / 32 * 32;
+  l.shared = (2ull * p.width + 2ull * l.tokens_each * p.rotary) * sizeof(float);
+  const size_t sums = backward ? (size_t)(l.threads >> l.lanes_log) * p.width * sizeof(float) : 0;
+  if (sums > l.shared) l.shared = sums;
+  if (l.shared > 48 * 1024) return false;
+  *out = l;
+  return true;
+}
+
 // The gain gradients: column sums of the CTAs' partial rows, in float64 and in a fixed order.
 __global__ void __launch_bounds__(256) gain_sums(const Params p, int partials) {
   __shared__ double part[8][33];
@@ -202,8 +414,29 @@ Params params_of(const tgcb_rotary_desc* d) {
   return p;
 }
 
+template <typename T, bool INTERLEAVED>
+unsigned run_vectors(const Params& p, const Layout& l, bool backward, cudaStream_t s) {
+  const long long tiles = (p.tokens + l.tokens_each - 1) / l.tokens_each;
+  if (!backward) {
+    const unsigned grid = (unsigned)(tiles < 0x7fffffffll ? tiles : 0x7fffffffll);
+    norm_rotate_vectors<T, INTERLEAVED, false><<<grid, l.threads, l.shared, s>>>(p, l);
+    return grid;
+  }
+  const unsigned grid = (unsigned)(tiles < kPartials ? tiles : kPartials);
+  norm_rotate_vectors<T, INTERLEAVED, true><<<grid, l.threads, l.shared, s>>>(p, l);
+  return grid;
+}
+
 template <typename T>
 int run(const Params& p, bool backward, cudaStream_t s) {
+  Layout l;
+  if (p.tokens > 0 && vectors<T>(p, backward, &l)) {
+    const unsigned grid = p.interleaved ? run_vectors<T, true>(p, l, backward, s) : run_vectors<T, false>(p, l, backward, s);
+    if (backward) gain_sums<<<(2 * p.width + 31) / 32, 256, 0, s>>>(p, (int)grid);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "norm_rotate", cudaGetErrorString(e));
+    return TGCB_OK;
+  }
   const long long rows = p.tokens * (p.side[0].heads + p.side[1].heads);
   const long long ctas = (rows + kRowWarps - 1) / kRowWarps;
   if (!backward) {
