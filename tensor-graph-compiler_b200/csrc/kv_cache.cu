@@ -17,7 +17,6 @@ namespace {
 using namespace tgcb_elem;
 using tgcb_kv::Batch;
 using tgcb_kv::Cache;
-using tgcb_kv::Place;
 
 struct Rows {
   char* data;
@@ -25,72 +24,250 @@ struct Rows {
 };
 
 constexpr int kThreads = 256;
+constexpr int kTokens = 8;  // tokens a CTA takes at most
 
-// One CTA per token, a warp per row of it.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values) {
-  __shared__ Place place;
-  __shared__ int later;
-  const long long token = blockIdx.x;
-  if (threadIdx.x == 0) later = 0, place.sequence = -1;
-  __syncthreads();
-  tgcb_kv::find(c, b, token, &place);
-  __syncthreads();
-  if (place.sequence < 0 || place.page < 0) return;
-  tgcb_kv::find_later(c, b, token, place, &later);
-  __syncthreads();
-  if (later) return;
+// Where a token row lies: its sequence (-1: none), and the page and place of its position
+// (page -1: the position or the table's entry is out of range).
+struct Place {
+  int sequence, page, row;
+};
+
+// The places of token rows [token0, token0 + count), by the whole CTA; a barrier must follow. Each thread
+// looks at its share of the sequences for the rows that are theirs.
+__device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long long token0, int count, Place* places) {
+  auto fill = [&](int s, long long first, long long token) {
+    const long long position = (long long)__ldg(b.starts + s) + token - first;
+    const int page = tgcb_kv::page_of(c, b, s, position);
+    if (page < 0) atomicAdd(c.faults, 1);
+    places[token - token0] = Place{s, page, (int)(position & (c.page - 1))};
+  };
+  if (b.offsets == nullptr) {
+    if (threadIdx.x < count) {
+      const int s = (int)((token0 + threadIdx.x) / b.each);
+      fill(s, (long long)s * b.each, token0 + threadIdx.x);
+    }
+    return;
+  }
+  for (int s = threadIdx.x; s < b.batch; s += kThreads) {
+    long long first, last;
+    tgcb_kv::range_of(b, s, &first, &last);
+    for (long long t = first > token0 ? first : token0; t < last && t < token0 + count; ++t) fill(s, first, t);
+  }
+}
+
+// later[i] becomes 1 where a later row of the call has row i's place: two sequences that share a page both
+// write to, or a page twice in one table row. The call's written pages are few beside its rows; a
+// thread takes a sequence, and a sequence of many pages is taken by its warp.
+__device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long long token0, int count, const Place* places, int* later) {
   const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < 2 * c.heads; r += kThreads / 32) {
-    const bool value = r >= c.heads;
-    const int h = value ? r - c.heads : r;
-    const Rows& rows = value ? values : keys;
-    const T* x = reinterpret_cast<const T*>(rows.data) + token * rows.t + h * rows.h;
-    unsigned m = 0;
-    for (int i = lane; i < c.width; i += 32) m = max(m, __float_as_uint(to_float(x[i])) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float largest = __uint_as_float(m);
-    const float scale = largest == 0.0f ? 1.0f : (float)((double)largest / 127.0);
-    const long long at = ((long long)place.page * c.heads + h) * c.page + place.row;
-    if (lane == 0) (value ? c.value_scales : c.key_scales)[at] = scale;
-    int8_t* q = (value ? c.values : c.keys) + at * c.width;
-    for (int i = lane; i < c.width; i += 32) {
-      const float t = fminf(fmaxf(rintf(__fdiv_rn(to_float(x[i]), scale)), -128.0f), 127.0f);
-      q[i] = (int8_t)(int)t;
+  int least = b.batch;
+  for (int i = 0; i < count; ++i)
+    if (places[i].sequence >= 0 && places[i].sequence < least) least = places[i].sequence;
+  auto look = [&](int s, long long slot, long long first, long long last, long long start) {
+    const int page = __ldg(b.table + s * b.table_stride + slot);
+    for (int i = 0; i < count; ++i) {
+      const long long at = first + (slot << c.page_bits) + places[i].row - start;
+      if (page == places[i].page && at > token0 + i && at >= first && at < last && places[i].sequence >= 0) later[i] = 1;
+    }
+  };
+  for (int s0 = least + (threadIdx.x & ~31); s0 < b.batch; s0 += kThreads) {
+    const int s = s0 + lane;
+    long long first = 0, last = 0, start = 0, slot = 0, end = 0;
+    if (s < b.batch) {
+      tgcb_kv::range_of(b, s, &first, &last);
+      start = __ldg(b.starts + s);
+      if (last > first && start + last - first > 0) {
+        slot = start < 0 ? 0 : start >> c.page_bits;
+        end = ((start + last - first - 1) >> c.page_bits) + 1;
+        end = end > b.max_pages ? b.max_pages : end;
+      }
+    }
+    const long long own = slot + 4 < end ? slot + 4 : end;
+    for (; slot < own; ++slot) look(s, slot, first, last, start);
+    unsigned more = __ballot_sync(0xffffffffu, slot < end);
+    while (more) {
+      const int from = __ffs(more) - 1;
+      more &= more - 1;
+      const long long f = __shfl_sync(0xffffffffu, first, from), l = __shfl_sync(0xffffffffu, last, from);
+      const long long st = __shfl_sync(0xffffffffu, start, from), e = __shfl_sync(0xffffffffu, end, from);
+      for (long long k = __shfl_sync(0xffffffffu, slot, from) + lane; k < e; k += 32) look(s0 + from, k, f, l, st);
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch b, const Rows keys, const Rows values) {
-  __shared__ Place place;
-  const long long token = blockIdx.x;
-  if (threadIdx.x == 0) place.sequence = -1;
+// Eight values of a row, a thread's share of it.
+template <typename T, bool WHOLE>
+struct Eight {
+  static constexpr int N = 8 * sizeof(T) / 16;
+  union {
+    uint4 raw[N];
+    T e[8];
+  };
+  __device__ Eight() {}
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = e[i];
+    }
+  }
+};
+
+// Bound by HBM: append reads a row and writes width + 4 bytes, read the reverse. A thread has eight values
+// of a row, width / 8 threads a row; a CTA takes up to kTokens tokens with all their heads, keys then
+// values, and has the values of kAhead rounds on their way at once. WHOLE: rows are 16-byte aligned.
+constexpr int kAhead = 4;
+
+// Codes of eight values: rint(x / scale). x * (1 / scale) is off by 2^-22 of the quotient at most, so
+// away from half-integers (3e-5) it rounds as the quotient does, and near them the quotient
+// decides. With a finite maximum and reciprocal |x / scale| <= 127 (1 + 2^-21): no clamp; other rows
+// divide and clamp. Adding 1.5 2^23 rounds to an integer, ties to even, in the sum's low bits.
+__device__ __forceinline__ uint2 codes_of(const float* x, float largest, float scale) {
+  const float inverse = __fdiv_rn(1.0f, scale);
+  unsigned q[8];
+  if (isfinite(inverse) && isfinite(largest)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = x[i] * inverse, rounded = t + 12582912.0f;
+      const float off = fabsf(t - (rounded - 12582912.0f));
+      q[i] = __float_as_uint(rounded);
+      if (off >= 0.49997f) q[i] = __float_as_uint(__fdiv_rn(x[i], scale) + 12582912.0f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = (unsigned)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -128.0f), 127.0f);
+  }
+  uint2 r;
+  r.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  r.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+  return r;
+}
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
+                                                        int lanes_log) {
+  __shared__ Place places[kTokens];
+  __shared__ int later[kTokens];
+  const long long token0 = (long long)blockIdx.x * each;
+  const int count = (int)min((long long)each, b.tokens - token0);
+  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
+  const int rows_at_once = kThreads >> lanes_log, rows = count * 2 * c.heads;
+  if (threadIdx.x < kTokens) places[threadIdx.x].sequence = -1, later[threadIdx.x] = 0;
+
+  for (int row0 = 0; row0 < rows; row0 += kAhead * rows_at_once) {
+    Eight<T, WHOLE> x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int row = row0 + i * rows_at_once + group;
+      if (row < rows) {
+        const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
+        const Rows& from = r >= c.heads ? values : keys;
+        x[i].load(reinterpret_cast<const T*>(from.data) + (token0 + token) * from.t + (r >= c.heads ? r - c.heads : r) * from.h + 8 * item);
+      }
+    }
+    if (row0 == 0) {
+      __syncthreads();
+      find_places(c, b, token0, count, places);
+      __syncthreads();
+      find_later(c, b, token0, count, places, later);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int row = row0 + i * rows_at_once + group;
+      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
+      float v[8];
+      unsigned m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = to_float(x[i].e[j]);
+        m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);  // the order of magnitudes, NaN above infinity
+      }
+      for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (row >= rows || places[token].sequence < 0 || places[token].page < 0 || later[token]) continue;
+      const bool value = r >= c.heads;
+      const float largest = __uint_as_float(m);
+      // float(double(largest) / 127) of the rule: a quotient of 24-bit numbers rounded to 53 bits on the
+      // way is never moved to another float32 by it
+      const float scale = largest == 0.0f ? 1.0f : __fdiv_rn(largest, 127.0f);
+      const long long at = ((long long)places[token].page * c.heads + (value ? r - c.heads : r)) * c.page + places[token].row;
+      *reinterpret_cast<uint2*>((value ? c.values : c.keys) + at * c.width + 8 * item) = codes_of(v, largest, scale);
+      if (item == 0) (value ? c.value_scales : c.key_scales)[at] = scale;
+    }
+  }
+}
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
+                                                      int lanes_log) {
+  __shared__ Place places[kTokens];
+  const long long token0 = (long long)blockIdx.x * each;
+  const int count = (int)min((long long)each, b.tokens - token0);
+  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
+  const int rows_at_once = kThreads >> lanes_log, rows = count * 2 * c.heads;
+  if (threadIdx.x < kTokens) places[threadIdx.x].sequence = -1;
   __syncthreads();
-  tgcb_kv::find(c, b, token, &place);
+  find_places(c, b, token0, count, places);
   __syncthreads();
-  if (place.sequence < 0) return;
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < 2 * c.heads; r += kThreads / 32) {
-    const bool value = r >= c.heads;
-    const int h = value ? r - c.heads : r;
-    const Rows& rows = value ? values : keys;
-    T* x = reinterpret_cast<T*>(rows.data) + token * rows.t + h * rows.h;
-    const long long at = ((long long)place.page * c.heads + h) * c.page + place.row;
-    const float scale = place.page < 0 ? __int_as_float(0x7fffffff) : (value ? c.value_scales : c.key_scales)[at];
-    const int8_t* q = (value ? c.values : c.keys) + at * c.width;
-    for (int i = lane; i < c.width; i += 32) x[i] = from_float<T>(place.page < 0 ? scale : (float)q[i] * scale);
+  for (int row0 = 0; row0 < rows; row0 += kAhead * rows_at_once) {
+    uint2 q[kAhead];
+    float scale[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int row = row0 + i * rows_at_once + group;
+      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
+      q[i] = make_uint2(0, 0);
+      scale[i] = __int_as_float(0x7fffffff);
+      if (row < rows && places[token].sequence >= 0 && places[token].page >= 0) {
+        const bool value = r >= c.heads;
+        const long long at = ((long long)places[token].page * c.heads + (value ? r - c.heads : r)) * c.page + places[token].row;
+        q[i] = *reinterpret_cast<const uint2*>((value ? c.values : c.keys) + at * c.width + 8 * item);
+        scale[i] = (value ? c.value_scales : c.key_scales)[at];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int row = row0 + i * rows_at_once + group;
+      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
+      if (row >= rows || places[token].sequence < 0) continue;
+      Eight<T, WHOLE> x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int code = (int)(signed char)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
+        x.e[j] = from_float<T>((float)code * scale[i]);
+      }
+      const Rows& to = r >= c.heads ? values : keys;
+      x.store(reinterpret_cast<T*>(to.data) + (token0 + token) * to.t + (r >= c.heads ? r - c.heads : r) * to.h + 8 * item);
+    }
   }
 }
 
 template <typename T>
 int run(const Cache& c, const Batch& b, const Rows& k, const Rows& v, bool read, cudaStream_t s) {
   if (b.tokens == 0) return TGCB_OK;
+  // one token a CTA while there are few
+  const int each = b.tokens <= 148 * 8 ? 1 : kTokens;
+  const unsigned grid = (unsigned)((b.tokens + each - 1) / each);
+  const int lanes_log = __builtin_ctz((unsigned)c.width / 8);
+  bool whole = true;
+  for (const Rows& r : {k, v})
+    whole = whole && ((reinterpret_cast<uintptr_t>(r.data) | (unsigned long long)(r.t * (long long)sizeof(T)) |
+                       (unsigned long long)(r.h * (long long)sizeof(T))) & 15u) == 0;
   if (read)
-    read_rows<T><<<(unsigned)b.tokens, kThreads, 0, s>>>(c, b, k, v);
+    (whole ? read_rows<T, true> : read_rows<T, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each, lanes_log);
   else
-    append_rows<T><<<(unsigned)b.tokens, kThreads, 0, s>>>(c, b, k, v);
+    (whole ? append_rows<T, true> : append_rows<T, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each, lanes_log);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "kv_cache", cudaGetErrorString(e));
   return TGCB_OK;

@@ -105,15 +105,15 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
     if not isinstance(cache, kv_cache.QuantisedCache):
         raise ConfigError("cached_attention reads a QuantisedCache")
     heads.check_rows("queries", queries)
-    device = cache.device
-    if queries.device != device:
-        raise ConfigError(f"queries must be on {device}, where the cache is")
+    index = cache.index
+    if queries.get_device() != index:
+        raise ConfigError(f"queries must be on {cache.device}, where the cache is")
     tokens, q_heads, width = queries.shape
     if width != cache.width or q_heads < 1 or q_heads % cache.kv_heads:
         raise ConfigError(f"queries must be [tokens, a multiple of {cache.kv_heads} heads, {cache.width}], got {tuple(queries.shape)}")
-    b = kv_cache.batch_of(table, starts, offsets, tokens, device)
+    b = cache.batch_of(table, starts, offsets, tokens)
     if visible is not None:
-        heads.check_vector("visible", visible, tokens, (torch.int64,), device)
+        heads.check_vector("visible", visible, tokens, (torch.int64,), index)
         if offsets is None and tokens > 64 * table.shape[0]:
             raise ConfigError(f"a tree has at most 64 tokens, got {tokens // table.shape[0]} a sequence")
     scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
@@ -128,14 +128,15 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
         heads.check_apart("out", out, "queries", queries)
     lib = _lib.load()
     need = lib.tgcb_cached_attention_scratch_bytes(cache.desc, b, q_heads)
-    with heads.on_stream(device, stream):
+    with heads.on_stream(index, stream):
         if out is None:
-            out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with heads.on_device(device):
+            out = queries.new_empty(queries.shape)
+        scratch = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    with heads.on_device(index):
         rc = lib.tgcb_cached_attention(
-            cache.desc, b, heads.DTYPES[queries.dtype], q_heads, heads.rows(queries), visible.data_ptr() if visible is not None else None,
-            scale, cap, heads.rows(out), scratch.data_ptr() if need else None, need, heads.raw(device, stream),
+            cache.desc, b, heads.DTYPES[queries.dtype], q_heads, _lib.Heads(*heads.rows(queries)),
+            visible.data_ptr() if visible is not None else None, scale, cap, _lib.Heads(*heads.rows(out)),
+            scratch.data_ptr() if need else None, need, heads.raw(index, stream),
         )
     _lib.check(rc, "tgcb_cached_attention")
     return out

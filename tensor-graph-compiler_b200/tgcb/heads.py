@@ -24,14 +24,15 @@ def check_rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> 
         raise ConfigError(f"{name} must be a CUDA tensor [tokens, heads, width] in float32, bfloat16 or float16")
     if t.stride(2) != 1 and t.shape[2] != 1:
         raise ConfigError(f"{name} must have a unit stride along its width")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ConfigError(f"{name} must have the type and device of the other rows")
 
 
-def check_vector(name: str, t: torch.Tensor, length: int, dtypes: tuple, device: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype not in dtypes:
-        raise ConfigError(f"{name} must be a tensor on {device} in {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != 1 or t.shape[0] != length or (length > 1 and t.stride(0) != 1):
+def check_vector(name: str, t: torch.Tensor, length: int, dtypes: tuple, index: int) -> None:
+    """A contiguous vector on CUDA device ``index``."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype not in dtypes:
+        raise ConfigError(f"{name} must be a tensor on cuda:{index} in {' or '.join(str(d) for d in dtypes)}")
+    if t.shape != (length,) or not t.is_contiguous():
         raise ConfigError(f"{name} must be a contiguous vector of {length}, got {tuple(t.shape)}")
 
 
@@ -73,25 +74,27 @@ def check_apart(name: str, out: torch.Tensor, other_name: str, other: torch.Tens
         raise ConfigError(f"{name} overlaps {other_name}")
 
 
-def rows(t: torch.Tensor) -> _lib.Heads:
-    return _lib.Heads(t.data_ptr(), t.stride(0), t.stride(1))
+def rows(t: torch.Tensor) -> tuple[int, int, int]:
+    """The fields of a ``_lib.Heads``."""
+    token, head, _ = t.stride()
+    return t.data_ptr(), token, head
 
 
-def on_device(device: torch.device):
-    """A context in which `device` is current, and set up."""
-    index = device.index
+def on_device(index: int):
+    """A context in which CUDA device ``index`` is current, and set up."""
     _lib.ensure_device(index)
-    return _here if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _here if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-def on_stream(device: torch.device, stream):
-    """A context in which `stream` (None: the current one) is current, for what a call allocates."""
+def on_stream(index: int, stream):
+    """A context in which ``stream`` (None: the current one) is current, for what a call allocates."""
     if stream is None:
         return _here
-    if stream.device != device:
-        raise ConfigError(f"the stream is on {stream.device}, the tensors on {device}")
+    if stream.device.index != index:
+        raise ConfigError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
     return torch.cuda.stream(stream)
 
 
-def raw(device: torch.device, stream) -> int:
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+def raw(index: int, stream) -> int:
+    """The handle of ``stream``, or of the device's current one (its number alone: a Stream object costs microseconds)."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)

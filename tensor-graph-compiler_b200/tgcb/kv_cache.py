@@ -23,24 +23,26 @@ from tgcb.errors import ConfigError
 PAGES = (16, 32, 64, 128)
 WIDTHS = (32, 64, 128, 256)
 MAX_BATCH = 4096
+MAX_POSITIONS = 1 << 30
+_INT32 = (torch.int32,)
 
 
-def batch_of(table: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor | None, tokens: int, device: torch.device) -> _lib.BatchDesc:
-    """The checked description of a call's sequences."""
-    if not isinstance(table, torch.Tensor) or table.device != device or table.dtype != torch.int32 or table.dim() != 2:
-        raise ConfigError(f"the page table must be an int32 matrix [batch, pages] on {device}")
+def batch_of(table: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor | None, tokens: int, index: int) -> _lib.BatchDesc:
+    """The checked description of a call's sequences, on CUDA device ``index``."""
+    if not isinstance(table, torch.Tensor) or table.get_device() != index or table.dtype is not torch.int32 or table.dim() != 2:
+        raise ConfigError(f"the page table must be an int32 matrix [batch, pages] on cuda:{index}")
     batch, pages = table.shape
-    if not 1 <= batch <= MAX_BATCH or pages < 1 or pages > 1 << 24:
-        raise ConfigError(f"a call takes 1 to {MAX_BATCH} sequences of 1 to 2^24 pages, got {batch} of {pages}")
-    if pages > 1 and table.stride(1) != 1:
+    step, unit = table.stride()
+    if not 1 <= batch <= MAX_BATCH or pages < 1:
+        raise ConfigError(f"a call takes 1 to {MAX_BATCH} sequences of at least one page, got {batch} of {pages}")
+    if pages > 1 and unit != 1:
         raise ConfigError("the page table must have a unit stride along its pages")
-    heads.check_vector("starts", starts, batch, (torch.int32,), device)
+    heads.check_vector("starts", starts, batch, _INT32, index)
     if offsets is not None:
-        heads.check_vector("offsets", offsets, batch + 1, (torch.int32,), device)
+        heads.check_vector("offsets", offsets, batch + 1, _INT32, index)
     elif tokens % batch:
         raise ConfigError(f"without offsets every sequence has the same number of tokens: {tokens} over {batch} sequences")
-    return _lib.BatchDesc(table.data_ptr(), starts.data_ptr(), offsets.data_ptr() if offsets is not None else None, table.stride(0),
-                          tokens, batch, pages)
+    return _lib.BatchDesc(table.data_ptr(), starts.data_ptr(), offsets.data_ptr() if offsets is not None else None, step, tokens, batch, pages)
 
 
 class QuantisedCache:
@@ -80,7 +82,7 @@ class QuantisedCache:
                 raise ConfigError(f"{name} must be contiguous and 16-byte aligned")
         self.keys, self.key_scales, self.values, self.value_scales = keys, key_scales, values, value_scales
         self.pages, self.kv_heads, self.page, self.width = pages, kv_heads, page, width
-        self.device = keys.device
+        self.device, self.index = keys.device, keys.get_device()
         self.faults = torch.zeros(1, dtype=torch.int32, device=keys.device)
         self.desc = _lib.CacheDesc(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
                                    self.faults.data_ptr(), pages, kv_heads, page, width)
@@ -91,10 +93,24 @@ class QuantisedCache:
 
     def _check_rows(self, name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
         heads.check_rows(name, t, like)
-        if t.device != self.device:
+        if t.get_device() != self.index:
             raise ConfigError(f"{name} must be on {self.device}, where the cache is")
-        if t.shape[1:] != (self.kv_heads, self.width) or (like is not None and t.shape != like.shape):
+        tokens, kv_heads, width = t.shape
+        if kv_heads != self.kv_heads or width != self.width or (like is not None and tokens != like.shape[0]):
             raise ConfigError(f"{name} must be [tokens, {self.kv_heads}, {self.width}], got {tuple(t.shape)}")
+
+    def batch_of(self, table: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor | None, tokens: int) -> _lib.BatchDesc:
+        """The checked description of a call's sequences."""
+        b = batch_of(table, starts, offsets, tokens, self.index)
+        if b.max_pages * self.page > MAX_POSITIONS:
+            raise ConfigError(f"a page table holds at most 2^30 positions a sequence, got {b.max_pages} pages of {self.page}")
+        return b
+
+    def _call(self, entry, name: str, keys, values, b: _lib.BatchDesc, stream) -> None:
+        with heads.on_device(self.index):
+            rc = entry(self.desc, b, heads.DTYPES[keys.dtype], _lib.Heads(*heads.rows(keys)), _lib.Heads(*heads.rows(values)),
+                       heads.raw(self.index, stream))
+        _lib.check(rc, name)
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                offsets: torch.Tensor | None = None, *, stream=None) -> None:
@@ -104,11 +120,8 @@ class QuantisedCache:
         """
         self._check_rows("keys", keys)
         self._check_rows("values", values, keys)
-        b = batch_of(table, starts, offsets, keys.shape[0], self.device)
-        with heads.on_device(self.device):
-            rc = _lib.load().tgcb_cache_append(self.desc, b, heads.DTYPES[keys.dtype], heads.rows(keys), heads.rows(values),
-                                               heads.raw(self.device, stream))
-        _lib.check(rc, "tgcb_cache_append")
+        b = self.batch_of(table, starts, offsets, keys.shape[0])
+        self._call(_lib.load().tgcb_cache_append, "tgcb_cache_append", keys, values, b, stream)
 
     def read_into(self, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
                   offsets: torch.Tensor | None = None, *, stream=None) -> None:
@@ -118,11 +131,8 @@ class QuantisedCache:
         heads.check_written("keys", keys)
         heads.check_written("values", values)
         heads.check_apart("keys", keys, "values", values)
-        b = batch_of(table, starts, offsets, keys.shape[0], self.device)
-        with heads.on_device(self.device):
-            rc = _lib.load().tgcb_cache_read(self.desc, b, heads.DTYPES[keys.dtype], heads.rows(keys), heads.rows(values),
-                                             heads.raw(self.device, stream))
-        _lib.check(rc, "tgcb_cache_read")
+        b = self.batch_of(table, starts, offsets, keys.shape[0])
+        self._call(_lib.load().tgcb_cache_read, "tgcb_cache_read", keys, values, b, stream)
 
     def read(self, tokens: int, table: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor | None = None, *,
              dtype: torch.dtype = torch.float32, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -134,9 +144,10 @@ class QuantisedCache:
             raise ConfigError(f"rows are read as float32, bfloat16 or float16, not {dtype}")
         if tokens < 0:
             raise ConfigError(f"there cannot be {tokens} tokens")
-        with heads.on_stream(self.device, stream):
-            keys, values = (torch.empty(tokens, self.kv_heads, self.width, dtype=dtype, device=self.device) for _ in range(2))
-        self.read_into(keys, values, table, starts, offsets, stream=stream)
+        b = self.batch_of(table, starts, offsets, tokens)
+        with heads.on_stream(self.index, stream):
+            keys, values = torch.empty((2, tokens, self.kv_heads, self.width), dtype=dtype, device=self.device).unbind()
+        self._call(_lib.load().tgcb_cache_read, "tgcb_cache_read", keys, values, b, stream)
         return keys, values
 
     def check(self) -> None:

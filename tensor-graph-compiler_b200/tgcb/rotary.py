@@ -21,6 +21,7 @@ from tgcb import _lib, heads
 from tgcb.errors import ConfigError
 
 MAX_WIDTH = 1024
+_NONE = (None, 0, 0)
 
 
 def frequencies(rotary: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -37,33 +38,33 @@ def _check(queries, keys, query_gain, key_gain, positions, freqs, epsilon) -> No
     heads.check_rows("queries", queries)
     heads.check_rows("keys", keys, queries)
     tokens, q_heads, width = queries.shape
-    if keys.shape[0] != tokens or keys.shape[2] != width:
+    k_tokens, k_heads, k_width = keys.shape
+    if k_tokens != tokens or k_width != width:
         raise ConfigError("queries and keys must have the same tokens and width")
-    if q_heads < 1 or keys.shape[1] < 1:
+    if q_heads < 1 or k_heads < 1:
         raise ConfigError("there has to be at least one query head and one key head")
     if not 2 <= width <= MAX_WIDTH:
         raise ConfigError(f"a head's width must be from 2 to {MAX_WIDTH}, got {width}")
-    device = queries.device
-    heads.check_vector("query_gain", query_gain, width, (torch.float32, queries.dtype), device)
-    heads.check_vector("key_gain", key_gain, width, (query_gain.dtype,), device)
-    heads.check_vector("positions", positions, tokens, (torch.int32, torch.int64), device)
+    index = queries.get_device()
+    heads.check_vector("query_gain", query_gain, width, (torch.float32, queries.dtype), index)
+    heads.check_vector("key_gain", key_gain, width, (query_gain.dtype,), index)
+    heads.check_vector("positions", positions, tokens, (torch.int32, torch.int64), index)
     half = freqs.shape[0] if isinstance(freqs, torch.Tensor) and freqs.dim() == 1 else 0
     if not 1 <= half <= width // 2:
         raise ConfigError(f"frequencies must be a vector of 1 to {width // 2} values for heads of width {width}")
-    heads.check_vector("frequencies", freqs, half, (torch.float64,), device)
+    heads.check_vector("frequencies", freqs, half, (torch.float64,), index)
     if not epsilon > 0:
         raise ConfigError(f"the epsilon has to be positive, got {epsilon}")
 
 
-def _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out) -> _lib.RotaryDesc:
-    d = _lib.RotaryDesc(
-        heads.DTYPES[queries.dtype], heads.DTYPES[query_gain.dtype], positions.element_size(), bool(interleaved), queries.shape[0],
-        (queries.shape[1], keys.shape[1]), queries.shape[2], 2 * freqs.shape[0], epsilon, positions.data_ptr(), freqs.data_ptr(),
-        (query_gain.data_ptr(), key_gain.data_ptr()),
+def _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out, grads=(_NONE, _NONE)) -> _lib.RotaryDesc:
+    tokens, q_heads, width = queries.shape
+    return _lib.RotaryDesc(
+        heads.DTYPES[queries.dtype], heads.DTYPES[query_gain.dtype], positions.element_size(), bool(interleaved), tokens,
+        (q_heads, keys.shape[1]), width, 2 * freqs.shape[0], epsilon, positions.data_ptr(), freqs.data_ptr(),
+        (query_gain.data_ptr(), key_gain.data_ptr()), (heads.rows(queries), heads.rows(keys)), grads,
+        (heads.rows(out[0]), heads.rows(out[1])),
     )
-    d.rows_in[0], d.rows_in[1] = heads.rows(queries), heads.rows(keys)
-    d.rows_out[0], d.rows_out[1] = heads.rows(out[0]), heads.rows(out[1])
-    return d
 
 
 def _check_outputs(out: tuple, names: tuple, inputs: tuple) -> None:
@@ -89,9 +90,9 @@ def norm_rotate_into(queries: torch.Tensor, keys: torch.Tensor, query_gain: torc
 
 def _run(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out, stream) -> None:
     d = _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out)
-    device = queries.device
-    with heads.on_device(device):
-        _lib.check(_lib.load().tgcb_norm_rotate(d, heads.raw(device, stream)), "tgcb_norm_rotate")
+    index = queries.get_device()
+    with heads.on_device(index):
+        _lib.check(_lib.load().tgcb_norm_rotate(d, heads.raw(index, stream)), "tgcb_norm_rotate")
 
 
 def norm_rotate(queries: torch.Tensor, keys: torch.Tensor, query_gain: torch.Tensor, key_gain: torch.Tensor,
@@ -103,9 +104,8 @@ def norm_rotate(queries: torch.Tensor, keys: torch.Tensor, query_gain: torch.Ten
     type, [width]; ``positions`` int32 or int64, [tokens]; ``frequencies`` float64, [1 .. width / 2].
     """
     _check(queries, keys, query_gain, key_gain, positions, frequencies, epsilon)
-    with heads.on_stream(queries.device, stream):
-        out = (torch.empty(queries.shape, dtype=queries.dtype, device=queries.device),
-               torch.empty(keys.shape, dtype=keys.dtype, device=keys.device))
+    with heads.on_stream(queries.get_device(), stream):
+        out = queries.new_empty(queries.shape), keys.new_empty(keys.shape)
     _run(queries, keys, query_gain, key_gain, positions, frequencies, epsilon, interleaved, out, stream)
     return out
 
@@ -119,7 +119,7 @@ def norm_rotate_backward(query_grad: torch.Tensor, key_grad: torch.Tensor, queri
     ``out`` names where the first two go (each may be its input or its output's gradient itself).
     """
     _check(queries, keys, query_gain, key_gain, positions, frequencies, epsilon)
-    device = queries.device
+    index = queries.get_device()
     for name, g, x in (("query_grad", query_grad, queries), ("key_grad", key_grad, keys)):
         heads.check_rows(name, g, x)
         if g.shape != x.shape:
@@ -128,15 +128,15 @@ def norm_rotate_backward(query_grad: torch.Tensor, key_grad: torch.Tensor, queri
         _check_outputs(tuple(out), ("query gradient", "key gradient"),
                        ((("queries", queries), ("query_grad", query_grad)), (("keys", keys), ("key_grad", key_grad))))
     lib, width = _lib.load(), queries.shape[2]
-    with heads.on_stream(device, stream):
+    with heads.on_stream(index, stream):
         if out is None:
-            out = (torch.empty(queries.shape, dtype=queries.dtype, device=device), torch.empty(keys.shape, dtype=keys.dtype, device=device))
-        gains = torch.empty(2, width, dtype=query_gain.dtype, device=device)
-        scratch = torch.empty(lib.tgcb_norm_rotate_scratch_bytes(width), dtype=torch.uint8, device=device)
-    d = _desc(queries, keys, query_gain, key_gain, positions, frequencies, epsilon, interleaved, out)
-    d.grad[0], d.grad[1] = heads.rows(query_grad), heads.rows(key_grad)
+            out = queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+        gains = query_gain.new_empty((2, width))
+        scratch = torch.empty(lib.tgcb_norm_rotate_scratch_bytes(width), dtype=torch.uint8, device=queries.device)
+    d = _desc(queries, keys, query_gain, key_gain, positions, frequencies, epsilon, interleaved, out,
+              (heads.rows(query_grad), heads.rows(key_grad)))
     d.gain_grad[0], d.gain_grad[1] = gains.data_ptr(), gains.data_ptr() + width * gains.element_size()
     d.scratch, d.scratch_bytes = scratch.data_ptr(), scratch.numel()
-    with heads.on_device(device):
-        _lib.check(lib.tgcb_norm_rotate_backward(d, heads.raw(device, stream)), "tgcb_norm_rotate_backward")
+    with heads.on_device(index):
+        _lib.check(lib.tgcb_norm_rotate_backward(d, heads.raw(index, stream)), "tgcb_norm_rotate_backward")
     return out[0], out[1], gains[0], gains[1]
