@@ -24,7 +24,7 @@ struct Rows {
 };
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 8;  // tokens a CTA takes at most
+constexpr int kTokens = 16;  // tokens a CTA takes at most
 
 // Where a token row lies: its sequence (-1: none), and the page and place of its position
 // (page -1: the position or the table's entry is out of range).
@@ -127,7 +127,8 @@ struct Eight {
 // Bound by HBM: append reads a row and writes width + 4 bytes, read the reverse. A thread has eight values
 // of a row, width / 8 threads a row; a CTA takes up to kTokens tokens with all their heads, keys then
 // values, and has the values of kAhead rounds on their way at once. WHOLE: rows are 16-byte aligned.
-constexpr int kAhead = 4;
+template <typename T>
+constexpr int kAhead = 8 / sizeof(T);  // 64 bytes a thread, within the registers of four CTAs an SM
 
 // Codes of eight values: rint(x / scale). x * (1 / scale) is off by 2^-22 of the quotient at most, so
 // away from half-integers (3e-5) it rounds as the quotient does, and near them the quotient
@@ -155,7 +156,7 @@ __device__ __forceinline__ uint2 codes_of(const float* x, float largest, float s
 }
 
 template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
+__global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
                                                         int lanes_log) {
   __shared__ Place places[kTokens];
   __shared__ int later[kTokens];
@@ -165,10 +166,10 @@ __global__ void __launch_bounds__(kThreads) append_rows(const Cache c, const Bat
   const int rows_at_once = kThreads >> lanes_log, rows = count * 2 * c.heads;
   if (threadIdx.x < kTokens) places[threadIdx.x].sequence = -1, later[threadIdx.x] = 0;
 
-  for (int row0 = 0; row0 < rows; row0 += kAhead * rows_at_once) {
-    Eight<T, WHOLE> x[kAhead];
+  for (int row0 = 0; row0 < rows; row0 += kAhead<T> * rows_at_once) {
+    Eight<T, WHOLE> x[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAhead<T>; ++i) {
       const int row = row0 + i * rows_at_once + group;
       if (row < rows) {
         const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) append_rows(const Cache c, const Bat
       __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAhead<T>; ++i) {
       const int row = row0 + i * rows_at_once + group;
       const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
       float v[8];
@@ -220,11 +221,11 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
   __syncthreads();
   find_places(c, b, token0, count, places);
   __syncthreads();
-  for (int row0 = 0; row0 < rows; row0 += kAhead * rows_at_once) {
-    uint2 q[kAhead];
-    float scale[kAhead];
+  for (int row0 = 0; row0 < rows; row0 += kAhead<T> * rows_at_once) {
+    uint2 q[kAhead<T>];
+    float scale[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAhead<T>; ++i) {
       const int row = row0 + i * rows_at_once + group;
       const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
       q[i] = make_uint2(0, 0);
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
       }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAhead<T>; ++i) {
       const int row = row0 + i * rows_at_once + group;
       const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
       if (row >= rows || places[token].sequence < 0) continue;

@@ -7,6 +7,8 @@
 // dx = r (e - x r^2 mean(e x)).
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -145,23 +147,35 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
 
 // Rows of 16-byte vectors. A group of `lanes` threads has one row: thread i of it holds two vectors, which in the turned
 // columns are the two halves of its pairs (or, interleaved, two neighbouring vectors), so that a
-// pair never leaves its thread. A CTA takes `tokens_each` tokens with `groups[side]` groups a side for each, every
-// group always on the same side and columns; the cosines of its tokens are computed once for all
-// heads, into shared memory, while the rows are on their way.
+// pair never leaves its thread. A CTA takes `tokens_each` tokens at a time, with `groups[side]` groups a side for each
+// (a side's heads in `passes` rounds); a group always has the same side and columns.
 //
-// Bound by HBM: each row is read and written once (backward: two read, one written). 8192
-// tokens of 32 + 8 bfloat16 heads of 128: forward 168 MB, backward 252 MB.
-constexpr int kVecThreads = 512;
+// Bound by HBM: each row is read and written once (backward: two read, one written). What has to be
+// hidden is the latency of the rows and of the angles (float64 products, which few threads
+// compute once a token for all heads). So CTAs are persistent, each thread copies its own vectors kStages
+// steps ahead into slots of shared memory that no other thread touches, and the angles of the next
+// tokens are computed while the present ones are turned.
+// Threads a CTA has at most, and the CTAs of that size that fit an SM's registers: 64 a thread forward, 102 backward.
+constexpr int kVecThreads[2] = {512, 320};
+constexpr int kVecResident = 2;
+constexpr int kStages = 4;
+constexpr size_t kMaxShared = 200 * 1024;
 
 struct Layout {
   int lanes_log, groups[2], tokens_each, passes, threads;
   size_t shared;
 };
 
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+
 template <typename T, bool INTERLEAVED, bool BACKWARD>
-__global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vectors(const Params p, const Layout layout) {
-  constexpr int V = Vec<T>::N;
-  // gains [side][width], then cosines and sines [2 buffers][tokens_each][cos, sin][half]; at the end the sums
+__global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rotate_vectors(const Params p, const Layout layout) {
+  constexpr int V = Vec<T>::N, SLOTS = BACKWARD ? 4 : 2;
+  if (BACKWARD) asm volatile("griddepcontrol.launch_dependents;");  // gain_sums, which waits for the end
+  // slots [stage][vector][thread] of 16 bytes, gains [side][width], cosines and sines [2 buffers][tokens_each][cos,
+  // sin][half]; at the end the sums
   extern __shared__ __align__(16) float shared[];
   const int half = p.rotary / 2, lanes = 1 << layout.lanes_log, per_token = layout.groups[0] + layout.groups[1];
   const int group = threadIdx.x >> layout.lanes_log, item = threadIdx.x & (lanes - 1);
@@ -184,42 +198,74 @@ __global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vec
     turn_a = turn_b = paired ? item * V : -1;
   }
   const bool has_a = working && a < p.width, has_b = working && b < p.width;
+  if (!has_a) a = 0;
+  if (!has_b) b = 0;
+  uint4* slots = reinterpret_cast<uint4*>(shared) + threadIdx.x;
+  const unsigned slots_at = static_cast<unsigned>(__cvta_generic_to_shared(slots));
+  float* gains = shared + kStages * SLOTS * blockDim.x * 4;
+  float* all_angles = gains + 2 * p.width;
+  for (int i = threadIdx.x; i < 2 * p.width; i += blockDim.x)
+    gains[i] = load_any(p.side[i >= p.width].gain, p.gain_dtype, i >= p.width ? i - p.width : i);
+  const float *gain_a = gains + which * p.width + a, *gain_b = gains + which * p.width + b;
   float sum_a[V], sum_b[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum_a[i] = sum_b[i] = 0.f;
-  for (int i = threadIdx.x; i < 2 * p.width; i += blockDim.x)
-    shared[i] = load_any(p.side[i >= p.width].gain, p.gain_dtype, i >= p.width ? i - p.width : i);
-  const float* gain_a = shared + which * p.width + (has_a ? a : 0);
-  const float* gain_b = shared + which * p.width + (has_b ? b : 0);
-  float* all_angles = shared + 2 * p.width;
 
-  int buffer = 0;
-  for (long long tile = blockIdx.x; tile * layout.tokens_each < p.tokens; tile += gridDim.x, buffer ^= 1) {
-    const long long token0 = tile * layout.tokens_each, token = token0 + token_in;
-    float* angles = all_angles + buffer * layout.tokens_each * p.rotary;
+  const long long tiles = (p.tokens + layout.tokens_each - 1) / layout.tokens_each;
+  const long long tile_step = (long long)gridDim.x * layout.tokens_each;
+  const long long mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // this CTA's tiles, one at least
+
+  // copies of (tile, pass) in order, kStages - 1 ahead of their use
+  long long ahead_token = (long long)blockIdx.x * layout.tokens_each + token_in, ahead_left = mine;
+  int ahead_pass = 0, ahead_stage = 0;
+  auto copy_ahead = [&]() {
+    if (ahead_left > 0) {
+      const int head = head0 + ahead_pass * heads_step;
+      const bool row = ahead_token < p.tokens && head < s.heads;
+      const long long token = row ? ahead_token : 0;
+      const int h = row ? head : 0;
+      const unsigned to = slots_at + ahead_stage * SLOTS * blockDim.x * 16;
+      const T* x = static_cast<const T*>(s.in) + token * s.in_t + h * s.in_h;
+      copy16(to, x + a, row && has_a);
+      copy16(to + blockDim.x * 16, x + b, row && has_b);
+      if (BACKWARD) {
+        const T* d = static_cast<const T*>(s.grad) + token * s.grad_t + h * s.grad_h;
+        copy16(to + 2 * blockDim.x * 16, d + a, row && has_a);
+        copy16(to + 3 * blockDim.x * 16, d + b, row && has_b);
+      }
+      if (++ahead_pass == layout.passes) ahead_pass = 0, ahead_token += tile_step, --ahead_left;
+    }
+    ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto angles_of = [&](long long token0, float* to) {
+    for (int i = threadIdx.x; i < layout.tokens_each * half; i += blockDim.x) {
+      const int t = i / half, f = i - t * half;
+      if (token0 + t < p.tokens) turn(position_of(p, token0 + t), p.frequencies[f], to + t * p.rotary + f, to + t * p.rotary + half + f);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) copy_ahead();
+  long long token0 = (long long)blockIdx.x * layout.tokens_each;
+  int buffer = 0, stage = 0;
+  angles_of(token0, all_angles);
+  __syncthreads();
+
+  for (long long tile = 0; tile < mine; ++tile, token0 += tile_step, buffer ^= 1) {
+    const long long token = token0 + token_in;
+    // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
+    const float* cs = all_angles + (buffer * layout.tokens_each + (working ? token_in : 0)) * p.rotary;
     for (int pass = 0; pass < layout.passes; ++pass) {
+      copy_ahead();
+      if (pass == 0 && tile + 1 < mine) angles_of(token0 + tile_step, all_angles + (buffer ^ 1) * layout.tokens_each * p.rotary);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       const int head = head0 + pass * heads_step;
       const bool row = token < p.tokens && head < s.heads;
-      const T* x = static_cast<const T*>(s.in) + token * s.in_t + head * s.in_h;
-      const T* d = BACKWARD ? static_cast<const T*>(s.grad) + token * s.grad_t + head * s.grad_h : nullptr;
       T* y = static_cast<T*>(s.out) + token * s.out_t + head * s.out_h;
-      Vec<T> xa, xb, da, db;
-      xa.raw = xb.raw = da.raw = db.raw = make_uint4(0, 0, 0, 0);
-      if (row && has_a) xa.raw = *reinterpret_cast<const uint4*>(x + a);
-      if (row && has_b) xb.raw = *reinterpret_cast<const uint4*>(x + b);
-      if (BACKWARD) {
-        if (row && has_a) da.raw = *reinterpret_cast<const uint4*>(d + a);
-        if (row && has_b) db.raw = *reinterpret_cast<const uint4*>(d + b);
-      }
-      if (pass == 0) {
-        for (int i = threadIdx.x; i < layout.tokens_each * half; i += blockDim.x) {
-          const int t = i / half, f = i - t * half;
-          if (token0 + t < p.tokens) turn(position_of(p, token0 + t), p.frequencies[f], angles + t * p.rotary + f, angles + t * p.rotary + half + f);
-        }
-        __syncthreads();  // the other buffer's readers are past it too, so the next tile may fill that one
-      }
-      // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
-      const float* cs = angles + (working ? token_in : 0) * p.rotary;
+      const uint4* from = slots + stage * SLOTS * blockDim.x;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      Vec<T> xa, xb;
+      xa.raw = from[0], xb.raw = from[blockDim.x];
       float fa[V], fb[V], square = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -255,6 +301,8 @@ __global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vec
         if (row && has_a) store_vec<T>(y + a, fa);
         if (row && has_b) store_vec<T>(y + b, fb);
       } else {
+        Vec<T> da, db;
+        da.raw = from[2 * blockDim.x], db.raw = from[3 * blockDim.x];
         float ga[V], gb[V], ex = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) ga[i] = to_float(da.e[i]), gb[i] = to_float(db.e[i]);
@@ -288,23 +336,22 @@ __global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vec
           ex += __shfl_xor_sync(0xffffffffu, ex, o);
         }
         const float r = 1.f / sqrtf(square / (float)p.width + p.epsilon), m = ex * r * r / (float)p.width;
+        if (row) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (row) {
+          for (int i = 0; i < V; ++i) {
             sum_a[i] = fmaf(ga[i] * r, fa[i], sum_a[i]);
             sum_b[i] = fmaf(gb[i] * r, fb[i], sum_b[i]);
+            fa[i] = r * (ga[i] * gain_a[i] - fa[i] * m);
+            fb[i] = r * (gb[i] * gain_b[i] - fb[i] * m);
           }
-          fa[i] = r * (ga[i] * gain_a[i] - fa[i] * m);
-          fb[i] = r * (gb[i] * gain_b[i] - fb[i] * m);
+          if (has_a) store_vec<T>(y + a, fa);
+          if (has_b) store_vec<T>(y + b, fb);
         }
-        if (row && has_a) store_vec<T>(y + a, fa);
-        if (row && has_b) store_vec<T>(y + b, fb);
       }
     }
+    __syncthreads();  // the next tile's angles are there, this one's are free
   }
   if (BACKWARD) {  // this CTA's gain gradients: the groups of a side added up in order
-    __syncthreads();
-    const int groups = layout.tokens_each * per_token;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (has_a) shared[group * p.width + a + i] = sum_a[i];
@@ -314,8 +361,9 @@ __global__ void __launch_bounds__(kVecThreads, BACKWARD ? 1 : 2) norm_rotate_vec
     for (int c = threadIdx.x; c < 2 * p.width; c += blockDim.x) {
       const int side = c >= p.width, column = c - side * p.width;
       float v = 0.f;
-      for (int g = 0; g < groups; ++g)
-        if ((g % per_token >= layout.groups[0]) == (side == 1)) v += shared[g * p.width + column];
+      for (int t = 0; t < layout.tokens_each; ++t)
+        for (int g = side ? layout.groups[0] : 0; g < (side ? per_token : layout.groups[0]); ++g)
+          v += shared[(t * per_token + g) * p.width + column];
       p.partials[(long long)blockIdx.x * 2 * p.width + c] = v;
     }
   }
@@ -337,39 +385,51 @@ bool vectors(const Params& p, bool backward, Layout* out) {
   Layout l = {};
   while ((1 << l.lanes_log) < items) ++l.lanes_log;
   if (l.lanes_log > 5) return false;
-  const int most = kVecThreads >> l.lanes_log;
+  const int most = kVecThreads[backward] >> l.lanes_log;
   for (l.passes = 1;; ++l.passes) {
     for (int i = 0; i < 2; ++i) l.groups[i] = (p.side[i].heads + l.passes - 1) / l.passes;
     if (l.groups[0] + l.groups[1] <= most) break;
   }
-  // several tokens a CTA where one has few heads and there are CTAs enough
+  // several tokens a CTA where one has few heads and there are tiles enough
   const int per_token = l.groups[0] + l.groups[1];
   l.tokens_each = 1;
   while (2 * l.tokens_each * per_token <= most / 2 && p.tokens / (2 * l.tokens_each) >= 148 * 8) l.tokens_each *= 2;
   l.threads = ((l.tokens_each * per_token << l.lanes_log) + 31) / 32 * 32;
-  l.shared = (2ull * p.width + 2ull * l.tokens_each * p.rotary) * sizeof(float);
+  l.shared = (2ull * p.width + 2ull * l.tokens_each * p.rotary) * sizeof(float) + (size_t)kStages * (backward ? 4 : 2) * l.threads * 16;
   const size_t sums = backward ? (size_t)(l.threads >> l.lanes_log) * p.width * sizeof(float) : 0;
   if (sums > l.shared) l.shared = sums;
-  if (l.shared > 48 * 1024) return false;
   *out = l;
-  return true;
+  return l.shared <= kMaxShared;
 }
 
-// The gain gradients: column sums of the CTAs' partial rows, in float64 and in a fixed order.
-__global__ void __launch_bounds__(256) gain_sums(const Params p, int partials) {
-  __shared__ double part[8][33];
+// The gain gradients: column sums of the CTAs' partial rows, in float64 and in a fixed order. 32 warps
+// for 32 columns, each with all its rows' loads in flight; with 8 warps that waited for every
+// load 592 partial rows took 30 us.
+__global__ void __launch_bounds__(1024) gain_sums(const Params p, int partials) {
+  __shared__ double part[32][33];
+  constexpr int PER = (kPartials + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int row = warp + 32 * i;
+    x[i] = c < 2 * p.width && row < partials ? __ldcg(p.partials + (long long)row * 2 * p.width + c) : 0.f;
+  }
   double v = 0.0;
-  if (c < 2 * p.width)
-    for (int i = warp; i < partials; i += 8) v += (double)p.partials[(long long)i * 2 * p.width + c];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v += (double)x[i];
   part[warp][lane] = v;
   __syncthreads();
-  if (warp == 0 && c < 2 * p.width) {
+  // warp w adds up column w
+  v = part[lane][warp];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) v += part[w][lane];
-    const int which = c >= p.width;
-    store_any(p.side[which].gain_grad, p.gain_dtype, c - which * p.width, (float)v);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
+  const int column = blockIdx.x * 32 + warp;
+  if (lane == 0 && column < 2 * p.width) {
+    const int which = column >= p.width;
+    store_any(p.side[which].gain_grad, p.gain_dtype, column - which * p.width, (float)v);
   }
 }
 
@@ -414,42 +474,63 @@ Params params_of(const tgcb_rotary_desc* d) {
   return p;
 }
 
-template <typename T, bool INTERLEAVED>
-unsigned run_vectors(const Params& p, const Layout& l, bool backward, cudaStream_t s) {
-  const long long tiles = (p.tokens + l.tokens_each - 1) / l.tokens_each;
-  if (!backward) {
-    const unsigned grid = (unsigned)(tiles < 0x7fffffffll ? tiles : 0x7fffffffll);
-    norm_rotate_vectors<T, INTERLEAVED, false><<<grid, l.threads, l.shared, s>>>(p, l);
-    return grid;
+int failed(cudaError_t e) { return e == cudaSuccess ? TGCB_OK : tgcb_internal_fail(TGCB_E_CUDA, "norm_rotate", cudaGetErrorString(e)); }
+
+// Queued behind the kernel that writes the partial rows, and resident before it ends.
+int run_gain_sums(const Params& p, unsigned partials, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((2 * p.width + 31) / 32);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return failed(cudaLaunchKernelEx(&cfg, gain_sums, p, (int)partials));
+}
+
+template <typename T, bool INTERLEAVED, bool BACKWARD>
+int run_vectors(const Params& p, const Layout& l, cudaStream_t s) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return failed(e);
+  static std::atomic<unsigned long long> configured{0};
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    e = cudaFuncSetAttribute(norm_rotate_vectors<T, INTERLEAVED, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared);
+    if (e != cudaSuccess) return failed(e);
+    configured.fetch_or(bit);
   }
-  const unsigned grid = (unsigned)(tiles < kPartials ? tiles : kPartials);
-  norm_rotate_vectors<T, INTERLEAVED, true><<<grid, l.threads, l.shared, s>>>(p, l);
-  return grid;
+  const long long tiles = (p.tokens + l.tokens_each - 1) / l.tokens_each;
+  // one CTA for each that fits
+  const long long by_registers = kVecThreads[BACKWARD] * kVecResident / l.threads, by_shared = 227 * 1024 / (l.shared + 1024);
+  const long long resident = 148 * std::max(1ll, std::min({by_registers, by_shared, 2048ll / l.threads}));
+  const unsigned grid = (unsigned)std::min({tiles, resident, (long long)kPartials});
+  norm_rotate_vectors<T, INTERLEAVED, BACKWARD><<<grid, l.threads, l.shared, s>>>(p, l);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return failed(e);
+  return BACKWARD ? run_gain_sums(p, grid, s) : TGCB_OK;
 }
 
 template <typename T>
 int run(const Params& p, bool backward, cudaStream_t s) {
   Layout l;
   if (p.tokens > 0 && vectors<T>(p, backward, &l)) {
-    const unsigned grid = p.interleaved ? run_vectors<T, true>(p, l, backward, s) : run_vectors<T, false>(p, l, backward, s);
-    if (backward) gain_sums<<<(2 * p.width + 31) / 32, 256, 0, s>>>(p, (int)grid);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "norm_rotate", cudaGetErrorString(e));
-    return TGCB_OK;
+    if (backward) return p.interleaved ? run_vectors<T, true, true>(p, l, s) : run_vectors<T, false, true>(p, l, s);
+    return p.interleaved ? run_vectors<T, true, false>(p, l, s) : run_vectors<T, false, false>(p, l, s);
   }
   const long long rows = p.tokens * (p.side[0].heads + p.side[1].heads);
   const long long ctas = (rows + kRowWarps - 1) / kRowWarps;
   if (!backward) {
     const unsigned grid = (unsigned)(ctas < 148 * 64 ? ctas : 148 * 64);
     if (grid) norm_rotate_rows<T, false><<<grid, 32 * kRowWarps, 0, s>>>(p);
-  } else {
-    const unsigned grid = (unsigned)(ctas < kPartials ? ctas : kPartials);
-    if (grid) norm_rotate_rows<T, true><<<grid, 32 * kRowWarps, kRowWarps * 2 * p.width * sizeof(float), s>>>(p);
-    gain_sums<<<(2 * p.width + 31) / 32, 256, 0, s>>>(p, (int)grid);
+    return failed(cudaGetLastError());
   }
+  const unsigned grid = (unsigned)(ctas < kPartials ? ctas : kPartials);
+  if (grid) norm_rotate_rows<T, true><<<grid, 32 * kRowWarps, kRowWarps * 2 * p.width * sizeof(float), s>>>(p);
   const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "norm_rotate", cudaGetErrorString(e));
-  return TGCB_OK;
+  return e != cudaSuccess ? failed(e) : run_gain_sums(p, grid, s);
 }
 
 int dispatch(const tgcb_rotary_desc* d, bool backward, void* stream) {
