@@ -26,20 +26,22 @@ struct Rows {
 constexpr int kThreads = 256;
 constexpr int kTokens = 16;  // tokens a CTA takes at most
 
-// Where a token row lies: its sequence (-1: none), and the page and place of its position
-// (page -1: the position or the table's entry is out of range).
-struct Place {
-  int sequence, page, row;
+// Where a token row lies: the page and place of its position. Page kNowhere: the position or the table's
+// entry is out of range; kNoSequence: the row belongs to no sequence.
+struct __align__(8) Place {
+  int page, row;
 };
+constexpr int kNowhere = -1, kNoSequence = -2;
 
 // The places of token rows [token0, token0 + count), by the whole CTA; a barrier must follow. Each thread
-// looks at its share of the sequences for the rows that are theirs.
-__device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long long token0, int count, Place* places) {
+// looks at its share of the sequences for the rows that are theirs. *least: the first sequence met.
+__device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long long token0, int count, Place* places, int* least) {
   auto fill = [&](int s, long long first, long long token) {
     const long long position = (long long)__ldg(b.starts + s) + token - first;
     const int page = tgcb_kv::page_of(c, b, s, position);
     if (page < 0) atomicAdd(c.faults, 1);
-    places[token - token0] = Place{s, page, (int)(position & (c.page - 1))};
+    places[token - token0] = Place{page, (int)(position & (c.page - 1))};
+    atomicMin(least, s);
   };
   if (b.offsets == nullptr) {
     if (threadIdx.x < count) {
@@ -58,16 +60,14 @@ __device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long
 // later[i] becomes 1 where a later row of the call has row i's place: two sequences that share a page both
 // write to, or a page twice in one table row. The call's written pages are few beside its rows; a
 // thread takes a sequence, and a sequence of many pages is taken by its warp.
-__device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long long token0, int count, const Place* places, int* later) {
+__device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long long token0, int count, const Place* places, int least, int* later) {
   const int lane = threadIdx.x & 31;
-  int least = b.batch;
-  for (int i = 0; i < count; ++i)
-    if (places[i].sequence >= 0 && places[i].sequence < least) least = places[i].sequence;
   auto look = [&](int s, long long slot, long long first, long long last, long long start) {
     const int page = __ldg(b.table + s * b.table_stride + slot);
+    if (page < 0) return;
     for (int i = 0; i < count; ++i) {
       const long long at = first + (slot << c.page_bits) + places[i].row - start;
-      if (page == places[i].page && at > token0 + i && at >= first && at < last && places[i].sequence >= 0) later[i] = 1;
+      if (page == places[i].page && at > token0 + i && at >= first && at < last) later[i] = 1;
     }
   };
   for (int s0 = least + (threadIdx.x & ~31); s0 < b.batch; s0 += kThreads) {
@@ -95,55 +95,70 @@ __device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long 
   }
 }
 
-// Eight values of a row, a thread's share of it.
+// Eight values of a row, a thread's share of it: eight in a row of 16-bit values, and of float32 four in each
+// half of the row, so that neighbouring threads' 16 bytes lie side by side. WHOLE: rows are 16-byte aligned.
 template <typename T, bool WHOLE>
 struct Eight {
-  static constexpr int N = 8 * sizeof(T) / 16;
+  static constexpr bool HALVES = sizeof(T) == 4;
   union {
-    uint4 raw[N];
+    uint4 raw[sizeof(T) / 2];
     T e[8];
   };
   __device__ Eight() {}
-  __device__ __forceinline__ void load(const T* p) {
+  static __device__ __forceinline__ int column(int item, int i, int width) {
+    return HALVES ? 4 * item + (i & 3) + (i >> 2) * (width / 2) : 8 * item + i;
+  }
+  __device__ __forceinline__ void load(const T* row, int item, int width) {
     if constexpr (WHOLE) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+      raw[0] = *reinterpret_cast<const uint4*>(row + column(item, 0, width));
+      if constexpr (HALVES) raw[1] = *reinterpret_cast<const uint4*>(row + column(item, 4, width));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = p[i];
+      for (int i = 0; i < 8; ++i) e[i] = row[column(item, i, width)];
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
+  __device__ __forceinline__ void store(T* row, int item, int width) const {
     if constexpr (WHOLE) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+      *reinterpret_cast<uint4*>(row + column(item, 0, width)) = raw[0];
+      if constexpr (HALVES) *reinterpret_cast<uint4*>(row + column(item, 4, width)) = raw[1];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = e[i];
+      for (int i = 0; i < 8; ++i) row[column(item, i, width)] = e[i];
+    }
+  }
+  static __device__ __forceinline__ uint2 load_codes(const int8_t* row, int item, int width) {
+    if constexpr (HALVES)
+      return make_uint2(*reinterpret_cast<const unsigned*>(row + 4 * item), *reinterpret_cast<const unsigned*>(row + 4 * item + width / 2));
+    return *reinterpret_cast<const uint2*>(row + 8 * item);
+  }
+  static __device__ __forceinline__ void store_codes(int8_t* row, int item, int width, uint2 q) {
+    if constexpr (HALVES) {
+      *reinterpret_cast<unsigned*>(row + 4 * item) = q.x;
+      *reinterpret_cast<unsigned*>(row + 4 * item + width / 2) = q.y;
+    } else {
+      *reinterpret_cast<uint2*>(row + 8 * item) = q;
     }
   }
 };
 
-// Bound by HBM: append reads a row and writes width + 4 bytes, read the reverse. A thread has eight values
-// of a row, width / 8 threads a row; a CTA takes up to kTokens tokens with all their heads, keys then
-// values, and has the values of kAhead rounds on their way at once. WHOLE: rows are 16-byte aligned.
-template <typename T>
-constexpr int kAhead = 8 / sizeof(T);  // 64 bytes a thread, within the registers of four CTAs an SM
-
 // Codes of eight values: rint(x / scale). x * (1 / scale) is off by 2^-22 of the quotient at most, so
-// away from half-integers (3e-5) it rounds as the quotient does, and near them the quotient
-// decides. With a finite maximum and reciprocal |x / scale| <= 127 (1 + 2^-21): no clamp; other rows
-// divide and clamp. Adding 1.5 2^23 rounds to an integer, ties to even, in the sum's low bits.
+// away from half-integers (3e-5) it rounds as the quotient does, and a thread with a value near one divides. With
+// a finite maximum and reciprocal |x / scale| <= 127 (1 + 2^-21): no clamp; other rows divide and
+// clamp. Adding 1.5 2^23 rounds to an integer, ties to even, in the sum's low bits.
 __device__ __forceinline__ uint2 codes_of(const float* x, float largest, float scale) {
   const float inverse = __fdiv_rn(1.0f, scale);
   unsigned q[8];
   if (isfinite(inverse) && isfinite(largest)) {
+    float near = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float t = x[i] * inverse, rounded = t + 12582912.0f;
-      const float off = fabsf(t - (rounded - 12582912.0f));
+      near = fmaxf(near, fabsf(t - (rounded - 12582912.0f)));
       q[i] = __float_as_uint(rounded);
-      if (off >= 0.49997f) q[i] = __float_as_uint(__fdiv_rn(x[i], scale) + 12582912.0f);
+    }
+    if (near >= 0.49997f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__fdiv_rn(x[i], scale) + 12582912.0f);
     }
   } else {
 #pragma unroll
@@ -155,55 +170,78 @@ __device__ __forceinline__ uint2 codes_of(const float* x, float largest, float s
   return r;
 }
 
+// The larger magnitude, NaN if either is.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+// Bound by HBM: append reads a row and writes width + 4 bytes, read the reverse. width / 8 threads have a
+// row; a CTA takes `each` tokens with all their heads, keys then values, and has the values of kAhead
+// rounds on their way at once.
+template <typename T>
+constexpr int kAhead = 8 / sizeof(T);  // 64 bytes a thread, within the registers of four CTAs an SM
+
+// A thread group's rows of a CTA, in order: token and row of it (keys, then values), by additions alone.
+struct Walk {
+  int token, row, rows, step_tokens, step_rows;
+  __device__ __forceinline__ Walk(int first, int step, int rows) : rows(rows) {
+    token = first / rows, row = first - token * rows;
+    step_tokens = step / rows, step_rows = step - step_tokens * rows;
+  }
+  __device__ __forceinline__ void next() {
+    token += step_tokens, row += step_rows;
+    if (row >= rows) row -= rows, ++token;
+  }
+};
+
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
                                                         int lanes_log) {
   __shared__ Place places[kTokens];
-  __shared__ int later[kTokens];
+  __shared__ int later[kTokens], least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
   const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
-  const int rows_at_once = kThreads >> lanes_log, rows = count * 2 * c.heads;
-  if (threadIdx.x < kTokens) places[threadIdx.x].sequence = -1, later[threadIdx.x] = 0;
+  const int rows_at_once = kThreads >> lanes_log;
+  if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence, later[threadIdx.x] = 0;
+  if (threadIdx.x == 0) least = b.batch;
 
-  for (int row0 = 0; row0 < rows; row0 += kAhead<T> * rows_at_once) {
+  Walk ahead(group, rows_at_once, 2 * c.heads), now(group, rows_at_once, 2 * c.heads);
+  for (int row0 = 0; row0 < count * 2 * c.heads; row0 += kAhead<T> * rows_at_once) {
     Eight<T, WHOLE> x[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i) {
-      const int row = row0 + i * rows_at_once + group;
-      if (row < rows) {
-        const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
-        const Rows& from = r >= c.heads ? values : keys;
-        x[i].load(reinterpret_cast<const T*>(from.data) + (token0 + token) * from.t + (r >= c.heads ? r - c.heads : r) * from.h + 8 * item);
+    for (int i = 0; i < kAhead<T>; ++i, ahead.next()) {
+      if (ahead.token < count) {
+        const bool value = ahead.row >= c.heads;
+        const T* from = reinterpret_cast<const T*>(value ? values.data : keys.data);
+        x[i].load(from + (token0 + ahead.token) * (value ? values.t : keys.t) + (value ? (ahead.row - c.heads) * values.h : ahead.row * keys.h),
+                  item, c.width);
       }
     }
     if (row0 == 0) {
       __syncthreads();
-      find_places(c, b, token0, count, places);
+      find_places(c, b, token0, count, places, &least);
       __syncthreads();
-      find_later(c, b, token0, count, places, later);
+      find_later(c, b, token0, count, places, least, later);
       __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i) {
-      const int row = row0 + i * rows_at_once + group;
-      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
-      float v[8];
-      unsigned m = 0;
+    for (int i = 0; i < kAhead<T>; ++i, now.next()) {
+      float v[8], largest = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = to_float(x[i].e[j]);
-        m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);  // the order of magnitudes, NaN above infinity
-      }
-      for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (row >= rows || places[token].sequence < 0 || places[token].page < 0 || later[token]) continue;
-      const bool value = r >= c.heads;
-      const float largest = __uint_as_float(m);
+      for (int j = 0; j < 8; ++j) v[j] = to_float(x[i].e[j]), largest = larger(largest, v[j]);
+      for (int o = lanes >> 1; o > 0; o >>= 1) largest = larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      if (now.token >= count || later[now.token]) continue;
+      const Place place = places[now.token];
+      if (place.page < 0) continue;
+      const bool value = now.row >= c.heads;
       // float(double(largest) / 127) of the rule: a quotient of 24-bit numbers rounded to 53 bits on the
       // way is never moved to another float32 by it
       const float scale = largest == 0.0f ? 1.0f : __fdiv_rn(largest, 127.0f);
-      const long long at = ((long long)places[token].page * c.heads + (value ? r - c.heads : r)) * c.page + places[token].row;
-      *reinterpret_cast<uint2*>((value ? c.values : c.keys) + at * c.width + 8 * item) = codes_of(v, largest, scale);
+      const long long at = ((long long)place.page * c.heads + (value ? now.row - c.heads : now.row)) * c.page + place.row;
+      Eight<T, WHOLE>::store_codes((value ? c.values : c.keys) + at * c.width, item, c.width, codes_of(v, largest, scale));
       if (item == 0) (value ? c.value_scales : c.key_scales)[at] = scale;
     }
   }
@@ -213,43 +251,46 @@ template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
                                                       int lanes_log) {
   __shared__ Place places[kTokens];
+  __shared__ int least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
   const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
-  const int rows_at_once = kThreads >> lanes_log, rows = count * 2 * c.heads;
-  if (threadIdx.x < kTokens) places[threadIdx.x].sequence = -1;
+  const int rows_at_once = kThreads >> lanes_log;
+  if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence;
+  if (threadIdx.x == 0) least = b.batch;
   __syncthreads();
-  find_places(c, b, token0, count, places);
+  find_places(c, b, token0, count, places, &least);
   __syncthreads();
-  for (int row0 = 0; row0 < rows; row0 += kAhead<T> * rows_at_once) {
+  Walk ahead(group, rows_at_once, 2 * c.heads), now(group, rows_at_once, 2 * c.heads);
+  for (int row0 = 0; row0 < count * 2 * c.heads; row0 += kAhead<T> * rows_at_once) {
     uint2 q[kAhead<T>];
     float scale[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i) {
-      const int row = row0 + i * rows_at_once + group;
-      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
+    for (int i = 0; i < kAhead<T>; ++i, ahead.next()) {
       q[i] = make_uint2(0, 0);
       scale[i] = __int_as_float(0x7fffffff);
-      if (row < rows && places[token].sequence >= 0 && places[token].page >= 0) {
-        const bool value = r >= c.heads;
-        const long long at = ((long long)places[token].page * c.heads + (value ? r - c.heads : r)) * c.page + places[token].row;
-        q[i] = *reinterpret_cast<const uint2*>((value ? c.values : c.keys) + at * c.width + 8 * item);
-        scale[i] = (value ? c.value_scales : c.key_scales)[at];
+      if (ahead.token < count) {
+        const Place place = places[ahead.token];
+        if (place.page >= 0) {
+          const bool value = ahead.row >= c.heads;
+          const long long at = ((long long)place.page * c.heads + (value ? ahead.row - c.heads : ahead.row)) * c.page + place.row;
+          q[i] = Eight<T, WHOLE>::load_codes((value ? c.values : c.keys) + at * c.width, item, c.width);
+          scale[i] = (value ? c.value_scales : c.key_scales)[at];
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i) {
-      const int row = row0 + i * rows_at_once + group;
-      const int token = row / (2 * c.heads), r = row - token * 2 * c.heads;
-      if (row >= rows || places[token].sequence < 0) continue;
+    for (int i = 0; i < kAhead<T>; ++i, now.next()) {
+      if (now.token >= count || places[now.token].page == kNoSequence) continue;
       Eight<T, WHOLE> x;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int code = (int)(signed char)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
         x.e[j] = from_float<T>((float)code * scale[i]);
       }
-      const Rows& to = r >= c.heads ? values : keys;
-      x.store(reinterpret_cast<T*>(to.data) + (token0 + token) * to.t + (r >= c.heads ? r - c.heads : r) * to.h + 8 * item);
+      const bool value = now.row >= c.heads;
+      T* to = reinterpret_cast<T*>(value ? values.data : keys.data);
+      x.store(to + (token0 + now.token) * (value ? values.t : keys.t) + (value ? (now.row - c.heads) * values.h : now.row * keys.h), item, c.width);
     }
   }
 }

@@ -40,7 +40,7 @@ struct Params {
   float* partials;
   long long tokens;
   int gain_dtype, position_bytes, interleaved, width, rotary;
-  float epsilon;
+  float epsilon, by_width;
 };
 
 // cos and sin of position * frequency. The turns are taken in float64 (a far position has many of them
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
       const float v = to_float(x[c]);
       square = fmaf(v, v, square);
     }
-    const float r = 1.f / sqrtf(warp_sum(square) / (float)p.width + p.epsilon);
+    const float r = rsqrtf(fmaf(warp_sum(square), p.by_width, p.epsilon));
 
     // items: `half` pairs, then the single columns behind them
     const int items = half + p.width - p.rotary;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
             mine[c0] += d0 * x0 * r;
             if (pair) mine[c1] += d1 * x1 * r;
           } else {
-            const float m = ex * r * r / (float)p.width;
+            const float m = ex * r * r * p.by_width;
             y[c0] = from_float<T>(r * (d0 * g0 - x0 * m));
             if (pair) y[c1] = from_float<T>(r * (d1 * g1 - x1 * m));
           }
@@ -151,10 +151,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
 // (a side's heads in `passes` rounds); a group always has the same side and columns.
 //
 // Bound by HBM: each row is read and written once (backward: two read, one written). What has to be
-// hidden is the latency of the rows and of the angles (float64 products, which few threads
-// compute once a token for all heads). So CTAs are persistent, each thread copies its own vectors kStages
-// steps ahead into slots of shared memory that no other thread touches, and the angles of the next
-// tokens are computed while the present ones are turned.
+// hidden is the latency of the rows and of the angles (float64 products, once a token for all
+// heads). So CTAs are persistent, and each thread copies its own vectors kStages - 1 steps ahead into slots of
+// shared memory that no other thread touches. Angles are computed for as many tiles of tokens at a time (a
+// batch) as gives every thread one, a batch ahead, so that there is one barrier a batch.
 // Threads a CTA has at most, and the CTAs of that size that fit an SM's registers: 64 a thread forward, 102 backward.
 constexpr int kVecThreads[2] = {512, 320};
 constexpr int kVecResident = 2;
@@ -162,7 +162,7 @@ constexpr int kStages = 4;
 constexpr size_t kMaxShared = 200 * 1024;
 
 struct Layout {
-  int lanes_log, groups[2], tokens_each, passes, threads;
+  int lanes_log, groups[2], tokens_each, passes, threads, batch;
   size_t shared;
 };
 
@@ -170,14 +170,60 @@ __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool valid
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float* out) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + i);
+      out[i] = x.x, out[i + 1] = x.y, out[i + 2] = x.z, out[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p + i);
+      out[i] = x.x, out[i + 1] = x.y;
+    }
+  }
+}
+
+// Turns the pairs of two vectors, by the angles that begin at `cosines` + turn_a and + turn_b (-1: not turned).
+template <int V, bool INTERLEAVED, bool BACK>
+__device__ __forceinline__ void turn_vectors(float* a, float* b, const float* cosines, int sines, int turn_a, int turn_b) {
+  auto pair = [](float* x, float* y, float c, float s) {
+    const float u = *x, v = *y;
+    *x = BACK ? u * c + v * s : u * c - v * s;
+    *y = BACK ? v * c - u * s : u * s + v * c;
+  };
+  if constexpr (!INTERLEAVED) {
+    if (turn_a < 0) return;
+    float c[V], s[V];
+    load_floats<V>(cosines + turn_a, c), load_floats<V>(cosines + sines + turn_a, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) pair(a + i, b + i, c[i], s[i]);
+  } else {
+    float c[V / 2], s[V / 2];
+    if (turn_a >= 0) {
+      load_floats<V / 2>(cosines + turn_a, c), load_floats<V / 2>(cosines + sines + turn_a, s);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) pair(a + 2 * i, a + 2 * i + 1, c[i], s[i]);
+    }
+    if (turn_b >= 0) {
+      load_floats<V / 2>(cosines + turn_b, c), load_floats<V / 2>(cosines + sines + turn_b, s);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) pair(b + 2 * i, b + 2 * i + 1, c[i], s[i]);
+    }
+  }
+}
+
 template <typename T, bool INTERLEAVED, bool BACKWARD>
 __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rotate_vectors(const Params p, const Layout layout) {
   constexpr int V = Vec<T>::N, SLOTS = BACKWARD ? 4 : 2;
   if (BACKWARD) asm volatile("griddepcontrol.launch_dependents;");  // gain_sums, which waits for the end
-  // slots [stage][vector][thread] of 16 bytes, gains [side][width], cosines and sines [2 buffers][tokens_each][cos,
-  // sin][half]; at the end the sums
+  // slots [stage][vector][thread] of 16 bytes, gains [side][width], cosines and sines [2 buffers][batch][tokens_each]
+  // [cos, sin][half rounded up to 4]; at the end the sums
   extern __shared__ __align__(16) float shared[];
-  const int half = p.rotary / 2, lanes = 1 << layout.lanes_log, per_token = layout.groups[0] + layout.groups[1];
+  const int half = p.rotary / 2, sines = (half + 3) & ~3, lanes = 1 << layout.lanes_log, per_token = layout.groups[0] + layout.groups[1];
   const int group = threadIdx.x >> layout.lanes_log, item = threadIdx.x & (lanes - 1);
   const int token_in = group / per_token, in_token = group - token_in * per_token;
   const int which = in_token >= layout.groups[0];
@@ -238,26 +284,34 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
     ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // angles of the batch of tiles that begins at token row token0
+  const int per_tile = layout.tokens_each * half;
   auto angles_of = [&](long long token0, float* to) {
-    for (int i = threadIdx.x; i < layout.tokens_each * half; i += blockDim.x) {
-      const int t = i / half, f = i - t * half;
-      if (token0 + t < p.tokens) turn(position_of(p, token0 + t), p.frequencies[f], to + t * p.rotary + f, to + t * p.rotary + half + f);
+    for (int i = threadIdx.x; i < layout.batch * per_tile; i += blockDim.x) {
+      const int tile = i / per_tile, in_tile = i - tile * per_tile, t = in_tile / half, f = in_tile - t * half;
+      const long long token = token0 + tile * tile_step + t;
+      float* at = to + (tile * layout.tokens_each + t) * 2 * sines + f;
+      if (token < p.tokens) turn(position_of(p, token), p.frequencies[f], at, at + sines);
     }
   };
+  const int batch_floats = layout.batch * layout.tokens_each * 2 * sines;
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) copy_ahead();
   long long token0 = (long long)blockIdx.x * layout.tokens_each;
-  int buffer = 0, stage = 0;
+  int buffer = 0, stage = 0, in_batch = 0;
   angles_of(token0, all_angles);
-  __syncthreads();
 
-  for (long long tile = 0; tile < mine; ++tile, token0 += tile_step, buffer ^= 1) {
+  for (long long tile = 0; tile < mine; ++tile, token0 += tile_step) {
     const long long token = token0 + token_in;
+    if (in_batch == 0) {
+      __syncthreads();  // this batch's angles are there, and the other buffer's are used up
+      if (tile + layout.batch < mine) angles_of(token0 + layout.batch * tile_step, all_angles + (buffer ^ 1) * batch_floats);
+    }
     // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
-    const float* cs = all_angles + (buffer * layout.tokens_each + (working ? token_in : 0)) * p.rotary;
+    const float* cs = all_angles + buffer * batch_floats + (in_batch * layout.tokens_each + (working ? token_in : 0)) * 2 * sines;
+    if (++in_batch == layout.batch) in_batch = 0, buffer ^= 1;
     for (int pass = 0; pass < layout.passes; ++pass) {
       copy_ahead();
-      if (pass == 0 && tile + 1 < mine) angles_of(token0 + tile_step, all_angles + (buffer ^ 1) * layout.tokens_each * p.rotary);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       const int head = head0 + pass * heads_step;
       const bool row = token < p.tokens && head < s.heads;
@@ -275,83 +329,48 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
       }
       if (!BACKWARD) {
         for (int o = lanes >> 1; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
-        const float r = 1.f / sqrtf(square / (float)p.width + p.epsilon);
+        const float r = rsqrtf(fmaf(square, p.by_width, p.epsilon));
+        float wa[V], wb[V];
+        load_floats<V>(gain_a, wa), load_floats<V>(gain_b, wb);
 #pragma unroll
-        for (int i = 0; i < V; ++i) fa[i] = fa[i] * r * gain_a[i], fb[i] = fb[i] * r * gain_b[i];
-        if (!INTERLEAVED) {
-          if (turn_a >= 0)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = fa[i], v = fb[i];
-              fa[i] = u * c - v * n, fb[i] = u * n + v * c;
-            }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            if (turn_a >= 0) {
-              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = fa[2 * i], v = fa[2 * i + 1];
-              fa[2 * i] = u * c - v * n, fa[2 * i + 1] = u * n + v * c;
-            }
-            if (turn_b >= 0) {
-              const float c = cs[turn_b + i], n = cs[half + turn_b + i], u = fb[2 * i], v = fb[2 * i + 1];
-              fb[2 * i] = u * c - v * n, fb[2 * i + 1] = u * n + v * c;
-            }
-          }
-        }
+        for (int i = 0; i < V; ++i) fa[i] = fa[i] * r * wa[i], fb[i] = fb[i] * r * wb[i];
+        turn_vectors<V, INTERLEAVED, false>(fa, fb, cs, sines, turn_a, turn_b);
         if (row && has_a) store_vec<T>(y + a, fa);
         if (row && has_b) store_vec<T>(y + b, fb);
       } else {
         Vec<T> da, db;
         da.raw = from[2 * blockDim.x], db.raw = from[3 * blockDim.x];
-        float ga[V], gb[V], ex = 0.f;
+        float ga[V], gb[V], wa[V], wb[V], ex = 0.f;
+        load_floats<V>(gain_a, wa), load_floats<V>(gain_b, wb);
 #pragma unroll
         for (int i = 0; i < V; ++i) ga[i] = to_float(da.e[i]), gb[i] = to_float(db.e[i]);
-        if (!INTERLEAVED) {
-          if (turn_a >= 0)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = ga[i], v = gb[i];
-              ga[i] = u * c + v * n, gb[i] = v * c - u * n;
-            }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            if (turn_a >= 0) {
-              const float c = cs[turn_a + i], n = cs[half + turn_a + i], u = ga[2 * i], v = ga[2 * i + 1];
-              ga[2 * i] = u * c + v * n, ga[2 * i + 1] = v * c - u * n;
-            }
-            if (turn_b >= 0) {
-              const float c = cs[turn_b + i], n = cs[half + turn_b + i], u = gb[2 * i], v = gb[2 * i + 1];
-              gb[2 * i] = u * c + v * n, gb[2 * i + 1] = v * c - u * n;
-            }
-          }
-        }
+        turn_vectors<V, INTERLEAVED, true>(ga, gb, cs, sines, turn_a, turn_b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          ex = fmaf(ga[i] * gain_a[i], fa[i], ex);
-          ex = fmaf(gb[i] * gain_b[i], fb[i], ex);
+          ex = fmaf(ga[i] * wa[i], fa[i], ex);
+          ex = fmaf(gb[i] * wb[i], fb[i], ex);
         }
         for (int o = lanes >> 1; o > 0; o >>= 1) {
           square += __shfl_xor_sync(0xffffffffu, square, o);
           ex += __shfl_xor_sync(0xffffffffu, ex, o);
         }
-        const float r = 1.f / sqrtf(square / (float)p.width + p.epsilon), m = ex * r * r / (float)p.width;
+        const float r = rsqrtf(fmaf(square, p.by_width, p.epsilon)), m = ex * r * r * p.by_width;
         if (row) {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             sum_a[i] = fmaf(ga[i] * r, fa[i], sum_a[i]);
             sum_b[i] = fmaf(gb[i] * r, fb[i], sum_b[i]);
-            fa[i] = r * (ga[i] * gain_a[i] - fa[i] * m);
-            fb[i] = r * (gb[i] * gain_b[i] - fb[i] * m);
+            fa[i] = r * (ga[i] * wa[i] - fa[i] * m);
+            fb[i] = r * (gb[i] * wb[i] - fb[i] * m);
           }
           if (has_a) store_vec<T>(y + a, fa);
           if (has_b) store_vec<T>(y + b, fb);
         }
       }
     }
-    __syncthreads();  // the next tile's angles are there, this one's are free
   }
   if (BACKWARD) {  // this CTA's gain gradients: the groups of a side added up in order
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (has_a) shared[group * p.width + a + i] = sum_a[i];
@@ -395,7 +414,8 @@ bool vectors(const Params& p, bool backward, Layout* out) {
   l.tokens_each = 1;
   while (2 * l.tokens_each * per_token <= most / 2 && p.tokens / (2 * l.tokens_each) >= 148 * 8) l.tokens_each *= 2;
   l.threads = ((l.tokens_each * per_token << l.lanes_log) + 31) / 32 * 32;
-  l.shared = (2ull * p.width + 2ull * l.tokens_each * p.rotary) * sizeof(float) + (size_t)kStages * (backward ? 4 : 2) * l.threads * 16;
+  l.batch = std::max(1, l.threads / (l.tokens_each * half));
+  l.shared = (2ull * p.width + 2ull * l.batch * l.tokens_each * 2 * ((half + 3) & ~3)) * sizeof(float) + (size_t)kStages * (backward ? 4 : 2) * l.threads * 16;
   const size_t sums = backward ? (size_t)(l.threads >> l.lanes_log) * p.width * sizeof(float) : 0;
   if (sums > l.shared) l.shared = sums;
   *out = l;
@@ -471,6 +491,7 @@ Params params_of(const tgcb_rotary_desc* d) {
   p.positions = d->positions, p.frequencies = d->frequencies, p.partials = static_cast<float*>(d->scratch);
   p.tokens = d->tokens, p.gain_dtype = d->gain_dtype, p.position_bytes = d->position_bytes;
   p.interleaved = d->interleaved != 0, p.width = d->width, p.rotary = d->rotary, p.epsilon = (float)d->epsilon;
+  p.by_width = (float)(1.0 / d->width);
   return p;
 }
 
