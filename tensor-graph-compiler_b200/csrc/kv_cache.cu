@@ -26,12 +26,12 @@ struct Rows {
 constexpr int kThreads = 256;
 constexpr int kTokens = 16;  // tokens a CTA takes at most
 
-// Where a token row lies: the page and place of its position. Page kNowhere: the position or the table's
+// Where a token row lies: the page and place of its position. Page -1: the position or the table's
 // entry is out of range; kNoSequence: the row belongs to no sequence.
 struct __align__(8) Place {
   int page, row;
 };
-constexpr int kNowhere = -1, kNoSequence = -2;
+constexpr int kNoSequence = -2;
 
 // The places of token rows [token0, token0 + count), by the whole CTA; a barrier must follow. Each thread
 // looks at its share of the sequences for the rows that are theirs. *least: the first sequence met.
@@ -183,16 +183,15 @@ __device__ __forceinline__ float larger(float a, float b) {
 template <typename T>
 constexpr int kAhead = 8 / sizeof(T);  // 64 bytes a thread, within the registers of four CTAs an SM
 
-// A thread group's rows of a CTA, in order: token and row of it (keys, then values), by additions alone.
-struct Walk {
-  int token, row, rows, step_tokens, step_rows;
-  __device__ __forceinline__ Walk(int first, int step, int rows) : rows(rows) {
-    token = first / rows, row = first - token * rows;
-    step_tokens = step / rows, step_rows = step - step_tokens * rows;
-  }
-  __device__ __forceinline__ void next() {
-    token += step_tokens, row += step_rows;
-    if (row >= rows) row -= rows, ++token;
+// The rows of one thread group: a side and head of the keys and values, and every step-th token from the
+// first. A CTA whose groups are fewer than a token's rows goes over its tokens several times.
+struct Group {
+  int row, rows, token, step;
+  __device__ __forceinline__ Group(int group, int groups, int rows) : rows(rows) {
+    const int at_once = min(groups, rows);
+    step = groups / at_once;
+    token = group / at_once, row = group - token * at_once;
+    if (token >= step) token = 1 << 30;  // more groups than whole tokens' rows: idle
   }
 };
 
@@ -203,46 +202,51 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cac
   __shared__ int later[kTokens], least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
-  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
-  const int rows_at_once = kThreads >> lanes_log;
+  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), groups = kThreads >> lanes_log;
+  const Group g(threadIdx.x >> lanes_log, groups, 2 * c.heads);
   if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence, later[threadIdx.x] = 0;
   if (threadIdx.x == 0) least = b.batch;
 
-  Walk ahead(group, rows_at_once, 2 * c.heads), now(group, rows_at_once, 2 * c.heads);
-  for (int row0 = 0; row0 < count * 2 * c.heads; row0 += kAhead<T> * rows_at_once) {
-    Eight<T, WHOLE> x[kAhead<T>];
+  for (int row0 = 0; row0 < g.rows; row0 += groups) {
+    const int row = row0 + g.row;
+    const bool real = row < g.rows, value = row >= c.heads;
+    const int head = value ? row - c.heads : row;
+    const Rows& rows = value ? values : keys;
+    const T* from = reinterpret_cast<const T*>(rows.data) + (real ? token0 * rows.t + head * rows.h : 0);
+    const long long t = rows.t;
+    int8_t* codes = value ? c.values : c.keys;
+    float* scales = value ? c.value_scales : c.key_scales;
+    for (int base = 0; base < count; base += kAhead<T> * g.step) {
+      Eight<T, WHOLE> x[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i, ahead.next()) {
-      if (ahead.token < count) {
-        const bool value = ahead.row >= c.heads;
-        const T* from = reinterpret_cast<const T*>(value ? values.data : keys.data);
-        x[i].load(from + (token0 + ahead.token) * (value ? values.t : keys.t) + (value ? (ahead.row - c.heads) * values.h : ahead.row * keys.h),
-                  item, c.width);
+      for (int i = 0; i < kAhead<T>; ++i) {
+        const int token = base + i * g.step + g.token;
+        if (real && token < count) x[i].load(from + token * t, item, c.width);
       }
-    }
-    if (row0 == 0) {
-      __syncthreads();
-      find_places(c, b, token0, count, places, &least);
-      __syncthreads();
-      find_later(c, b, token0, count, places, least, later);
-      __syncthreads();
-    }
+      if (row0 == 0 && base == 0) {
+        __syncthreads();
+        find_places(c, b, token0, count, places, &least);
+        __syncthreads();
+        find_later(c, b, token0, count, places, least, later);
+        __syncthreads();
+      }
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i, now.next()) {
-      float v[8], largest = 0.f;
+      for (int i = 0; i < kAhead<T>; ++i) {
+        float v[8], largest = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_float(x[i].e[j]), largest = larger(largest, v[j]);
-      for (int o = lanes >> 1; o > 0; o >>= 1) largest = larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      if (now.token >= count || later[now.token]) continue;
-      const Place place = places[now.token];
-      if (place.page < 0) continue;
-      const bool value = now.row >= c.heads;
-      // float(double(largest) / 127) of the rule: a quotient of 24-bit numbers rounded to 53 bits on the
-      // way is never moved to another float32 by it
-      const float scale = largest == 0.0f ? 1.0f : __fdiv_rn(largest, 127.0f);
-      const long long at = ((long long)place.page * c.heads + (value ? now.row - c.heads : now.row)) * c.page + place.row;
-      Eight<T, WHOLE>::store_codes((value ? c.values : c.keys) + at * c.width, item, c.width, codes_of(v, largest, scale));
-      if (item == 0) (value ? c.value_scales : c.key_scales)[at] = scale;
+        for (int j = 0; j < 8; ++j) v[j] = to_float(x[i].e[j]), largest = larger(largest, v[j]);
+        for (int o = lanes >> 1; o > 0; o >>= 1) largest = larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        const int token = base + i * g.step + g.token;
+        if (!real || token >= count || later[token]) continue;
+        const Place place = places[token];
+        if (place.page < 0) continue;
+        // float(double(largest) / 127) of the rule: a quotient of 24-bit numbers rounded to 53 bits on the
+        // way is never moved to another float32 by it
+        const float scale = largest == 0.0f ? 1.0f : __fdiv_rn(largest, 127.0f);
+        const long long at = ((long long)place.page * c.heads + head) * c.page + place.row;
+        Eight<T, WHOLE>::store_codes(codes + at * c.width, item, c.width, codes_of(v, largest, scale));
+        if (item == 0) scales[at] = scale;
+      }
     }
   }
 }
@@ -254,43 +258,48 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
   __shared__ int least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
-  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log;
-  const int rows_at_once = kThreads >> lanes_log;
+  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), groups = kThreads >> lanes_log;
+  const Group g(threadIdx.x >> lanes_log, groups, 2 * c.heads);
   if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence;
   if (threadIdx.x == 0) least = b.batch;
   __syncthreads();
   find_places(c, b, token0, count, places, &least);
   __syncthreads();
-  Walk ahead(group, rows_at_once, 2 * c.heads), now(group, rows_at_once, 2 * c.heads);
-  for (int row0 = 0; row0 < count * 2 * c.heads; row0 += kAhead<T> * rows_at_once) {
-    uint2 q[kAhead<T>];
-    float scale[kAhead<T>];
+  for (int row = g.row; row < g.rows; row += groups) {
+    const bool value = row >= c.heads;
+    const int head = value ? row - c.heads : row;
+    const Rows& rows = value ? values : keys;
+    T* to = reinterpret_cast<T*>(rows.data) + token0 * rows.t + head * rows.h;
+    const long long t = rows.t;
+    const int8_t* codes = value ? c.values : c.keys;
+    const float* scales = value ? c.value_scales : c.key_scales;
+    for (int base = g.token; base < count; base += kAhead<T> * g.step) {
+      uint2 q[kAhead<T>];
+      float scale[kAhead<T>];
+      bool mine[kAhead<T>];
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i, ahead.next()) {
-      q[i] = make_uint2(0, 0);
-      scale[i] = __int_as_float(0x7fffffff);
-      if (ahead.token < count) {
-        const Place place = places[ahead.token];
+      for (int i = 0; i < kAhead<T>; ++i) {
+        q[i] = make_uint2(0, 0);
+        scale[i] = __int_as_float(0x7fffffff);
+        const int token = base + i * g.step;
+        const Place place = token < count ? places[token] : Place{kNoSequence, 0};
+        mine[i] = place.page != kNoSequence;
         if (place.page >= 0) {
-          const bool value = ahead.row >= c.heads;
-          const long long at = ((long long)place.page * c.heads + (value ? ahead.row - c.heads : ahead.row)) * c.page + place.row;
-          q[i] = Eight<T, WHOLE>::load_codes((value ? c.values : c.keys) + at * c.width, item, c.width);
-          scale[i] = (value ? c.value_scales : c.key_scales)[at];
+          const long long at = ((long long)place.page * c.heads + head) * c.page + place.row;
+          q[i] = Eight<T, WHOLE>::load_codes(codes + at * c.width, item, c.width);
+          scale[i] = scales[at];
         }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i, now.next()) {
-      if (now.token >= count || places[now.token].page == kNoSequence) continue;
-      Eight<T, WHOLE> x;
+      for (int i = 0; i < kAhead<T>; ++i) {
+        Eight<T, WHOLE> x;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int code = (int)(signed char)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
-        x.e[j] = from_float<T>((float)code * scale[i]);
+        for (int j = 0; j < 8; ++j) {
+          const int code = (int)(signed char)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
+          x.e[j] = from_float<T>((float)code * scale[i]);
+        }
+        if (mine[i]) x.store(to + (base + i * g.step) * t, item, c.width);
       }
-      const bool value = now.row >= c.heads;
-      T* to = reinterpret_cast<T*>(value ? values.data : keys.data);
-      x.store(to + (token0 + now.token) * (value ? values.t : keys.t) + (value ? (now.row - c.heads) * values.h : now.row * keys.h), item, c.width);
     }
   }
 }
@@ -298,8 +307,9 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
 template <typename T>
 int run(const Cache& c, const Batch& b, const Rows& k, const Rows& v, bool read, cudaStream_t s) {
   if (b.tokens == 0) return TGCB_OK;
-  // one token a CTA while there are few
-  const int each = b.tokens <= 148 * 8 ? 1 : kTokens;
+  // whole rounds of the 592 CTAs that are resident at once, of at most kTokens tokens each
+  const long long rounds = (b.tokens + 592 * kTokens - 1) / (592 * kTokens);
+  const int each = (int)((b.tokens + 592 * rounds - 1) / (592 * rounds));
   const unsigned grid = (unsigned)((b.tokens + each - 1) / each);
   const int lanes_log = __builtin_ctz((unsigned)c.width / 8);
   bool whole = true;

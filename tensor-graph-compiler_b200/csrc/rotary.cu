@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
   const bool has_a = working && a < p.width, has_b = working && b < p.width;
   if (!has_a) a = 0;
   if (!has_b) b = 0;
-  uint4* slots = reinterpret_cast<uint4*>(shared) + threadIdx.x;
-  const unsigned slots_at = static_cast<unsigned>(__cvta_generic_to_shared(slots));
+  const unsigned slots_at = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + threadIdx.x * 16, slot = blockDim.x * 16;
+  const unsigned stage_bytes = SLOTS * slot, ring_end = kStages * stage_bytes;
   float* gains = shared + kStages * SLOTS * blockDim.x * 4;
   float* all_angles = gains + 2 * p.width;
   for (int i = threadIdx.x; i < 2 * p.width; i += blockDim.x)
@@ -258,32 +258,10 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
   for (int i = 0; i < V; ++i) sum_a[i] = sum_b[i] = 0.f;
 
   const long long tiles = (p.tokens + layout.tokens_each - 1) / layout.tokens_each;
-  const long long tile_step = (long long)gridDim.x * layout.tokens_each;
-  const long long mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // this CTA's tiles, one at least
+  const long long tile_step = (long long)gridDim.x * layout.tokens_each, tile0 = (long long)blockIdx.x * layout.tokens_each;
+  const int mine = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);  // this CTA's tiles, one at least
+  const long long in_step = tile_step * s.in_t, grad_step = tile_step * s.grad_t, out_step = tile_step * s.out_t;
 
-  // copies of (tile, pass) in order, kStages - 1 ahead of their use
-  long long ahead_token = (long long)blockIdx.x * layout.tokens_each + token_in, ahead_left = mine;
-  int ahead_pass = 0, ahead_stage = 0;
-  auto copy_ahead = [&]() {
-    if (ahead_left > 0) {
-      const int head = head0 + ahead_pass * heads_step;
-      const bool row = ahead_token < p.tokens && head < s.heads;
-      const long long token = row ? ahead_token : 0;
-      const int h = row ? head : 0;
-      const unsigned to = slots_at + ahead_stage * SLOTS * blockDim.x * 16;
-      const T* x = static_cast<const T*>(s.in) + token * s.in_t + h * s.in_h;
-      copy16(to, x + a, row && has_a);
-      copy16(to + blockDim.x * 16, x + b, row && has_b);
-      if (BACKWARD) {
-        const T* d = static_cast<const T*>(s.grad) + token * s.grad_t + h * s.grad_h;
-        copy16(to + 2 * blockDim.x * 16, d + a, row && has_a);
-        copy16(to + 3 * blockDim.x * 16, d + b, row && has_b);
-      }
-      if (++ahead_pass == layout.passes) ahead_pass = 0, ahead_token += tile_step, --ahead_left;
-    }
-    ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
   // angles of the batch of tiles that begins at token row token0
   const int per_tile = layout.tokens_each * half;
   auto angles_of = [&](long long token0, float* to) {
@@ -294,54 +272,74 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
       if (token < p.tokens) turn(position_of(p, token), p.frequencies[f], at, at + sines);
     }
   };
-  const int batch_floats = layout.batch * layout.tokens_each * 2 * sines;
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) copy_ahead();
-  long long token0 = (long long)blockIdx.x * layout.tokens_each;
-  int buffer = 0, stage = 0, in_batch = 0;
-  angles_of(token0, all_angles);
+  const int token_floats = layout.tokens_each * 2 * sines, batch_floats = layout.batch * token_floats;
 
-  for (long long tile = 0; tile < mine; ++tile, token0 += tile_step) {
-    const long long token = token0 + token_in;
-    if (in_batch == 0) {
-      __syncthreads();  // this batch's angles are there, and the other buffer's are used up
-      if (tile + layout.batch < mine) angles_of(token0 + layout.batch * tile_step, all_angles + (buffer ^ 1) * batch_floats);
-    }
-    // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
-    const float* cs = all_angles + buffer * batch_floats + (in_batch * layout.tokens_each + (working ? token_in : 0)) * 2 * sines;
-    if (++in_batch == layout.batch) in_batch = 0, buffer ^= 1;
-    for (int pass = 0; pass < layout.passes; ++pass) {
+  for (int pass = 0; pass < layout.passes; ++pass) {
+    const int head = head0 + pass * heads_step;
+    const bool mine_too = working && head < s.heads;
+    const int h = mine_too ? head : 0;
+    // rows of this pass that are this thread's: the tokens tile0 + token_in, a tile_step further each
+    const int tokens_left = mine_too && tile0 + token_in < p.tokens ? (int)((p.tokens - tile0 - token_in + tile_step - 1) / tile_step) : 0;
+    const long long first = tokens_left ? tile0 + token_in : 0;
+    const T* x = static_cast<const T*>(s.in) + first * s.in_t + h * s.in_h;
+    const T* d = BACKWARD ? static_cast<const T*>(s.grad) + first * s.grad_t + h * s.grad_h : nullptr;
+    T* y = static_cast<T*>(s.out) + first * s.out_t + h * s.out_h;
+    int ahead_left = tokens_left;
+    unsigned ahead_at = 0, now_at = 0;
+    auto copy_ahead = [&]() {
+      const bool row = ahead_left > 0;
+      --ahead_left;
+      const unsigned to = slots_at + ahead_at;
+      ahead_at = ahead_at + stage_bytes == ring_end ? 0 : ahead_at + stage_bytes;
+      copy16(to, x + a, row && has_a);
+      copy16(to + slot, x + b, row && has_b);
+      if (BACKWARD) {
+        copy16(to + 2 * slot, d + a, row && has_a);
+        copy16(to + 3 * slot, d + b, row && has_b);
+        if (ahead_left > 0) d += grad_step;
+      }
+      if (ahead_left > 0) x += in_step;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy_ahead();
+    __syncthreads();  // the last pass's angles are used up
+    angles_of(tile0, all_angles);
+    int buffer = 0, in_batch = 0;
+
+    for (int tile = 0; tile < mine; ++tile) {
+      if (in_batch == 0) {
+        __syncthreads();  // this batch's angles are there, and the other buffer's are used up
+        if (tile + layout.batch < mine) angles_of(tile0 + (tile + layout.batch) * tile_step, all_angles + (buffer ^ 1) * batch_floats);
+      }
+      // (cos, sin) of vector a's and vector b's pairs; of the half-split order a pair is (a[i], b[i])
+      const float* cs = all_angles + buffer * batch_floats + in_batch * token_floats + (working ? token_in : 0) * 2 * sines;
+      if (++in_batch == layout.batch) in_batch = 0, buffer ^= 1;
       copy_ahead();
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      const int head = head0 + pass * heads_step;
-      const bool row = token < p.tokens && head < s.heads;
-      T* y = static_cast<T*>(s.out) + token * s.out_t + head * s.out_h;
-      const uint4* from = slots + stage * SLOTS * blockDim.x;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const bool row = tile < tokens_left;
+      const char* from = reinterpret_cast<const char*>(shared) + threadIdx.x * 16 + now_at;
+      now_at = now_at + stage_bytes == ring_end ? 0 : now_at + stage_bytes;
       Vec<T> xa, xb;
-      xa.raw = from[0], xb.raw = from[blockDim.x];
-      float fa[V], fb[V], square = 0.f;
+      xa.raw = *reinterpret_cast<const uint4*>(from), xb.raw = *reinterpret_cast<const uint4*>(from + slot);
+      float fa[V], fb[V], wa[V], wb[V], square = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         fa[i] = to_float(xa.e[i]), fb[i] = to_float(xb.e[i]);
         square = fmaf(fa[i], fa[i], square);
         square = fmaf(fb[i], fb[i], square);
       }
+      load_floats<V>(gain_a, wa), load_floats<V>(gain_b, wb);
       if (!BACKWARD) {
         for (int o = lanes >> 1; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
         const float r = rsqrtf(fmaf(square, p.by_width, p.epsilon));
-        float wa[V], wb[V];
-        load_floats<V>(gain_a, wa), load_floats<V>(gain_b, wb);
 #pragma unroll
         for (int i = 0; i < V; ++i) fa[i] = fa[i] * r * wa[i], fb[i] = fb[i] * r * wb[i];
         turn_vectors<V, INTERLEAVED, false>(fa, fb, cs, sines, turn_a, turn_b);
-        if (row && has_a) store_vec<T>(y + a, fa);
-        if (row && has_b) store_vec<T>(y + b, fb);
       } else {
         Vec<T> da, db;
-        da.raw = from[2 * blockDim.x], db.raw = from[3 * blockDim.x];
-        float ga[V], gb[V], wa[V], wb[V], ex = 0.f;
-        load_floats<V>(gain_a, wa), load_floats<V>(gain_b, wb);
+        da.raw = *reinterpret_cast<const uint4*>(from + 2 * slot), db.raw = *reinterpret_cast<const uint4*>(from + 3 * slot);
+        float ga[V], gb[V], ex = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) ga[i] = to_float(da.e[i]), gb[i] = to_float(db.e[i]);
         turn_vectors<V, INTERLEAVED, true>(ga, gb, cs, sines, turn_a, turn_b);
@@ -363,11 +361,15 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
             fa[i] = r * (ga[i] * wa[i] - fa[i] * m);
             fb[i] = r * (gb[i] * wb[i] - fb[i] * m);
           }
-          if (has_a) store_vec<T>(y + a, fa);
-          if (has_b) store_vec<T>(y + b, fb);
         }
       }
+      if (row) {
+        if (has_a) store_vec<T>(y + a, fa);
+        if (has_b) store_vec<T>(y + b, fb);
+        y += out_step;
+      }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   if (BACKWARD) {  // this CTA's gain gradients: the groups of a side added up in order
     __syncthreads();
