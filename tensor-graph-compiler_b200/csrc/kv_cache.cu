@@ -62,12 +62,12 @@ __device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long
 // thread takes a sequence, and a sequence of many pages is taken by its warp.
 __device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long long token0, int count, const Place* places, int least, int* later) {
   const int lane = threadIdx.x & 31;
-  auto look = [&](int s, long long slot, long long first, long long last, long long start) {
-    const int page = __ldg(b.table + s * b.table_stride + slot);
+  auto look = [&](int page, long long slot, long long first, long long last, long long start) {
     if (page < 0) return;
     for (int i = 0; i < count; ++i) {
+      if (page != places[i].page) continue;
       const long long at = first + (slot << c.page_bits) + places[i].row - start;
-      if (page == places[i].page && at > token0 + i && at >= first && at < last) later[i] = 1;
+      if (at > token0 + i && at >= first && at < last) later[i] = 1;
     }
   };
   for (int s0 = least + (threadIdx.x & ~31); s0 < b.batch; s0 += kThreads) {
@@ -82,15 +82,24 @@ __device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long 
         end = end > b.max_pages ? b.max_pages : end;
       }
     }
-    const long long own = slot + 4 < end ? slot + 4 : end;
-    for (; slot < own; ++slot) look(s, slot, first, last, start);
-    unsigned more = __ballot_sync(0xffffffffu, slot < end);
+    const int* pages = b.table + s * b.table_stride;
+    const int page0 = slot < end ? __ldg(pages + slot) : -1, page1 = slot + 1 < end ? __ldg(pages + slot + 1) : -1;
+    look(page0, slot, first, last, start);
+    look(page1, slot + 1, first, last, start);
+    unsigned more = __ballot_sync(0xffffffffu, slot + 2 < end);
     while (more) {
       const int from = __ffs(more) - 1;
       more &= more - 1;
       const long long f = __shfl_sync(0xffffffffu, first, from), l = __shfl_sync(0xffffffffu, last, from);
       const long long st = __shfl_sync(0xffffffffu, start, from), e = __shfl_sync(0xffffffffu, end, from);
-      for (long long k = __shfl_sync(0xffffffffu, slot, from) + lane; k < e; k += 32) look(s0 + from, k, f, l, st);
+      const int* row = b.table + (s0 + from) * b.table_stride;
+      for (long long k = __shfl_sync(0xffffffffu, slot, from) + 2 + lane; k < e; k += 128) {
+        int page[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) page[i] = k + 32 * i < e ? __ldg(row + k + 32 * i) : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) look(page[i], k + 32 * i, f, l, st);
+      }
     }
   }
 }

@@ -43,18 +43,12 @@ struct Params {
   float epsilon, by_width;
 };
 
-// cos and sin of position * frequency. The turns are taken in float64 (a far position has many of them
-// and float32 would lose the angle), reduced to a quarter turn and an eighth of a turn either way,
-// so that rounding the rest to float32 costs 2^-25 of an eighth of a turn at most.
+// cos and sin of position * frequency. The half turns are taken in float64 (a far position has many of them
+// and float32 would lose the angle) and reduced to one either way, so that rounding the rest to
+// float32 costs 2^-25 of a half turn at most.
 __device__ __forceinline__ void turn(double position, double frequency, float* c, float* s) {
-  const double quarters = position * (frequency * 0.63661977236758134308);  // 2 / pi
-  const double whole = rint(quarters);
-  float sv, cv;
-  sincospif(0.5f * (float)(quarters - whole), &sv, &cv);
-  const int k = (int)((long long)whole & 3);
-  const float a = (k & 1) ? sv : cv, b = (k & 1) ? cv : sv;
-  *c = (k == 1 || k == 2) ? -a : a;
-  *s = (k >= 2) ? -b : b;
+  const double halves = position * (frequency * 0.31830988618379067154);  // 1 / pi
+  sincospif((float)(halves - 2.0 * rint(0.5 * halves)), s, c);
 }
 
 __device__ __forceinline__ double position_of(const Params& p, long long token) {
@@ -146,8 +140,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
 }
 
 // Rows of 16-byte vectors. A group of `lanes` threads has one row: thread i of it holds two vectors, which in the turned
-// columns are the two halves of its pairs (or, interleaved, two neighbouring vectors), so that a
-// pair never leaves its thread. A CTA takes `tokens_each` tokens at a time, with `groups[side]` groups a side for each
+// columns are the two halves of its pairs (or, interleaved, two vectors of whole pairs), so that a
+// pair never leaves its thread, and neighbouring threads' vectors lie side by side. A CTA takes `tokens_each` tokens at a time, with `groups[side]` groups a side for each
 // (a side's heads in `passes` rounds); a group always has the same side and columns.
 //
 // Bound by HBM: each row is read and written once (backward: two read, one written). What has to be
@@ -162,7 +156,7 @@ constexpr int kStages = 4;
 constexpr size_t kMaxShared = 200 * 1024;
 
 struct Layout {
-  int lanes_log, groups[2], tokens_each, passes, threads, batch;
+  int items, lanes_log, groups[2], tokens_each, passes, threads, batch;
   size_t shared;
 };
 
@@ -234,16 +228,16 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
   // this thread's columns a and b, V of each, and the first of the frequencies that turn them (-1: none)
   int a, b, turn_a, turn_b;
   if (INTERLEAVED) {
-    a = 2 * item * V, b = a + V;
+    a = item * V, b = a + layout.items * V;
     turn_a = a < p.rotary ? a / 2 : -1, turn_b = b < p.rotary ? b / 2 : -1;
   } else {
     const int pairs = half / V;
     const bool paired = item < pairs;
-    a = paired ? item * V : p.rotary + 2 * (item - pairs) * V;
-    b = paired ? half + item * V : a + V;
+    a = paired ? item * V : p.rotary + (item - pairs) * V;
+    b = paired ? half + item * V : a + (layout.items - pairs) * V;
     turn_a = turn_b = paired ? item * V : -1;
   }
-  const bool has_a = working && a < p.width, has_b = working && b < p.width;
+  const bool has_a = working && item < layout.items, has_b = has_a && b < p.width;
   if (!has_a) a = 0;
   if (!has_b) b = 0;
   const unsigned slots_at = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + threadIdx.x * 16, slot = blockDim.x * 16;
@@ -262,14 +256,26 @@ __global__ void __launch_bounds__(kVecThreads[BACKWARD], kVecResident) norm_rota
   const int mine = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);  // this CTA's tiles, one at least
   const long long in_step = tile_step * s.in_t, grad_step = tile_step * s.grad_t, out_step = tile_step * s.out_t;
 
-  // angles of the batch of tiles that begins at token row token0
+  // angles of the batch of tiles that begins at token row token0; a thread's first is the same each time
   const int per_tile = layout.tokens_each * half;
+  auto angle_at = [&](int i, long long* token, int* f, int* at) {
+    const int tile = i / per_tile, in_tile = i - tile * per_tile, t = in_tile / half;
+    *f = in_tile - t * half;
+    *token = tile * tile_step + t;
+    *at = (tile * layout.tokens_each + t) * 2 * sines + *f;
+  };
+  long long angle_token = 0;
+  int angle_f = 0, angle_to = 0;
+  angle_at(threadIdx.x, &angle_token, &angle_f, &angle_to);
+  const double angle_frequency = p.frequencies[angle_f];
   auto angles_of = [&](long long token0, float* to) {
-    for (int i = threadIdx.x; i < layout.batch * per_tile; i += blockDim.x) {
-      const int tile = i / per_tile, in_tile = i - tile * per_tile, t = in_tile / half, f = in_tile - t * half;
-      const long long token = token0 + tile * tile_step + t;
-      float* at = to + (tile * layout.tokens_each + t) * 2 * sines + f;
-      if (token < p.tokens) turn(position_of(p, token), p.frequencies[f], at, at + sines);
+    if (threadIdx.x >= layout.batch * per_tile) return;
+    if (token0 + angle_token < p.tokens) turn(position_of(p, token0 + angle_token), angle_frequency, to + angle_to, to + angle_to + sines);
+    for (int i = threadIdx.x + blockDim.x; i < layout.batch * per_tile; i += blockDim.x) {  // only where one tile has more angles than the CTA threads
+      long long token;
+      int f, at;
+      angle_at(i, &token, &f, &at);
+      if (token0 + token < p.tokens) turn(position_of(p, token0 + token), p.frequencies[f], to + at, to + at + sines);
     }
   };
   const int token_floats = layout.tokens_each * 2 * sines, batch_floats = layout.batch * token_floats;
@@ -404,6 +410,7 @@ bool vectors(const Params& p, bool backward, Layout* out) {
     if (!whole(s.in, s.in_t, s.in_h) || !whole(s.out, s.out_t, s.out_h) || (backward && !whole(s.grad, s.grad_t, s.grad_h))) return false;
   const int single = p.width / V, items = p.interleaved ? (single + 1) / 2 : half / V + (single - p.rotary / V + 1) / 2;
   Layout l = {};
+  l.items = items;
   while ((1 << l.lanes_log) < items) ++l.lanes_log;
   if (l.lanes_log > 5) return false;
   const int most = kVecThreads[backward] >> l.lanes_log;
