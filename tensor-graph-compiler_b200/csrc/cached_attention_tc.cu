@@ -1,0 +1,626 @@
+// Attention over the int8 cache for many query rows at once (prompt pieces, larger trees) on tcgen05.
+//
+// A unit is one sequence, one key head and up to 128 query rows (tokens x the heads that share the
+// key head). One CTA an SM; its keys come in tiles of 128, even tiles to group 0 and odd ones to
+// group 1, two halves of the CTA that each keep their own maxima, sums and accumulator for the
+// same rows and are joined at the unit's end. While one group is in its softmax, the other's products run.
+//
+//   converters (4 warps): codes from the cache to 16-bit matrices in shared memory (128-byte
+//     swizzle; the next tile's codes are in registers by then), the scales, and a unit's queries.
+//   products (1 thread): S = Q K^T into the group's 128 columns of tensor memory; O += P V with P read from tensor
+//     memory and V as it lies (columns contiguous).
+//   softmax (2 x 4 warps, a thread per row): the row's maximum, then weights e^(s - m) times the value's
+//     scale as two bfloat16 parts (16 bits, as in the kernel for few rows), written over the scores
+//     they came from: 32 scores' columns hold 16 columns of leading and 16 of remaining parts.
+//     The accumulator is rescaled only when a maximum grows by more than 2^8, since the weights' sum
+//     and the products share whatever reference they were taken against.
+//
+// Bound by the softmax warps' issue slots: about 11 instructions a score against 3 x 128 x 2 tensor operations.
+// All waits are bounded (4 s); a CTA that gives up records status 2 and unwinds.
+#include <atomic>
+#include <type_traits>
+#include <cmath>
+
+#include "cached_attention.cuh"
+
+namespace {
+
+using namespace tgcb_attend;
+
+constexpr int kKeys = 128;
+constexpr int kGroupThreads = 128;
+constexpr int kConverters = 2 * kGroupThreads;           // first thread of the converters
+constexpr int kProducts = kConverters + 128;             // first thread of the warp that issues products
+constexpr int kTensorThreads = kProducts + 32;
+constexpr int kLeastTiles = 2;                           // one for each group
+constexpr int kStatusTimeout = 2;
+constexpr float kGrowth = 8.f;                           // of a maximum, in powers of two, before anything is rescaled
+
+template <int W>
+struct Memory {
+  static constexpr int TILE = kKeys * W * 2;
+  static constexpr int QUERIES = 0;
+  static constexpr int STAGES = kTensorRows * W * 2;     // group g: keys, then values
+  static constexpr int KEY_SCALES = STAGES + 4 * TILE;   // float [group][turn][128]
+  static constexpr int VALUE_SCALES = KEY_SCALES + 4 * kKeys * 4;
+  static constexpr int EXCHANGE = VALUE_SCALES + 4 * kKeys * 4;  // float [128][33]
+  static constexpr int ROWS = EXCHANGE + 128 * 33 * 4;   // float2 [parity][group][128]: maximum and sum
+  static constexpr int BYTES = ROWS + 4 * 128 * 8 + 1024;  // and room to begin on a 1024-byte boundary
+};
+
+struct Shared {
+  unsigned long long q_full, q_free, k_full[2], scaled[2][2], v_full[2], s_full[2], p_ready[2], pv_done[2], rows_full, x_full, x_free, drained;
+  unsigned tmem, valid[2][2];  // valid: a bit for each 16 keys of a tile whose page is there
+  int abort;
+};
+
+__device__ __forceinline__ unsigned at(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(at(bar)) : "memory");
+}
+
+// Waits for a barrier's phase; false when the CTA gives up.
+__device__ __forceinline__ bool wait(unsigned long long* bar, unsigned parity, Shared* sh, int* status) {
+  unsigned long long start = 0;
+  for (unsigned it = 0;; ++it) {
+    unsigned ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(at(bar)), "r"(parity)
+                 : "memory");
+    if (ok) return true;
+    if ((it & 255u) == 255u) {
+      if (*reinterpret_cast<volatile int*>(&sh->abort)) return false;
+      unsigned long long now;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+      if (start == 0) {
+        start = now;
+      } else if (now - start > 4000000000ull) {
+        *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+        atomicCAS(status, 0, kStatusTimeout);
+        return false;
+      }
+    }
+  }
+}
+
+// The same for a whole warp, of which one thread polls.
+__device__ __forceinline__ bool wait_warp(unsigned long long* bar, unsigned parity, Shared* sh, int* status) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = wait(bar, parity, sh, status);
+  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  __syncwarp();
+  return ok;
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void commit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(at(bar)) : "memory");
+}
+
+#define TGCB_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define TGCB_S8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+
+// 32 columns of a warp's 32 rows of tensor memory, a row a thread.
+__device__ __forceinline__ void load32(unsigned tmem, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : TGCB_R8(r, 0), TGCB_R8(r, 8), TGCB_R8(r, 16), TGCB_R8(r, 24)
+      : "r"(tmem));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store32(unsigned tmem, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(tmem),
+      TGCB_S8(r, 0), TGCB_S8(r, 8), TGCB_S8(r, 16), TGCB_S8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A matrix in shared memory with the 128-byte swizzle: rows of 128 bytes, eight to an atom. `lbo`: from one 128-byte
+// column block to the next where the columns are not the summed dimension.
+__device__ __forceinline__ unsigned long long matrix(unsigned start, unsigned lbo) {
+  return (unsigned long long)((start >> 4) & 0x3fffu) | (unsigned long long)((lbo >> 4) & 0x3fffu) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ void product_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned how, bool add) {
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p; }" ::"r"(d), "l"(a),
+               "l"(b), "r"(how), "r"((unsigned)add), "r"(0u)
+               : "memory");
+}
+__device__ __forceinline__ void product_ts(unsigned d, unsigned a, unsigned long long b, unsigned how, bool add) {
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p; }" ::"r"(d), "r"(a),
+               "l"(b), "r"(how), "r"((unsigned)add), "r"(0u)
+               : "memory");
+}
+
+// Two codes as float16, bytes 0 and 2 of a word: with the sign bit flipped they are x + 128, the low bits of 1024 + x
+// + 128.
+__device__ __forceinline__ unsigned half_codes(unsigned w, unsigned mask, unsigned magic) {
+  unsigned u, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x78;" : "=r"(u) : "r"(magic), "r"(w), "r"(mask));  // magic ^ (w & mask)
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x64806480u));
+  return r;
+}
+
+// The pieces of this CTA's share of the work, as every role walks through them.
+struct Walk {
+  const Cache& c;
+  const Batch& b;
+  const Args& a;
+  long long place, stop, chunk, unit;
+  Sequence q;
+  int s, from;
+  int head, tile, to, rows, tiles, all;  // of the present piece: `tiles` of 128 keys from `from`; positions below `all` are seen by all rows
+
+  __device__ __forceinline__ Walk(const Cache& c, const Batch& b, const Args& a, const Begin& begin, long long chunk)
+      : c(c), b(b), a(a), chunk(chunk) {
+    place = blockIdx.x * chunk;
+    stop = min(place + chunk, begin.total);
+    s = begin.sequence;
+    q = sequence_of<kTensorRows, kKeys>(b, a, s);
+    const int per = a.whole ? 1 : q.steps;
+    unit = begin.offset / per;
+    from = (int)(begin.offset - unit * per);
+  }
+  __device__ __forceinline__ bool next() {
+    if (place >= stop) return false;
+    while (unit >= (long long)c.heads * q.tiles) {
+      q = sequence_of<kTensorRows, kKeys>(b, a, ++s);
+      unit = 0;
+    }
+    head = (int)(unit / q.tiles), tile = (int)(unit - (long long)head * q.tiles);
+    to = q.steps;
+    if (!a.whole) to = stop - place < to - from ? from + (int)(stop - place) : to;
+    rows = min(kTensorRows, q.rows * a.group - tile * kTensorRows);
+    const int first = tile * kTensorRows / a.group, last = (tile * kTensorRows + rows - 1) / a.group;
+    auto clip = [&](long long v, int most) { return (int)(v < 0 ? 0 : v > most ? most : v); };
+    all = clip(a.visible ? q.start : q.start + first + 1, a.capacity);
+    const int end = a.visible ? to : min(to, (clip(q.start + last + 1, q.end) + kKeys - 1) / kKeys);
+    tiles = max(0, end - from);
+    return true;
+  }
+  __device__ __forceinline__ void advance() {
+    place += a.whole ? 1 : to - from;
+    ++unit;
+    from = 0;
+  }
+};
+
+template <typename T, int W>
+__device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, int* status) {
+  using M = Memory<W>;
+  constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;  // 16-code pieces of a row; rows a pass copies
+  constexpr bool HALF = sizeof(T) == 2 && !std::is_same_v<T, __nv_bfloat16>;
+  const int tid = threadIdx.x - kConverters, piece = tid % CH, in_pass = tid / CH;
+  const float factor = (HALF ? 1.f : kCodeScale) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
+  unsigned mask, flip, magic;
+  asm volatile("mov.u32 %0, 0x00ff00ff;" : "=r"(mask));
+  asm volatile("mov.u32 %0, 0x00800080;" : "=r"(flip));
+  asm volatile("mov.u32 %0, 0x64806480;" : "=r"(magic));
+  const bool wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)(a.q_t * 2) | (unsigned long long)(a.q_h * 2)) & 7u) == 0;
+  unsigned turns[2] = {0, 0}, units = 0;
+
+  while (walk.next()) {
+    if (walk.tiles > 0) {
+      const Sequence& q = walk.q;
+      const int head = walk.head;
+      // where a key's row lies, -1 where it is not there or not read
+      auto row_of = [&](int position) -> long long {
+        if (position >= q.end) return -1;
+        const int page = tgcb_kv::page_of(c, b, walk.s, position);
+        return page < 0 ? -1 : ((long long)page * c.heads + head) * c.page + (position & (c.page - 1));
+      };
+      auto scales_of = [&](int tile, float* ks, float* vs) {  // of key tid; whether it is there
+        const int position = (walk.from + tile) * kKeys + tid;
+        const long long row = row_of(position);
+        if (row < 0 && position < q.end && (tid & 15) == 0) atomicAdd(c.faults, 1);
+        *ks = row < 0 ? 0.f : c.key_scales[row], *vs = row < 0 ? 0.f : c.value_scales[row];
+        return row >= 0;
+      };
+      auto load = [&](const int8_t* from, int tile, uint4* raw) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const long long row = row_of((walk.from + tile) * kKeys + i * PER + in_pass);
+          raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(from + row * W) + piece);
+        }
+      };
+      auto store = [&](unsigned char* to, const uint4* raw, bool half) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int key = i * PER + in_pass;
+          const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint4 out[2];
+          unsigned* o = reinterpret_cast<unsigned*>(out);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // columns 4 j + {0, 2} and {1, 3}
+            o[2 * j] = half ? half_codes(w[j], mask, magic) : codes(w[j], mask, flip);
+            o[2 * j + 1] = half ? half_codes(w[j] >> 8, mask, magic) : codes(w[j] >> 8, mask, flip);
+          }
+          unsigned char* row = to + (piece / 4) * (kKeys * 128) + key * 128;
+          const int p0 = (piece % 4) * 2, odd = piece / 4;  // eight threads of a row meet all banks
+          *reinterpret_cast<uint4*>(row + 16 * ((p0 + odd) ^ (key & 7))) = odd ? out[1] : out[0];
+          *reinterpret_cast<uint4*>(row + 16 * ((p0 + 1 - odd) ^ (key & 7))) = odd ? out[0] : out[1];
+        }
+      };
+      uint4 keys[PASSES], values[PASSES];
+      float ks, vs;
+      bool held = scales_of(0, &ks, &vs);
+      load(c.keys, 0, keys);
+      load(c.values, 0, values);
+
+      // the unit's queries, their columns in the order in which `codes` leaves the keys'
+      if (units && !wait_warp(&sh->q_free, (units - 1) & 1, sh, status)) return;
+      for (int i = tid; i < kTensorRows * W / 4; i += 128) {
+        const int r = i / (W / 4), quad = i % (W / 4);
+        uint2 v = make_uint2(0, 0);
+        if (r < walk.rows) {
+          const int row = walk.tile * kTensorRows + r, token = row / a.group, in_group = row - token * a.group;
+          const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h + 4 * quad;
+          uint2 x;
+          if (wide_q) {
+            x = *reinterpret_cast<const uint2*>(p);
+          } else {
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
+            x = make_uint2(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16);
+          }
+          v = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));  // (0, 2), (1, 3)
+        }
+        const int in_row = quad % 16;
+        *reinterpret_cast<uint2*>(memory + M::QUERIES + (quad / 16) * (kTensorRows * 128) + r * 128 + 16 * ((in_row / 2) ^ (r & 7)) + 8 * (in_row & 1)) = v;
+      }
+      fence_async();
+      arrive(&sh->q_full);
+      ++units;
+
+      for (int t = 0; t < walk.tiles; ++t) {
+        const int g = t & 1;
+        const unsigned turn = turns[g]++;
+        unsigned char* stage = memory + M::STAGES + g * 2 * M::TILE;
+        if (turn && !wait_warp(&sh->s_full[g], (turn - 1) & 1, sh, status)) return;  // the last scores are there: their keys are used up
+        store(stage, keys, HALF);
+        float* scales = reinterpret_cast<float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
+        scales[tid] = ks * factor;
+        scales[tid + (M::VALUE_SCALES - M::KEY_SCALES) / 4] = vs * kCodeScale;
+        const unsigned there = __ballot_sync(0xffffffffu, held);
+        if ((tid & 31) == 0) reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1);
+        fence_async();
+        arrive(&sh->k_full[g]);
+        arrive(&sh->scaled[g][turn & 1]);  // of the softmax; k_full may be a phase further when it gets there
+        const bool more = t + 1 < walk.tiles;
+        if (more) {
+          held = scales_of(t + 1, &ks, &vs);
+          load(c.keys, t + 1, keys);
+        }
+        if (turn && !wait_warp(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;
+        store(stage + M::TILE, values, false);
+        fence_async();
+        arrive(&sh->v_full[g]);
+        if (more) load(c.values, t + 1, values);
+      }
+    }
+    walk.advance();
+  }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* memory, unsigned tmem, int* status) {
+  using M = Memory<W>;
+  constexpr bool HALF = !std::is_same_v<T, __nv_bfloat16>;
+  // float32 results; both factors float16 or both bfloat16; the values with their columns contiguous
+  constexpr unsigned kScores = 1u << 4 | (HALF ? 0u : 1u << 7 | 1u << 10) | (unsigned)(kKeys >> 3) << 17 | 8u << 24;
+  constexpr unsigned kOutputs = 1u << 4 | 1u << 7 | 1u << 10 | 1u << 16 | (unsigned)(W >> 3) << 17 | 8u << 24;
+  const unsigned queries = at(memory + M::QUERIES);
+  unsigned score_turns[2] = {0, 0}, output_turns[2] = {0, 0}, units = 0;
+  while (walk.next()) {
+    if (walk.tiles > 0) {
+      if (!wait(&sh->q_full, units++ & 1, sh, status)) return;
+      for (int t = 0; t <= walk.tiles; ++t) {
+        if (t < walk.tiles) {
+          const int g = t & 1;
+          const unsigned turn = score_turns[g]++;
+          if (!wait(&sh->k_full[g], turn & 1, sh, status)) return;
+          if (turn && !wait(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;  // the weights there are used up
+          fence_after();
+          const unsigned keys = at(memory + M::STAGES + g * 2 * M::TILE);
+#pragma unroll
+          for (int k = 0; k < W / 16; ++k) {
+            const unsigned to = (k / 4) * (kKeys * 128) + (k % 4) * 32;
+            product_ss(tmem + 2 * W + g * kKeys, matrix(queries + to, 16), matrix(keys + to, 16), kScores, k > 0);
+          }
+          commit(&sh->s_full[g]);
+          if (t + 1 == walk.tiles) commit(&sh->q_free);
+        }
+        if (t > 0) {
+          const int g = (t - 1) & 1;
+          const unsigned turn = output_turns[g]++;
+          if (!wait(&sh->p_ready[g], turn & 1, sh, status)) return;
+          if (!wait(&sh->v_full[g], turn & 1, sh, status)) return;
+          fence_after();
+          const unsigned values = at(memory + M::STAGES + g * 2 * M::TILE + M::TILE), weights = tmem + 2 * W + g * kKeys;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+              product_ts(tmem + g * W, weights + 32 * (k / 2) + 16 * part + 8 * (k % 2), matrix(values + k * 16 * 128, kKeys * 128), kOutputs,
+                         t > 2 || k > 0 || part > 0);
+          commit(&sh->pv_done[g]);
+        }
+      }
+    }
+    walk.advance();
+  }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, unsigned tmem,
+                                      int* status) {
+  using M = Memory<W>;
+  const int g = threadIdx.x / kGroupThreads, row = threadIdx.x % kGroupThreads;
+  const unsigned lanes = (unsigned)(row & ~31) << 16;
+  const unsigned scores = tmem + lanes + 2 * W + g * kKeys, sums = tmem + lanes + g * W;
+  const float cap2 = a.cap * 1.4426950408889634f;
+  const bool wide = out_wide<T>(a);
+  float* exchange = reinterpret_cast<float*>(memory + M::EXCHANGE) + row * 33;
+  unsigned turns = 0, pieces = 0, chunks = 0;
+
+  while (walk.next()) {
+    const Sequence& q = walk.q;
+    const int mine = walk.tile * kTensorRows + min(row, walk.rows - 1), token = mine / a.group;
+    const long long sees = a.visible ? q.start : q.start + token + 1;
+    const int limit = (int)(sees < 0 ? 0 : sees > a.capacity ? a.capacity : sees);
+    unsigned long long bits = 0;
+    if (a.visible) {
+      bits = (unsigned long long)__ldg(a.visible + q.first + token);
+      if (q.rows < 64) bits &= (1ull << q.rows) - 1;
+    }
+    float m = -INFINITY, sum = 0.f;
+    bool seen = false;
+    for (int t = g; t < walk.tiles; t += 2) {
+      const unsigned turn = turns++;
+      const int position = (walk.from + t) * kKeys;
+      if (!wait_warp(&sh->scaled[g][turn & 1], turn >> 1 & 1, sh, status) || !wait_warp(&sh->s_full[g], turn & 1, sh, status)) return;
+      fence_after();
+      const float* ks = reinterpret_cast<const float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
+      const float* vs = ks + (M::VALUE_SCALES - M::KEY_SCALES) / 4;
+      const unsigned word = sh->valid[g][turn & 1];
+      const bool inside = position + kKeys <= walk.all && word == 0x03030303u;
+      // the keys of 32 from column 32 ch that this row sees
+      auto seen_of = [&](int ch) -> unsigned {
+        if (inside) return 0xffffffffu;
+        const int first = position + 32 * ch, below = limit - first;
+        unsigned s = below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
+        if (a.visible) {
+          const long long since = first - q.start;
+          if (since >= 0 && since < 64) s |= (unsigned)(bits >> since);
+          if (since < 0 && since > -32) s |= (unsigned)(bits << -since);
+        }
+        const unsigned halves = word >> (8 * ch);
+        return s & ((halves & 1 ? 0xffffu : 0u) | (halves & 2 ? 0xffff0000u : 0u));
+      };
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ++ch) {
+        unsigned r[32];
+        load32(scores + 32 * ch, r);
+        const unsigned see = seen_of(ch);
+        seen = seen || see;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j);
+          float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
+          if (!inside) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (see >> (j + i)) & 1 ? x[i] : -INFINITY;
+          }
+          top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), top);
+        }
+      }
+      if (a.cap > 0) top = top == -INFINITY ? top : cap2 * tanh_of<T>(top);
+      const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, grown)) {
+        const float keep = grown ? exp2_fast(m - top) : 1.f;
+        m = grown ? top : m;
+        sum *= keep;
+        if (t > 1) {
+          if (!wait_warp(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;
+          fence_after();
+#pragma unroll 1
+          for (int ch = 0; ch < W / 32; ++ch) {
+            unsigned r[32];
+            load32(sums + 32 * ch, r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+            store32(sums + 32 * ch, r);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ++ch) {
+        unsigned r[32], parts[32];
+        load32(scores + 32 * ch, r);
+        const unsigned see = seen_of(ch);
+        float some[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j), v = *reinterpret_cast<const float4*>(vs + 32 * ch + j);
+          float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
+          const float scale[4] = {v.x, v.y, v.z, v.w};
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (a.cap > 0) x[i] = cap2 * tanh_of<T>(x[i]);
+            float p = exp2_fast(x[i] - base);
+            w[i] = p * scale[i];
+            if (!inside && !((see >> (j + i)) & 1)) p = 0.f, w[i] = 0.f;  // whatever lies there
+            some[i] += p;
+          }
+          unsigned two[2];
+          split<2>(w[0], w[1], two);
+          parts[j / 2] = two[0], parts[16 + j / 2] = two[1];
+          split<2>(w[2], w[3], two);
+          parts[j / 2 + 1] = two[0], parts[16 + j / 2 + 1] = two[1];
+        }
+        sum += (some[0] + some[1]) + (some[2] + some[3]);
+        store32(scores + 32 * ch, parts);
+      }
+      stored();
+      fence_before();
+      arrive(&sh->p_ready[g]);
+    }
+
+    // join the groups: maxima and sums through shared memory, then 32 columns at a time
+    const bool any = g < walk.tiles;
+    if (any && !wait_warp(&sh->pv_done[g], (turns - 1) & 1, sh, status)) return;
+    fence_after();
+    float2* rows = reinterpret_cast<float2*>(memory + M::ROWS) + (pieces & 1) * 256;
+    rows[g * 128 + row] = make_float2(m, seen && m == -INFINITY ? -1.f : sum);
+    arrive(&sh->rows_full);
+    if (!wait_warp(&sh->rows_full, pieces++ & 1, sh, status)) return;
+    const float2 other = rows[(g ^ 1) * 128 + row], own = rows[g * 128 + row];
+    const float mm = fmaxf(own.x, other.x), base = mm == -INFINITY ? 0.f : mm;
+    const float factor = exp2_fast(own.x - base);
+    const bool complete = walk.from == 0 && walk.to == q.steps;
+    float* part = complete ? nullptr : a.parts + (2ll * blockIdx.x + (walk.from == 0)) * kTensorRows * (W + 2);
+    float all_sum = 0.f;
+    add_sum(&all_sum, own.y, factor);
+    add_sum(&all_sum, other.y, exp2_fast(other.x - base));
+    const bool two = walk.tiles > 1;
+    T* out = out_row<T>(a, q, walk.head, mine);
+#pragma unroll 1
+    for (int ch = 0; ch < W / 32; ++ch) {
+      unsigned r[32];
+      if (any) load32(sums + 32 * ch, r);
+      if (g == 1) {
+        if (!two) break;
+        if (chunks && !wait_warp(&sh->x_free, (chunks - 1) & 1, sh, status)) return;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) exchange[j] = __uint_as_float(r[j]) * factor;
+        arrive(&sh->x_full);
+        ++chunks;
+        continue;
+      }
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = any ? __uint_as_float(r[j]) * factor : 0.f;
+      if (two) {
+        if (!wait_warp(&sh->x_full, chunks++ & 1, sh, status)) return;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += exchange[j];
+        arrive(&sh->x_free);
+      }
+      if (row < walk.rows) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float x[4] = {v[j], v[j + 2], v[j + 1], v[j + 3]};  // the columns' order
+          if (complete) {
+            const float y[4] = {answer(x[0], all_sum), answer(x[1], all_sum), answer(x[2], all_sum), answer(x[3], all_sum)};
+            store4<T>(out + 32 * ch + j, y, wide);
+          } else {
+            *reinterpret_cast<float2*>(part + row * W + 32 * ch + j) = make_float2(x[0], x[1]);
+            *reinterpret_cast<float2*>(part + row * W + 32 * ch + j + 2) = make_float2(x[2], x[3]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    __syncwarp();
+    fence_before();
+    if (!complete && g == 0) {
+      if (row < walk.rows) *reinterpret_cast<float2*>(part + kTensorRows * W + 2 * row) = make_float2(mm, all_sum);
+      if (walk.from == 0 && row == 0) a.cuts[blockIdx.x] = make_int4(walk.s, walk.head, walk.tile, (int)((walk.place + q.steps - 1) / walk.chunk));
+    }
+    walk.advance();
+  }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kTensorThreads, 1) attend_tiles(const Cache c, const Batch b, const Args a, int* status) {
+  extern __shared__ unsigned char raw[];
+  __shared__ Shared sh;
+  __shared__ Begin begin;
+  asm volatile("griddepcontrol.launch_dependents;");
+  unsigned char* memory = raw + ((1024u - (at(raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    auto init = [](unsigned long long* bar, unsigned count) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at(bar)), "r"(count));
+    };
+    init(&sh.q_full, 128), init(&sh.q_free, 1), init(&sh.rows_full, 256), init(&sh.x_full, 128), init(&sh.x_free, 128), init(&sh.drained, 1);
+    for (int g = 0; g < 2; ++g) {
+      init(&sh.k_full[g], 128), init(&sh.scaled[g][0], 128), init(&sh.scaled[g][1], 128), init(&sh.v_full[g], 128), init(&sh.s_full[g], 1), init(&sh.p_ready[g], 128), init(&sh.pv_done[g], 1);
+      sh.valid[g][0] = sh.valid[g][1] = 0;
+    }
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kProducts / 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at(&sh.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  long long chunk;
+  fence_before();
+  begin_at<kTensorRows, kKeys, kTensorThreads / 32>(c, b, a, kLeastTiles, &chunk, &begin);  // ends with a barrier
+  fence_after();
+  const unsigned tmem = sh.tmem;
+  if (!a.whole && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  __syncthreads();  // a cut that is written below comes after
+  if (blockIdx.x * chunk < begin.total) {
+    const Walk walk(c, b, a, begin, chunk);
+    if (threadIdx.x < kConverters) {
+      weigh<T, W>(c, b, a, walk, &sh, memory, tmem, status);
+    } else if (threadIdx.x < kProducts) {
+      convert<T, W>(c, b, a, walk, &sh, memory, status);
+    } else if (threadIdx.x == kProducts) {
+      multiply<T, W>(walk, &sh, memory, tmem, status);
+      commit(&sh.drained);  // whatever was queued has ended before the memory is given back
+      wait(&sh.drained, 0, &sh, status);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == kProducts / 32) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+template <typename T, int W>
+int launch(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
+  const char* what = "tgcb_cached_attention";
+  int dev = 0, *status = nullptr;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+  const int rc = tgcb_internal_status_word(&status);
+  if (rc != TGCB_OK) return rc;
+  static std::atomic<unsigned long long> configured{0};
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    e = cudaFuncSetAttribute(attend_tiles<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Memory<W>::BYTES);
+    if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+    configured.fetch_or(bit);
+  }
+  const long long tiles = (b.tokens * a.group + kTensorRows - 1) / kTensorRows + b.batch;
+  const long long steps = a.whole ? 1 : (a.capacity + kKeys - 1) / kKeys;
+  const long long pieces = (tiles * c.heads * steps + (a.whole ? 0 : kLeastTiles - 1)) / (a.whole ? 1 : kLeastTiles);
+  const unsigned grid = (unsigned)(pieces < kTensorCtas ? pieces : kTensorCtas);
+  attend_tiles<T, W><<<grid, kTensorThreads, Memory<W>::BYTES, s>>>(c, b, a, status);
+  e = cudaGetLastError();
+  if (e == cudaSuccess && !a.whole) e = launch_combine<T, W, kTensorRows / 8>(c, b, a, grid, s);
+  if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
+  return TGCB_OK;
+}
+
+}  // namespace
+
+int tgcb_attend::attend_tensor(const Cache& c, const Batch& b, const Args& a, int dtype, cudaStream_t s) {
+  if (dtype == TGCB_BF16) return c.width == 128 ? launch<__nv_bfloat16, 128>(c, b, a, s) : launch<__nv_bfloat16, 64>(c, b, a, s);
+  return c.width == 128 ? launch<__half, 128>(c, b, a, s) : launch<__half, 64>(c, b, a, s);
+}
