@@ -211,25 +211,26 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
     if (walk.tiles > 0) {
       const Sequence& q = walk.q;
       const int head = walk.head;
-      // where a key's row lies, -1 where it is not there or not read
-      auto row_of = [&](int position) -> long long {
-        if (position >= q.end) return -1;
+      // The rows of a tile's first keys of each 16 (one page holds them), a lane each: -1 where they are not there or not
+      // read. With widths from 64 a cache in memory has fewer than 2^31 rows.
+      auto rows_of = [&](int tile) {
+        const int lane = tid & 31, position = (walk.from + tile) * kKeys + 16 * lane;
+        if (lane >= 8 || tile >= walk.tiles || position >= q.end) return -1;
         const int page = tgcb_kv::page_of(c, b, walk.s, position);
-        return page < 0 ? -1 : ((long long)page * c.heads + head) * c.page + (position & (c.page - 1));
+        if (page < 0 && tid < 32) atomicAdd(c.faults, 1);
+        return page < 0 ? -1 : (page * c.heads + head) * c.page + (position & (c.page - 1));
       };
-      auto scales_of = [&](int tile, float* ks, float* vs) {  // of key tid; whether it is there
-        const int position = (walk.from + tile) * kKeys + tid;
-        const long long row = row_of(position);
-        if (row < 0 && position < q.end && (tid & 15) == 0) atomicAdd(c.faults, 1);
-        *ks = row < 0 ? 0.f : c.key_scales[row], *vs = row < 0 ? 0.f : c.value_scales[row];
-        return row >= 0;
-      };
-      auto load = [&](const int8_t* from, int tile, uint4* raw) {
+      auto load = [&](const int8_t* from, int rows, uint4* raw) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const long long row = row_of((walk.from + tile) * kKeys + i * PER + in_pass);
-          raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(from + row * W) + piece);
+          const int row = __shfl_sync(0xffffffffu, rows, (i * PER + (tid & ~31) / CH) / 16);
+          raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(from + (long long)(row + in_pass % 16) * W) + piece);
         }
+      };
+      auto scales_of = [&](int rows, float* ks, float* vs) {  // of key tid; whether its page is there
+        const int row = __shfl_sync(0xffffffffu, rows, tid / 16);
+        *ks = row < 0 ? 0.f : c.key_scales[row + tid % 16], *vs = row < 0 ? 0.f : c.value_scales[row + tid % 16];
+        return row >= 0;
       };
       auto store = [&](unsigned char* to, const uint4* raw, bool half) {
 #pragma unroll
@@ -251,9 +252,11 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
       };
       uint4 keys[PASSES], values[PASSES];
       float ks, vs;
-      bool held = scales_of(0, &ks, &vs);
-      load(c.keys, 0, keys);
-      load(c.values, 0, values);
+      int rows = rows_of(0);
+      bool held = scales_of(rows, &ks, &vs);
+      load(c.keys, rows, keys);
+      load(c.values, rows, values);
+      rows = rows_of(1);
 
       // the unit's queries, their columns in the order in which `codes` leaves the keys'
       if (units && !wait_warp(&sh->q_free, (units - 1) & 1, sh, status)) return;
@@ -295,14 +298,17 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
         arrive(&sh->scaled[g][turn & 1]);  // of the softmax; k_full may be a phase further when it gets there
         const bool more = t + 1 < walk.tiles;
         if (more) {
-          held = scales_of(t + 1, &ks, &vs);
-          load(c.keys, t + 1, keys);
+          held = scales_of(rows, &ks, &vs);
+          load(c.keys, rows, keys);
         }
         if (turn && !wait_warp(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;
         store(stage + M::TILE, values, false);
         fence_async();
         arrive(&sh->v_full[g]);
-        if (more) load(c.values, t + 1, values);
+        if (more) {
+          load(c.values, rows, values);
+          rows = rows_of(t + 2);
+        }
       }
     }
     walk.advance();
@@ -358,6 +364,63 @@ __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* m
   }
 }
 
+// The largest of a row's 128 scaled scores, of those alone that `seen_of` shows where MASKED.
+template <bool MASKED, class Seen>
+__device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen seen_of) {
+  float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int ch = 0; ch < 4; ++ch) {
+    unsigned r[32];
+    load32(scores + 32 * ch, r);
+    const unsigned see = MASKED ? seen_of(ch) : 0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j);
+      float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
+      if (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (see >> (j + i)) & 1 ? x[i] : -INFINITY;
+      }
+      top[0] = fmaxf(top[0], fmaxf(x[0], x[1])), top[1] = fmaxf(top[1], fmaxf(x[2], x[3]));
+    }
+  }
+  return fmaxf(top[0], top[1]);
+}
+
+// Writes a row's 128 weights times the values' scales over its scores, 32 at a time as 16 columns of leading and 16 of
+// remaining parts, and returns the weights' sum.
+template <typename T, bool CAP, bool MASKED, class Seen>
+__device__ __forceinline__ float weights(unsigned scores, const float* ks, const float* vs, float base, float cap2, Seen seen_of) {
+  float some[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int ch = 0; ch < 4; ++ch) {
+    unsigned r[32], parts[32];
+    load32(scores + 32 * ch, r);
+    const unsigned see = MASKED ? seen_of(ch) : 0;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j), v = *reinterpret_cast<const float4*>(vs + 32 * ch + j);
+      const float by[4] = {k.x, k.y, k.z, k.w}, scale[4] = {v.x, v.y, v.z, v.w};
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float s = __uint_as_float(r[j + i]);
+        float p = exp2_fast(CAP ? fmaf(cap2, tanh_of<T>(s * by[i]), -base) : fmaf(s, by[i], -base));
+        w[i] = p * scale[i];
+        if (MASKED && !((see >> (j + i)) & 1)) p = 0.f, w[i] = 0.f;  // whatever lies there
+        some[i] += p;
+      }
+      unsigned two[2];
+      split<2>(w[0], w[1], two);
+      parts[j / 2] = two[0], parts[16 + j / 2] = two[1];
+      split<2>(w[2], w[3], two);
+      parts[j / 2 + 1] = two[0], parts[16 + j / 2 + 1] = two[1];
+    }
+    store32(scores + 32 * ch, parts);
+  }
+  return (some[0] + some[1]) + (some[2] + some[3]);
+}
+
 template <typename T, int W>
 __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, unsigned tmem,
                                       int* status) {
@@ -393,7 +456,6 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
       const bool inside = position + kKeys <= walk.all && word == 0x03030303u;
       // the keys of 32 from column 32 ch that this row sees
       auto seen_of = [&](int ch) -> unsigned {
-        if (inside) return 0xffffffffu;
         const int first = position + 32 * ch, below = limit - first;
         unsigned s = below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
         if (a.visible) {
@@ -405,22 +467,12 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         return s & ((halves & 1 ? 0xffffu : 0u) | (halves & 2 ? 0xffff0000u : 0u));
       };
       float top = -INFINITY;
-#pragma unroll 1
-      for (int ch = 0; ch < 4; ++ch) {
-        unsigned r[32];
-        load32(scores + 32 * ch, r);
-        const unsigned see = seen_of(ch);
-        seen = seen || see;
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j);
-          float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
-          if (!inside) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (see >> (j + i)) & 1 ? x[i] : -INFINITY;
-          }
-          top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), top);
-        }
+      if (inside) {
+        top = top_of<false>(scores, ks, seen_of);
+        seen = true;
+      } else {
+        top = top_of<true>(scores, ks, seen_of);
+        seen = seen || seen_of(0) || seen_of(1) || seen_of(2) || seen_of(3);
       }
       if (a.cap > 0) top = top == -INFINITY ? top : cap2 * tanh_of<T>(top);
       const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
@@ -442,35 +494,10 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-      for (int ch = 0; ch < 4; ++ch) {
-        unsigned r[32], parts[32];
-        load32(scores + 32 * ch, r);
-        const unsigned see = seen_of(ch);
-        float some[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j), v = *reinterpret_cast<const float4*>(vs + 32 * ch + j);
-          float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
-          const float scale[4] = {v.x, v.y, v.z, v.w};
-          float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (a.cap > 0) x[i] = cap2 * tanh_of<T>(x[i]);
-            float p = exp2_fast(x[i] - base);
-            w[i] = p * scale[i];
-            if (!inside && !((see >> (j + i)) & 1)) p = 0.f, w[i] = 0.f;  // whatever lies there
-            some[i] += p;
-          }
-          unsigned two[2];
-          split<2>(w[0], w[1], two);
-          parts[j / 2] = two[0], parts[16 + j / 2] = two[1];
-          split<2>(w[2], w[3], two);
-          parts[j / 2 + 1] = two[0], parts[16 + j / 2 + 1] = two[1];
-        }
-        sum += (some[0] + some[1]) + (some[2] + some[3]);
-        store32(scores + 32 * ch, parts);
-      }
+      if (a.cap > 0)
+        sum += inside ? weights<T, true, false>(scores, ks, vs, base, cap2, seen_of) : weights<T, true, true>(scores, ks, vs, base, cap2, seen_of);
+      else
+        sum += inside ? weights<T, false, false>(scores, ks, vs, base, cap2, seen_of) : weights<T, false, true>(scores, ks, vs, base, cap2, seen_of);
       stored();
       fence_before();
       arrive(&sh->p_ready[g]);
