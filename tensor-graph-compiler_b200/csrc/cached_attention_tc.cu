@@ -65,12 +65,12 @@ __device__ __forceinline__ bool wait(unsigned long long* bar, unsigned parity, S
   unsigned long long start = 0;
   for (unsigned it = 0;; ++it) {
     unsigned ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
                  : "=r"(ok)
-                 : "r"(at(bar)), "r"(parity)
+                 : "r"(at(bar)), "r"(parity), "r"(100000u)  // nanoseconds that the hardware may wait
                  : "memory");
     if (ok) return true;
-    if ((it & 255u) == 255u) {
+    if ((it & 15u) == 15u) {
       if (*reinterpret_cast<volatile int*>(&sh->abort)) return false;
       unsigned long long now;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
@@ -109,10 +109,10 @@ __device__ __forceinline__ void commit(unsigned long long* bar) {
 __device__ __forceinline__ void load32(unsigned tmem, unsigned* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32]; tcgen05.wait::ld.sync.aligned;"
       : TGCB_R8(r, 0), TGCB_R8(r, 8), TGCB_R8(r, 16), TGCB_R8(r, 24)
-      : "r"(tmem));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(tmem)
+      : "memory");
 }
 __device__ __forceinline__ void store32(unsigned tmem, const unsigned* r) {
   asm volatile(
@@ -196,15 +196,17 @@ struct Walk {
 template <typename T, int W>
 __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, int* status) {
   using M = Memory<W>;
-  constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;  // 16-code pieces of a row; rows a pass copies
+  // 16-code pieces of a row; rows a pass copies. Eight neighbouring threads have four pieces of two rows, whose halves lie on
+  // different banks.
+  constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;
   constexpr bool HALF = sizeof(T) == 2 && !std::is_same_v<T, __nv_bfloat16>;
-  const int tid = threadIdx.x - kConverters, piece = tid % CH, in_pass = tid / CH;
+  const int tid = threadIdx.x - kConverters, piece = tid % 4 + (W == 128 ? tid / 64 * 4 : 0), in_pass = W == 128 ? tid % 64 / 4 : tid / 4;
   const float factor = (HALF ? 1.f : kCodeScale) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
   unsigned mask, flip, magic;
   asm volatile("mov.u32 %0, 0x00ff00ff;" : "=r"(mask));
   asm volatile("mov.u32 %0, 0x00800080;" : "=r"(flip));
   asm volatile("mov.u32 %0, 0x64806480;" : "=r"(magic));
-  const bool wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)(a.q_t * 2) | (unsigned long long)(a.q_h * 2)) & 7u) == 0;
+  const bool wide_q = ((reinterpret_cast<uintptr_t>(a.q) | (unsigned long long)(a.q_t * 2) | (unsigned long long)(a.q_h * 2)) & 15u) == 0;
   unsigned turns[2] = {0, 0}, units = 0;
 
   while (walk.next()) {
@@ -223,7 +225,7 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
       auto load = [&](const int8_t* from, int rows, uint4* raw) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int row = __shfl_sync(0xffffffffu, rows, (i * PER + (tid & ~31) / CH) / 16);
+          const int row = __shfl_sync(0xffffffffu, rows, W == 128 ? i : 2 * i + tid / 64);
           raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(from + (long long)(row + in_pass % 16) * W) + piece);
         }
       };
@@ -245,9 +247,8 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
             o[2 * j + 1] = half ? half_codes(w[j] >> 8, mask, magic) : codes(w[j] >> 8, mask, flip);
           }
           unsigned char* row = to + (piece / 4) * (kKeys * 128) + key * 128;
-          const int p0 = (piece % 4) * 2, odd = piece / 4;  // eight threads of a row meet all banks
-          *reinterpret_cast<uint4*>(row + 16 * ((p0 + odd) ^ (key & 7))) = odd ? out[1] : out[0];
-          *reinterpret_cast<uint4*>(row + 16 * ((p0 + 1 - odd) ^ (key & 7))) = odd ? out[0] : out[1];
+          *reinterpret_cast<uint4*>(row + 16 * ((2 * (piece % 4)) ^ (key & 7))) = out[0];
+          *reinterpret_cast<uint4*>(row + 16 * ((2 * (piece % 4) + 1) ^ (key & 7))) = out[1];
         }
       };
       uint4 keys[PASSES], values[PASSES];
@@ -260,23 +261,32 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
 
       // the unit's queries, their columns in the order in which `codes` leaves the keys'
       if (units && !wait_warp(&sh->q_free, (units - 1) & 1, sh, status)) return;
-      for (int i = tid; i < kTensorRows * W / 4; i += 128) {
-        const int r = i / (W / 4), quad = i % (W / 4);
-        uint2 v = make_uint2(0, 0);
-        if (r < walk.rows) {
-          const int row = walk.tile * kTensorRows + r, token = row / a.group, in_group = row - token * a.group;
-          const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h + 4 * quad;
-          uint2 x;
-          if (wide_q) {
-            x = *reinterpret_cast<const uint2*>(p);
-          } else {
-            const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
-            x = make_uint2(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16);
+      constexpr int EIGHTS = W / 8, ROUNDS = kTensorRows * EIGHTS / 128, SOME = 8;  // 8-column pieces of a row; SOME in flight
+#pragma unroll 1
+      for (int i0 = 0; i0 < ROUNDS; i0 += SOME) {
+        uint4 v[SOME];
+#pragma unroll
+        for (int i = 0; i < SOME; ++i) {
+          const int r = ((i0 + i) * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r < walk.rows) {
+            const int row = walk.tile * kTensorRows + r, token = row / a.group, in_group = row - token * a.group;
+            const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h + 8 * eight;
+            if (wide_q) {
+              v[i] = *reinterpret_cast<const uint4*>(p);
+            } else {
+              const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
+              v[i] = make_uint4(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16, e[4] | (unsigned)e[5] << 16, e[6] | (unsigned)e[7] << 16);
+            }
           }
-          v = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));  // (0, 2), (1, 3)
         }
-        const int in_row = quad % 16;
-        *reinterpret_cast<uint2*>(memory + M::QUERIES + (quad / 16) * (kTensorRows * 128) + r * 128 + 16 * ((in_row / 2) ^ (r & 7)) + 8 * (in_row & 1)) = v;
+#pragma unroll
+        for (int i = 0; i < SOME; ++i) {
+          const int r = ((i0 + i) * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
+          const uint4 x = v[i];  // each four columns as (0, 2), (1, 3)
+          *reinterpret_cast<uint4*>(memory + M::QUERIES + (eight / 8) * (kTensorRows * 128) + r * 128 + 16 * ((eight % 8) ^ (r & 7))) =
+              make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+        }
       }
       fence_async();
       arrive(&sh->q_full);
@@ -364,6 +374,20 @@ __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* m
   }
 }
 
+// Whether rows of 16-bit outputs lie on 16-byte boundaries, and eight of their columns stored.
+__device__ __forceinline__ bool out_whole(const Args& a) {
+  return ((reinterpret_cast<uintptr_t>(a.out) | (unsigned long long)(a.out_t * 2) | (unsigned long long)(a.out_h * 2)) & 15u) == 0;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v, bool whole) {
+  if (whole) {
+    store_vec<T>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = from_float<T>(v[i]);
+  }
+}
+
 // The largest of a row's 128 scaled scores, of those alone that `seen_of` shows where MASKED.
 template <bool MASKED, class Seen>
 __device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen seen_of) {
@@ -429,7 +453,7 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
   const unsigned lanes = (unsigned)(row & ~31) << 16;
   const unsigned scores = tmem + lanes + 2 * W + g * kKeys, sums = tmem + lanes + g * W;
   const float cap2 = a.cap * 1.4426950408889634f;
-  const bool wide = out_wide<T>(a);
+  const bool wide = out_whole(a);
   float* exchange = reinterpret_cast<float*>(memory + M::EXCHANGE) + row * 33;
   unsigned turns = 0, pieces = 0, chunks = 0;
 
@@ -543,25 +567,29 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         for (int j = 0; j < 32; ++j) v[j] += exchange[j];
         arrive(&sh->x_free);
       }
-      if (row < walk.rows) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float x[4] = {v[j], v[j + 2], v[j + 1], v[j + 3]};  // the columns' order
-          if (complete) {
-            const float y[4] = {answer(x[0], all_sum), answer(x[1], all_sum), answer(x[2], all_sum), answer(x[3], all_sum)};
-            store4<T>(out + 32 * ch + j, y, wide);
-          } else {
-            *reinterpret_cast<float2*>(part + row * W + 32 * ch + j) = make_float2(x[0], x[1]);
-            *reinterpret_cast<float2*>(part + row * W + 32 * ch + j + 2) = make_float2(x[2], x[3]);
-          }
+      for (int j = 0; j < 32; j += 4) {  // the columns' order
+        const float x = v[j + 1];
+        v[j + 1] = v[j + 2], v[j + 2] = x;
+      }
+      if (complete) {
+        const float by = all_sum > 0.f ? 1.f / all_sum : answer(0.f, all_sum);  // nothing seen: times zero
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[j + i] *= by;
+          if (row < walk.rows) store8<T>(out + 32 * ch + j, v + j, wide);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part[(32 * ch + j) * kTensorRows + row] = v[j];
       }
       __syncwarp();
     }
     __syncwarp();
     fence_before();
     if (!complete && g == 0) {
-      if (row < walk.rows) *reinterpret_cast<float2*>(part + kTensorRows * W + 2 * row) = make_float2(mm, all_sum);
+      part[W * kTensorRows + row] = mm, part[(W + 1) * kTensorRows + row] = all_sum;
       if (walk.from == 0 && row == 0) a.cuts[blockIdx.x] = make_int4(walk.s, walk.head, walk.tile, (int)((walk.place + q.steps - 1) / walk.chunk));
     }
     walk.advance();
@@ -619,6 +647,42 @@ __global__ void __launch_bounds__(kTensorThreads, 1) attend_tiles(const Cache c,
   }
 }
 
+// Joins the parts of the unit that begins in CTA blockIdx.x and was cut at its end, in the order of the keys: a thread per
+// row, kColumns columns a CTA, since the parts lie column by column (a row is a thread where they are made).
+constexpr int kColumns = 16;
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kTensorRows) join_columns(const Cache c, const Batch b, const Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.x < 0) return;
+  const Sequence q = sequence_of<kTensorRows, kKeys>(b, a, cut.x);
+  const int row = threadIdx.x, column = blockIdx.y * kColumns, n = cut.w - blockIdx.x + 1;
+  auto part = [&](int i) { return a.parts + (i == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + i)) * kTensorRows * (W + 2) + row; };
+  float mm = -INFINITY;
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) mm = fmaxf(mm, part(k)[W * kTensorRows]);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float all_sum = 0.f, v[kColumns];
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i) v[i] = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const float* p = part(k);
+    const float f = exp2_fast(p[W * kTensorRows] - base);
+    add_sum(&all_sum, p[(W + 1) * kTensorRows], f);
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i) v[i] = fmaf(p[(column + i) * kTensorRows], f, v[i]);
+  }
+  if (row >= q.rows * a.group - cut.z * kTensorRows) return;
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i) v[i] = answer(v[i], all_sum);
+  T* out = out_row<T>(a, q, cut.y, cut.z * kTensorRows + row) + column;
+  const bool whole = out_whole(a);
+#pragma unroll
+  for (int i = 0; i < kColumns; i += 8) store8<T>(out + i, v + i, whole);
+}
+
 template <typename T, int W>
 int launch(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
   const char* what = "tgcb_cached_attention";
@@ -640,7 +704,18 @@ int launch(const Cache& c, const Batch& b, const Args& a, cudaStream_t s) {
   const unsigned grid = (unsigned)(pieces < kTensorCtas ? pieces : kTensorCtas);
   attend_tiles<T, W><<<grid, kTensorThreads, Memory<W>::BYTES, s>>>(c, b, a, status);
   e = cudaGetLastError();
-  if (e == cudaSuccess && !a.whole) e = launch_combine<T, W, kTensorRows / 8>(c, b, a, grid, s);
+  if (e == cudaSuccess && !a.whole) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, W / kColumns);
+    cfg.blockDim = dim3(kTensorRows);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, join_columns<T, W>, c, b, a);
+  }
   if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, what, cudaGetErrorString(e));
   return TGCB_OK;
 }
