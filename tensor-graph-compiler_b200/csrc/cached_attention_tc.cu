@@ -5,8 +5,9 @@
 // group 1, two halves of the CTA that each keep their own maxima, sums and accumulator for the
 // same rows and are joined at the unit's end. While one group is in its softmax, the other's products run.
 //
-//   converters (4 warps): codes from the cache to 16-bit matrices in shared memory (128-byte
-//     swizzle; the next tile's codes are in registers by then), the scales, and a unit's queries.
+//   converters (4 warps for the keys, 4 for the values): codes from the cache to 16-bit matrices in shared memory
+//     (128-byte swizzle; the next tile's codes are in registers by then); the first also bring the scales, the
+//     others a unit's queries.
 //   products (1 thread): S = Q K^T into the group's 128 columns of tensor memory; O += P V with P read from tensor
 //     memory and V as it lies (columns contiguous).
 //   softmax (2 x 4 warps, a thread per row): the row's maximum, then weights e^(s - m) times the value's
@@ -29,9 +30,14 @@ using namespace tgcb_attend;
 
 constexpr int kKeys = 128;
 constexpr int kGroupThreads = 128;
-constexpr int kConverters = 2 * kGroupThreads;           // first thread of the converters
-constexpr int kProducts = kConverters + 128;             // first thread of the warp that issues products
-constexpr int kTensorThreads = kProducts + 32;
+constexpr int kKeyThreads = 2 * kGroupThreads;           // first thread of the keys' converters
+constexpr int kValueThreads = kKeyThreads + 128;         // of the values'
+constexpr int kProducts = kValueThreads + 128;           // of the four warps of which one thread issues products
+constexpr int kTensorThreads = kProducts + 128;
+// Registers a thread: the launch gives 96 to each of the five groups of 128, 480 in all, which the
+// roles share out between them.
+constexpr int kSoftmaxRegisters = 136, kConverterRegisters = 80, kProductRegisters = 48;
+static_assert(2 * kSoftmaxRegisters + 2 * kConverterRegisters + kProductRegisters <= 5 * 96, "the launch has no more registers");
 constexpr int kLeastTiles = 2;                           // one for each group
 constexpr int kStatusTimeout = 2;
 constexpr float kGrowth = 8.f;                           // of a maximum, in powers of two, before anything is rescaled
@@ -98,6 +104,15 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void commit(unsigned long long* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(at(bar)) : "memory");
 }
@@ -149,6 +164,12 @@ __device__ __forceinline__ unsigned half_codes(unsigned w, unsigned mask, unsign
   return r;
 }
 
+// 16 bytes of codes, loaded where it stands: a plain load of constant memory may be moved down to its use, which is a
+// tile later.
+__device__ __forceinline__ void load_now(uint4* to, const int8_t* from) {
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to->x), "=r"(to->y), "=r"(to->z), "=r"(to->w) : "l"(from));
+}
+
 // The pieces of this CTA's share of the work, as every role walks through them.
 struct Walk {
   const Cache& c;
@@ -193,14 +214,14 @@ struct Walk {
   }
 };
 
-template <typename T, int W>
+template <typename T, int W, bool VALUES>
 __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, int* status) {
   using M = Memory<W>;
   // 16-code pieces of a row; rows a pass copies. Eight neighbouring threads have four pieces of two rows, whose halves lie on
   // different banks.
   constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;
-  constexpr bool HALF = sizeof(T) == 2 && !std::is_same_v<T, __nv_bfloat16>;
-  const int tid = threadIdx.x - kConverters, piece = tid % 4 + (W == 128 ? tid / 64 * 4 : 0), in_pass = W == 128 ? tid % 64 / 4 : tid / 4;
+  constexpr bool HALF = !VALUES && !std::is_same_v<T, __nv_bfloat16>;  // the values meet bfloat16 weights
+  const int tid = threadIdx.x - (VALUES ? kValueThreads : kKeyThreads), piece = tid % 4 + (W == 128 ? tid / 64 * 4 : 0), in_pass = W == 128 ? tid % 64 / 4 : tid / 4;
   const float factor = (HALF ? 1.f : kCodeScale) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
   unsigned mask, flip, magic;
   asm volatile("mov.u32 %0, 0x00ff00ff;" : "=r"(mask));
@@ -219,14 +240,16 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
         const int lane = tid & 31, position = (walk.from + tile) * kKeys + 16 * lane;
         if (lane >= 8 || tile >= walk.tiles || position >= q.end) return -1;
         const int page = tgcb_kv::page_of(c, b, walk.s, position);
-        if (page < 0 && tid < 32) atomicAdd(c.faults, 1);
+        if (!VALUES && page < 0 && tid < 32) atomicAdd(c.faults, 1);
         return page < 0 ? -1 : (page * c.heads + head) * c.page + (position & (c.page - 1));
       };
-      auto load = [&](const int8_t* from, int rows, uint4* raw) {
+      const int8_t* from = VALUES ? c.values : c.keys;
+      auto load = [&](int rows, uint4* raw) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
           const int row = __shfl_sync(0xffffffffu, rows, W == 128 ? i : 2 * i + tid / 64);
-          raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(from + (long long)(row + in_pass % 16) * W) + piece);
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (row >= 0) load_now(raw + i, from + (long long)(row + in_pass % 16) * W + 16 * piece);
         }
       };
       auto scales_of = [&](int rows, float* ks, float* vs) {  // of key tid; whether its page is there
@@ -234,7 +257,7 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
         *ks = row < 0 ? 0.f : c.key_scales[row + tid % 16], *vs = row < 0 ? 0.f : c.value_scales[row + tid % 16];
         return row >= 0;
       };
-      auto store = [&](unsigned char* to, const uint4* raw, bool half) {
+      auto store = [&](unsigned char* to, const uint4* raw) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
           const int key = i * PER + in_pass;
@@ -243,22 +266,23 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
           unsigned* o = reinterpret_cast<unsigned*>(out);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // columns 4 j + {0, 2} and {1, 3}
-            o[2 * j] = half ? half_codes(w[j], mask, magic) : codes(w[j], mask, flip);
-            o[2 * j + 1] = half ? half_codes(w[j] >> 8, mask, magic) : codes(w[j] >> 8, mask, flip);
+            o[2 * j] = HALF ? half_codes(w[j], mask, magic) : codes(w[j], mask, flip);
+            o[2 * j + 1] = HALF ? half_codes(w[j] >> 8, mask, magic) : codes(w[j] >> 8, mask, flip);
           }
           unsigned char* row = to + (piece / 4) * (kKeys * 128) + key * 128;
           *reinterpret_cast<uint4*>(row + 16 * ((2 * (piece % 4)) ^ (key & 7))) = out[0];
           *reinterpret_cast<uint4*>(row + 16 * ((2 * (piece % 4) + 1) ^ (key & 7))) = out[1];
         }
       };
-      uint4 keys[PASSES], values[PASSES];
-      float ks, vs;
+      uint4 raw[PASSES];
+      float ks = 0.f, vs = 0.f;
+      bool held = false;
       int rows = rows_of(0);
-      bool held = scales_of(rows, &ks, &vs);
-      load(c.keys, rows, keys);
-      load(c.values, rows, values);
+      if (!VALUES) held = scales_of(rows, &ks, &vs);
+      load(rows, raw);
       rows = rows_of(1);
 
+      if (VALUES) {
       // the unit's queries, their columns in the order in which `codes` leaves the keys'
       if (units && !wait_warp(&sh->q_free, (units - 1) & 1, sh, status)) return;
       constexpr int EIGHTS = W / 8, ROUNDS = kTensorRows * EIGHTS / 128, SOME = 8;  // 8-column pieces of a row; SOME in flight
@@ -291,32 +315,28 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
       fence_async();
       arrive(&sh->q_full);
       ++units;
+      }
 
       for (int t = 0; t < walk.tiles; ++t) {
         const int g = t & 1;
         const unsigned turn = turns[g]++;
-        unsigned char* stage = memory + M::STAGES + g * 2 * M::TILE;
-        if (turn && !wait_warp(&sh->s_full[g], (turn - 1) & 1, sh, status)) return;  // the last scores are there: their keys are used up
-        store(stage, keys, HALF);
-        float* scales = reinterpret_cast<float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
-        scales[tid] = ks * factor;
-        scales[tid + (M::VALUE_SCALES - M::KEY_SCALES) / 4] = vs * kCodeScale;
-        const unsigned there = __ballot_sync(0xffffffffu, held);
-        if ((tid & 31) == 0) reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1);
-        fence_async();
-        arrive(&sh->k_full[g]);
-        arrive(&sh->scaled[g][turn & 1]);  // of the softmax; k_full may be a phase further when it gets there
-        const bool more = t + 1 < walk.tiles;
-        if (more) {
-          held = scales_of(rows, &ks, &vs);
-          load(c.keys, rows, keys);
+        unsigned char* stage = memory + M::STAGES + (2 * g + VALUES) * M::TILE;
+        // the group's last scores (outputs) are there: their keys (values) are used up
+        if (turn && !wait_warp(VALUES ? &sh->pv_done[g] : &sh->s_full[g], (turn - 1) & 1, sh, status)) return;
+        store(stage, raw);
+        if (!VALUES) {
+          float* scales = reinterpret_cast<float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
+          scales[tid] = ks * factor;
+          scales[tid + (M::VALUE_SCALES - M::KEY_SCALES) / 4] = vs * kCodeScale;
+          const unsigned there = __ballot_sync(0xffffffffu, held);
+          if ((tid & 31) == 0) reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1);
         }
-        if (turn && !wait_warp(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;
-        store(stage + M::TILE, values, false);
         fence_async();
-        arrive(&sh->v_full[g]);
-        if (more) {
-          load(c.values, rows, values);
+        arrive(VALUES ? &sh->v_full[g] : &sh->k_full[g]);
+        if (!VALUES) arrive(&sh->scaled[g][turn & 1]);  // of the softmax; k_full may be a phase further when it gets there
+        if (t + 1 < walk.tiles) {
+          if (!VALUES) held = scales_of(rows, &ks, &vs);
+          load(rows, raw);
           rows = rows_of(t + 2);
         }
       }
@@ -629,14 +649,22 @@ __global__ void __launch_bounds__(kTensorThreads, 1) attend_tiles(const Cache c,
   __syncthreads();  // a cut that is written below comes after
   if (blockIdx.x * chunk < begin.total) {
     const Walk walk(c, b, a, begin, chunk);
-    if (threadIdx.x < kConverters) {
+    if (threadIdx.x < kKeyThreads) {
+      more_registers<kSoftmaxRegisters>();
       weigh<T, W>(c, b, a, walk, &sh, memory, tmem, status);
+    } else if (threadIdx.x < kValueThreads) {
+      fewer_registers<kConverterRegisters>();
+      convert<T, W, false>(c, b, a, walk, &sh, memory, status);
     } else if (threadIdx.x < kProducts) {
-      convert<T, W>(c, b, a, walk, &sh, memory, status);
-    } else if (threadIdx.x == kProducts) {
-      multiply<T, W>(walk, &sh, memory, tmem, status);
-      commit(&sh.drained);  // whatever was queued has ended before the memory is given back
-      wait(&sh.drained, 0, &sh, status);
+      fewer_registers<kConverterRegisters>();
+      convert<T, W, true>(c, b, a, walk, &sh, memory, status);
+    } else {
+      fewer_registers<kProductRegisters>();
+      if (threadIdx.x == kProducts) {
+        multiply<T, W>(walk, &sh, memory, tmem, status);
+        commit(&sh.drained);  // whatever was queued has ended before the memory is given back
+        wait(&sh.drained, 0, &sh, status);
+      }
     }
   }
   fence_before();
