@@ -3,8 +3,11 @@
 Tolerance. A score is a sum of `width` products in float32, truncated by the tensor cores at
 worst: off by (width + 8) * 2^-23 of scale * sum |q_i k_i| (plus 2^-21 of a cap); a weight is off by
 that relatively, and once more through the sum of the weights. The weighted values of n keys are added up in
-float32, at most n / 16 + 64 of them in a row. 16-bit rows hold the weights to 16 bits or more and
-round the result once: half of the type's eps of the value.
+float32, at most n / 16 + 64 of them in a row. 16-bit rows round the result once: half of the type's eps of the
+value. Their weights: those of float16 rows are held to 16 bits or more, those of bfloat16 rows may
+be one float16 relative to the row's largest weight (times its value's scale): off by 2^-11 of themselves or, below 2^-14
+of the largest, by 2^-25 of that one, whose value row has a code of 127 and so the row's largest sum
+p_j |v_j| at least.
 """
 
 from __future__ import annotations
@@ -68,7 +71,9 @@ def check(got, q, cache, table, starts, offsets, visible=None, scale=None, cap=N
     part = 2 * delta + (longest / 16 + 64) * 2.0**-24
     tol = part * size + 1e-37
     if q.dtype != torch.float32:
-        tol = (part + 2.0**-16) * size + torch.finfo(q.dtype).eps / 2 * (want.abs() + part * size) + 2.0**-25
+        weights = 2.0**-11 if q.dtype == torch.bfloat16 else 2.0**-16
+        tol = (part + weights) * size + longest * 2.0**-25 * size.amax(-1, keepdim=True)
+        tol = tol + torch.finfo(q.dtype).eps / 2 * (want.abs() + tol) + 2.0**-25
     off = (got.cpu().double() - want).abs()
     ratio = (off / tol)[mine]
     assert not bool(got.cpu()[mine].isnan().any())
