@@ -532,10 +532,14 @@ int row_tiles(const Batch& b, int group, int width) {
   return 4;
 }
 
-// Calls whose sequences have more than 32 query rows a key head on average, in 16 bits and widths 64 and 128, take
-// the tcgen05 kernel with units of 128 rows.
-bool for_tensor(const Batch& b, int group, int width) {
-  return (b.tokens + b.batch - 1) / b.batch * group > 32 && (width == 64 || width == 128);
+// Calls in 16 bits and widths 64 and 128 take the tcgen05 kernel, with units of 128 rows, where sequences have more than
+// 32 query rows a key head on average and the call may have four tiles of 128 keys for every SM. Measured there and
+// here: 2 x 509 tokens behind 4000 positions 143 and 363 us, 32 trees of 1 to 31 nodes over 2000 to 8000 positions 306
+// and 485 us; one tree of 13 nodes over 2047 positions, too little to fill the longer pipeline, 43 and 37 us.
+bool for_tensor(const Cache& c, const Batch& b, int group) {
+  if ((c.width != 64 && c.width != 128) || (b.tokens + b.batch - 1) / b.batch * group <= 32) return false;
+  const long long units = (b.tokens * group + kTensorRows - 1) / kTensorRows * c.heads;
+  return units * ((long long)b.max_pages * c.page / 128) >= 4 * kTensorCtas;
 }
 
 size_t cuts_bytes() { return kMaxCtas * sizeof(int4); }
@@ -543,7 +547,7 @@ size_t cuts_bytes() { return kMaxCtas * sizeof(int4); }
 size_t scratch_bytes(const Cache& c, const Batch& b, int q_heads) {
   if (b.tokens == 0 || (long long)b.max_pages * c.page <= kWholeBelow) return 0;
   size_t rows = 2ull * kMaxCtas * 8 * row_tiles(b, q_heads / c.heads, c.width);
-  if (for_tensor(b, q_heads / c.heads, c.width)) rows = std::max<size_t>(rows, 2ull * kTensorCtas * kTensorRows);
+  if (for_tensor(c, b, q_heads / c.heads)) rows = std::max<size_t>(rows, 2ull * kTensorCtas * kTensorRows);
   return cuts_bytes() + rows * (c.width + 2) * sizeof(float);
 }
 
@@ -635,7 +639,7 @@ int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int 
   a.q_heads = q_heads, a.group = q_heads / c.heads, a.scale = scale, a.cap = cap;
   a.capacity = b.max_pages * c.page, a.whole = need == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype != TGCB_F32 && for_tensor(b, a.group, c.width)) return attend_tensor(c, b, a, dtype, s);
+  if (dtype != TGCB_F32 && for_tensor(c, b, a.group)) return attend_tensor(c, b, a, dtype, s);
   switch (dtype) {
     case TGCB_F32: return run<float>(c, b, a, s);
     case TGCB_BF16: return run<__nv_bfloat16>(c, b, a, s);

@@ -10,16 +10,13 @@
 //     others a unit's queries.
 //   products (1 thread): S = Q K^T into the group's 128 columns of tensor memory; O += P V with P read from tensor
 //     memory and V as it lies (columns contiguous).
-//   softmax (2 x 4 warps, a thread per row). A key's value scale enters as its logarithm: with x_j = s_j + log2 vs_j in
-//     powers of two and r the row's largest x_j, the weights 2^(x_j - r) are what multiplies the value codes, and
-//     2^(x_j - r) / vs_j is what is summed. So the largest weight is near 1 whatever the scales, and a float16
-//     holds the weights to 2^-11 of their value (what is below 2^-14 of the largest, to 2^-25 of that): an eighth
-//     of a bfloat16 row's own rounding. Float16 rows take a second float16 for the rest. The weights are written over
-//     the scores they came from: 32 columns of scores hold 16 of weights and 16 of rests.
-//     The accumulator is rescaled only when r grows by more than 2^8, since the sums and the products share
-//     whatever reference they were taken against.
+//   softmax (2 x 4 warps, a thread per row): the row's maximum, then weights e^(s - m) times the value's
+//     scale as two bfloat16 parts (16 bits, as in the kernel for few rows), written over the scores
+//     they came from: 32 scores' columns hold 16 columns of leading and 16 of remaining parts.
+//     The accumulator is rescaled only when a maximum grows by more than 2^8, since the weights' sum
+//     and the products share whatever reference they were taken against.
 //
-// Bound by the softmax warps' issue slots: about 5 instructions a score against 4 x 128 tensor operations.
+// Bound by the softmax warps' issue slots: about 11 instructions a score against 3 x 128 x 2 tensor operations.
 // All waits are bounded (4 s); a CTA that gives up records status 2 and unwinds.
 #include <atomic>
 #include <type_traits>
@@ -39,8 +36,10 @@ constexpr int kProducts = kValueThreads + 128;           // of the four warps of
 constexpr int kTensorThreads = kProducts + 128;
 // Registers a thread: the launch gives 96 to each of the five groups of 128, 480 in all, which the
 // roles share out between them.
-constexpr int kSoftmaxRegisters = 136, kConverterRegisters = 80, kProductRegisters = 48;
-static_assert(2 * kSoftmaxRegisters + 2 * kConverterRegisters + kProductRegisters <= 5 * 96, "the launch has no more registers");
+constexpr int kSoftmaxRegisters = 136, kConverterRegisters = 80, kProductRegisters = 48, kLaunchRegisters = 96;
+static_assert(2 * kSoftmaxRegisters + 2 * kConverterRegisters + kProductRegisters <= 5 * kLaunchRegisters, "the launch has no more registers");
+static_assert(kSoftmaxRegisters >= kLaunchRegisters && kConverterRegisters <= kLaunchRegisters && kProductRegisters <= kLaunchRegisters,
+              "more_registers only goes up, fewer_registers only down");
 constexpr int kLeastTiles = 2;                           // one for each group
 constexpr int kStatusTimeout = 2;
 constexpr float kGrowth = 8.f;                           // of a maximum, in powers of two, before anything is rescaled
@@ -50,14 +49,15 @@ struct Memory {
   static constexpr int TILE = kKeys * W * 2;
   static constexpr int QUERIES = 0;
   static constexpr int STAGES = kTensorRows * W * 2;     // group g: keys, then values
-  static constexpr int SCALES = STAGES + 4 * TILE;       // float [group][turn][kind][128]: key scales, logarithms and reciprocals of value scales
-  static constexpr int EXCHANGE = SCALES + 4 * 3 * kKeys * 4;  // float [group][128][33]
-  static constexpr int ROWS = EXCHANGE + 2 * 128 * 33 * 4;     // float2 [parity][group][128]: reference and sum
+  static constexpr int KEY_SCALES = STAGES + 4 * TILE;   // float [group][turn][128]
+  static constexpr int VALUE_SCALES = KEY_SCALES + 4 * kKeys * 4;
+  static constexpr int EXCHANGE = VALUE_SCALES + 4 * kKeys * 4;  // float [128][33]
+  static constexpr int ROWS = EXCHANGE + 128 * 33 * 4;   // float2 [parity][group][128]: maximum and sum
   static constexpr int BYTES = ROWS + 4 * 128 * 8 + 1024;  // and room to begin on a 1024-byte boundary
 };
 
 struct Shared {
-  unsigned long long q_full, q_free, k_full[2], scaled[2][2], v_full[2], s_full[2], p_ready[2], pv_done[2], rows_full, x_full[2], x_free[2], drained;
+  unsigned long long q_full, q_free, k_full[2], scaled[2][2], v_full[2], s_full[2], p_ready[2], pv_done[2], rows_full, x_full, x_free, drained;
   unsigned tmem, valid[2][2];  // valid: a bit for each 16 keys of a tile whose page is there
   int abort;
 };
@@ -73,12 +73,12 @@ __device__ __forceinline__ bool wait(unsigned long long* bar, unsigned parity, S
   unsigned long long start = 0;
   for (unsigned it = 0;; ++it) {
     unsigned ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                  : "=r"(ok)
-                 : "r"(at(bar)), "r"(parity), "r"(100000u)  // nanoseconds that the hardware may wait
+                 : "r"(at(bar)), "r"(parity)
                  : "memory");
     if (ok) return true;
-    if ((it & 15u) == 15u) {
+    if ((it & 255u) == 255u) {
       if (*reinterpret_cast<volatile int*>(&sh->abort)) return false;
       unsigned long long now;
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
@@ -138,28 +138,27 @@ __device__ __forceinline__ void store32(unsigned tmem, const unsigned* r) {
       TGCB_S8(r, 0), TGCB_S8(r, 8), TGCB_S8(r, 16), TGCB_S8(r, 24)
       : "memory");
 }
-__device__ __forceinline__ void store16(unsigned tmem, const unsigned* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(tmem),
-               TGCB_S8(r, 0), TGCB_S8(r, 8)
-               : "memory");
-}
 __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A matrix in shared memory with the 128-byte swizzle: rows of 128 bytes, eight to an atom. `lbo`: from one 128-byte
-// column block to the next where the columns are not the summed dimension.
-__device__ __forceinline__ unsigned long long matrix(unsigned start, unsigned lbo) {
-  return (unsigned long long)((start >> 4) & 0x3fffu) | (unsigned long long)((lbo >> 4) & 0x3fffu) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
-}
+// A matrix in shared memory with the 128-byte swizzle: rows of 128 bytes, eight to an atom. The lower half of its
+// description, to which steps in 16-byte units are added; `lbo`: from one 128-byte column block to the next where
+// the columns are not the summed dimension. The upper half is the same for all.
+__device__ __forceinline__ unsigned matrix(unsigned start, unsigned lbo) { return ((start >> 4) & 0x3fffu) | (lbo >> 4) << 16; }
+constexpr unsigned kMatrixHigh = 64u | 1u << 14 | 2u << 29;
 
-__device__ __forceinline__ void product_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned how, bool add) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p; }" ::"r"(d), "l"(a),
-               "l"(b), "r"(how), "r"((unsigned)add), "r"(0u)
-               : "memory");
+__device__ __forceinline__ void product_ss(unsigned d, unsigned a, unsigned b, unsigned how, bool add) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 a, b; setp.ne.b32 p, %4, 0; mov.b64 a, {%1, %6}; mov.b64 b, {%2, %6};"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, {%5, %5, %5, %5}, p; }" ::"r"(d),
+      "r"(a), "r"(b), "r"(how), "r"((unsigned)add), "r"(0u), "r"(kMatrixHigh)
+      : "memory");
 }
-__device__ __forceinline__ void product_ts(unsigned d, unsigned a, unsigned long long b, unsigned how, bool add) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p; }" ::"r"(d), "r"(a),
-               "l"(b), "r"(how), "r"((unsigned)add), "r"(0u)
-               : "memory");
+__device__ __forceinline__ void product_ts(unsigned d, unsigned a, unsigned b, unsigned how, bool add) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 b; setp.ne.b32 p, %4, 0; mov.b64 b, {%2, %6};"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, {%5, %5, %5, %5}, p; }" ::"r"(d),
+      "r"(a), "r"(b), "r"(how), "r"((unsigned)add), "r"(0u), "r"(kMatrixHigh)
+      : "memory");
 }
 
 // Two codes as float16, bytes 0 and 2 of a word: with the sign bit flipped they are x + 128, the low bits of 1024 + x
@@ -227,9 +226,9 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
   // 16-code pieces of a row; rows a pass copies. Eight neighbouring threads have four pieces of two rows, whose halves lie on
   // different banks.
   constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;
-  constexpr bool HALF = VALUES || !std::is_same_v<T, __nv_bfloat16>;  // the values meet float16 weights
+  constexpr bool HALF = !VALUES && !std::is_same_v<T, __nv_bfloat16>;  // the values meet bfloat16 weights
   const int tid = threadIdx.x - (VALUES ? kValueThreads : kKeyThreads), piece = tid % 4 + (W == 128 ? tid / 64 * 4 : 0), in_pass = W == 128 ? tid % 64 / 4 : tid / 4;
-  const float factor = (std::is_same_v<T, __nv_bfloat16> ? kCodeScale : 1.f) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
+  const float factor = (HALF ? 1.f : kCodeScale) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
   unsigned mask, flip, magic;
   asm volatile("mov.u32 %0, 0x00ff00ff;" : "=r"(mask));
   asm volatile("mov.u32 %0, 0x00800080;" : "=r"(flip));
@@ -241,14 +240,18 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
     if (walk.tiles > 0) {
       const Sequence& q = walk.q;
       const int head = walk.head;
-      // The rows of a tile's first keys of each 16 (one page holds them), a lane each: -1 where they are not there or not
-      // read. With widths from 64 a cache in memory has fewer than 2^31 rows.
-      auto rows_of = [&](int tile) {
+      // A tile's pages, a lane for each 16 keys (one page holds them), and, once they are there, the rows of the first of
+      // those keys: -1 where they are not there or not read. With widths from 64 a cache in memory has fewer than 2^31 rows.
+      constexpr int kUnread = -2;
+      auto pages_of = [&](int tile) {
         const int lane = tid & 31, position = (walk.from + tile) * kKeys + 16 * lane;
-        if (lane >= 8 || tile >= walk.tiles || position >= q.end) return -1;
-        const int page = tgcb_kv::page_of(c, b, walk.s, position);
-        if (!VALUES && page < 0 && tid < 32) atomicAdd(c.faults, 1);
-        return page < 0 ? -1 : (page * c.heads + head) * c.page + (position & (c.page - 1));
+        if (lane >= kKeys / 16 || tile >= walk.tiles || position >= q.end) return kUnread;
+        return __ldg(b.table + walk.s * b.table_stride + (position >> c.page_bits));
+      };
+      auto rows_of = [&](int tile, int page) {
+        const bool there = page >= 0 && page < c.pages;
+        if (!VALUES && !there && page != kUnread && tid < 32) atomicAdd(c.faults, 1);
+        return there ? (page * c.heads + head) * c.page + (((walk.from + tile) * kKeys + 16 * (tid & 31)) & (c.page - 1)) : -1;
       };
       const int8_t* from = VALUES ? c.values : c.keys;
       auto load = [&](int rows, uint4* raw) {
@@ -284,41 +287,47 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
       uint4 raw[PASSES];
       float ks = 0.f, vs = 0.f;
       bool held = false;
-      int rows = rows_of(0);
-      if (!VALUES) held = scales_of(rows, &ks, &vs);
-      load(rows, raw);
-      rows = rows_of(1);
+      {
+        const int rows = rows_of(0, pages_of(0));
+        if (!VALUES) held = scales_of(rows, &ks, &vs);
+        load(rows, raw);
+      }
+      int pages = pages_of(1);
 
-      // the unit's queries, their columns in the order in which `codes` leaves the keys', half of them here and half by the
-      // other converters
+      if (VALUES) {
+      // the unit's queries, their columns in the order in which `codes` leaves the keys'
       if (units && !wait_warp(&sh->q_free, (units - 1) & 1, sh, status)) return;
-      constexpr int EIGHTS = W / 8, ROUNDS = kTensorRows / 2 * EIGHTS / 128;  // 8-column pieces of a row
-      uint4 v[ROUNDS];
+      constexpr int EIGHTS = W / 8, ROUNDS = kTensorRows * EIGHTS / 128, SOME = 8;  // 8-column pieces of a row; SOME in flight
+#pragma unroll 1
+      for (int i0 = 0; i0 < ROUNDS; i0 += SOME) {
+        uint4 v[SOME];
 #pragma unroll
-      for (int i = 0; i < ROUNDS; ++i) {
-        const int r = VALUES * (kTensorRows / 2) + (i * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (r < walk.rows) {
-          const int row = walk.tile * kTensorRows + r, token = row / a.group, in_group = row - token * a.group;
-          const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h + 8 * eight;
-          if (wide_q) {
-            v[i] = *reinterpret_cast<const uint4*>(p);
-          } else {
-            const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
-            v[i] = make_uint4(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16, e[4] | (unsigned)e[5] << 16, e[6] | (unsigned)e[7] << 16);
+        for (int i = 0; i < SOME; ++i) {
+          const int r = ((i0 + i) * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r < walk.rows) {
+            const int row = walk.tile * kTensorRows + r, token = row / a.group, in_group = row - token * a.group;
+            const T* p = reinterpret_cast<const T*>(a.q) + (q.first + token) * a.q_t + (long long)(head * a.group + in_group) * a.q_h + 8 * eight;
+            if (wide_q) {
+              v[i] = *reinterpret_cast<const uint4*>(p);
+            } else {
+              const unsigned short* e = reinterpret_cast<const unsigned short*>(p);
+              v[i] = make_uint4(e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16, e[4] | (unsigned)e[5] << 16, e[6] | (unsigned)e[7] << 16);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < ROUNDS; ++i) {
-        const int r = VALUES * (kTensorRows / 2) + (i * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
-        const uint4 x = v[i];  // each four columns as (0, 2), (1, 3)
-        *reinterpret_cast<uint4*>(memory + M::QUERIES + (eight / 8) * (kTensorRows * 128) + r * 128 + 16 * ((eight % 8) ^ (r & 7))) =
-            make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+        for (int i = 0; i < SOME; ++i) {
+          const int r = ((i0 + i) * 128 + tid) / EIGHTS, eight = tid % EIGHTS;
+          const uint4 x = v[i];  // each four columns as (0, 2), (1, 3)
+          *reinterpret_cast<uint4*>(memory + M::QUERIES + (eight / 8) * (kTensorRows * 128) + r * 128 + 16 * ((eight % 8) ^ (r & 7))) =
+              make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+        }
       }
       fence_async();
       arrive(&sh->q_full);
       ++units;
+      }
 
       for (int t = 0; t < walk.tiles; ++t) {
         const int g = t & 1;
@@ -328,11 +337,9 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
         if (turn && !wait_warp(VALUES ? &sh->pv_done[g] : &sh->s_full[g], (turn - 1) & 1, sh, status)) return;
         store(stage, raw);
         if (!VALUES) {
-          float* scales = reinterpret_cast<float*>(memory + M::SCALES) + (g * 2 + (turn & 1)) * 3 * kKeys + tid;
-          const float least = vs < 0x1p-100f ? 0x1p-100f : vs;  // a scale too small to count: its reciprocal stays finite
-          scales[0] = ks * factor;
-          scales[kKeys] = log2f(least);
-          scales[2 * kKeys] = 1.f / least;
+          float* scales = reinterpret_cast<float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
+          scales[tid] = ks * factor;
+          scales[tid + (M::VALUE_SCALES - M::KEY_SCALES) / 4] = vs * kCodeScale;
           const unsigned there = __ballot_sync(0xffffffffu, held);
           if ((tid & 31) == 0) reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1);
         }
@@ -340,9 +347,10 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
         arrive(VALUES ? &sh->v_full[g] : &sh->k_full[g]);
         if (!VALUES) arrive(&sh->scaled[g][turn & 1]);  // of the softmax; k_full may be a phase further when it gets there
         if (t + 1 < walk.tiles) {
+          const int rows = rows_of(t + 1, pages);
           if (!VALUES) held = scales_of(rows, &ks, &vs);
           load(rows, raw);
-          rows = rows_of(t + 2);
+          pages = pages_of(t + 2);
         }
       }
     }
@@ -350,18 +358,14 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
   }
 }
 
-// Parts of a weight.
-template <typename T>
-constexpr int kParts = std::is_same_v<T, __half> ? 2 : 1;
-
 template <typename T, int W>
 __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* memory, unsigned tmem, int* status) {
   using M = Memory<W>;
   constexpr bool HALF = !std::is_same_v<T, __nv_bfloat16>;
-  // float32 results; both factors float16 or both bfloat16; the values (float16) with their columns contiguous
+  // float32 results; both factors float16 or both bfloat16; the values with their columns contiguous
   constexpr unsigned kScores = 1u << 4 | (HALF ? 0u : 1u << 7 | 1u << 10) | (unsigned)(kKeys >> 3) << 17 | 8u << 24;
-  constexpr unsigned kOutputs = 1u << 4 | 1u << 16 | (unsigned)(W >> 3) << 17 | 8u << 24;
-  const unsigned queries = at(memory + M::QUERIES);
+  constexpr unsigned kOutputs = 1u << 4 | 1u << 7 | 1u << 10 | 1u << 16 | (unsigned)(W >> 3) << 17 | 8u << 24;
+  const unsigned queries = matrix(at(memory + M::QUERIES), 16);
   unsigned score_turns[2] = {0, 0}, output_turns[2] = {0, 0}, units = 0;
   while (walk.next()) {
     if (walk.tiles > 0) {
@@ -373,11 +377,11 @@ __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* m
           if (!wait(&sh->k_full[g], turn & 1, sh, status)) return;
           if (turn && !wait(&sh->pv_done[g], (turn - 1) & 1, sh, status)) return;  // the weights there are used up
           fence_after();
-          const unsigned keys = at(memory + M::STAGES + g * 2 * M::TILE);
+          const unsigned keys = matrix(at(memory + M::STAGES + g * 2 * M::TILE), 16);
 #pragma unroll
           for (int k = 0; k < W / 16; ++k) {
-            const unsigned to = (k / 4) * (kKeys * 128) + (k % 4) * 32;
-            product_ss(tmem + 2 * W + g * kKeys, matrix(queries + to, 16), matrix(keys + to, 16), kScores, k > 0);
+            const unsigned to = ((k / 4) * (kKeys * 128) + (k % 4) * 32) / 16;
+            product_ss(tmem + 2 * W + g * kKeys, queries + to, keys + to, kScores, k > 0);
           }
           commit(&sh->s_full[g]);
           if (t + 1 == walk.tiles) commit(&sh->q_free);
@@ -388,12 +392,12 @@ __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* m
           if (!wait(&sh->p_ready[g], turn & 1, sh, status)) return;
           if (!wait(&sh->v_full[g], turn & 1, sh, status)) return;
           fence_after();
-          const unsigned values = at(memory + M::STAGES + g * 2 * M::TILE + M::TILE), weights = tmem + 2 * W + g * kKeys;
+          const unsigned values = matrix(at(memory + M::STAGES + g * 2 * M::TILE + M::TILE), kKeys * 128), weights = tmem + 2 * W + g * kKeys;
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
 #pragma unroll
-            for (int part = 0; part < kParts<T>; ++part)
-              product_ts(tmem + g * W, weights + 32 * (k / 2) + 16 * part + 8 * (k % 2), matrix(values + k * 16 * 128, kKeys * 128), kOutputs,
+            for (int part = 0; part < 2; ++part)
+              product_ts(tmem + g * W, weights + 32 * (k / 2) + 16 * part + 8 * (k % 2), values + k * 16 * 128 / 16, kOutputs,
                          t > 2 || k > 0 || part > 0);
           commit(&sh->pv_done[g]);
         }
@@ -417,24 +421,9 @@ __device__ __forceinline__ void store8(T* p, const float* v, bool whole) {
   }
 }
 
-// Two floats at a time.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
-  return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-
-// The largest x_j of a row's 128 scores, of those alone that `seen_of` shows where MASKED. With CAP the x_j are left in
-// the scores' place, for `weights` to take from there.
-template <typename T, bool CAP, bool MASKED, class Seen>
-__device__ __forceinline__ float top_of(unsigned scores, const float* scales, float cap2, Seen seen_of) {
+// The largest of a row's 128 scaled scores, of those alone that `seen_of` shows where MASKED.
+template <bool MASKED, class Seen>
+__device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen seen_of) {
   float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
   for (int ch = 0; ch < 4; ++ch) {
@@ -443,76 +432,50 @@ __device__ __forceinline__ float top_of(unsigned scores, const float* scales, fl
     const unsigned see = MASKED ? seen_of(ch) : 0;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(scales + 32 * ch + j), l = *reinterpret_cast<const float4*>(scales + kKeys + 32 * ch + j);
-      float2 x = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), y = make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-      if (CAP) {
-        x = make_float2(fmaf(cap2, tanh_of<T>(x.x * k.x), l.x), fmaf(cap2, tanh_of<T>(x.y * k.y), l.y));
-        y = make_float2(fmaf(cap2, tanh_of<T>(y.x * k.z), l.z), fmaf(cap2, tanh_of<T>(y.y * k.w), l.w));
-        r[j] = __float_as_uint(x.x), r[j + 1] = __float_as_uint(x.y), r[j + 2] = __float_as_uint(y.x), r[j + 3] = __float_as_uint(y.y);
-      } else {
-        x = fma2(x, make_float2(k.x, k.y), make_float2(l.x, l.y));
-        y = fma2(y, make_float2(k.z, k.w), make_float2(l.z, l.w));
-      }
+      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j);
+      float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
       if (MASKED) {
-        x.x = (see >> j) & 1 ? x.x : -INFINITY, x.y = (see >> (j + 1)) & 1 ? x.y : -INFINITY;
-        y.x = (see >> (j + 2)) & 1 ? y.x : -INFINITY, y.y = (see >> (j + 3)) & 1 ? y.y : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (see >> (j + i)) & 1 ? x[i] : -INFINITY;
       }
-      top[0] = fmaxf(top[0], fmaxf(x.x, x.y)), top[1] = fmaxf(top[1], fmaxf(y.x, y.y));
+      top[0] = fmaxf(top[0], fmaxf(x[0], x[1])), top[1] = fmaxf(top[1], fmaxf(x[2], x[3]));
     }
-    if (CAP) store32(scores + 32 * ch, r);
   }
-  if (CAP) stored();
   return fmaxf(top[0], top[1]);
 }
 
-// Writes a row's 128 weights over its scores, 32 at a time as 16 columns of float16 pairs and, with two parts, 16 of what
-// they leave over, and returns the sum of the weights over their values' scales.
+// Writes a row's 128 weights times the values' scales over its scores, 32 at a time as 16 columns of leading and 16 of
+// remaining parts, and returns the weights' sum.
 template <typename T, bool CAP, bool MASKED, class Seen>
-__device__ __forceinline__ float weights(unsigned scores, const float* scales, float base, Seen seen_of) {
-  float2 sum = make_float2(0.f, 0.f), more = sum;
-  const float2 less = make_float2(-base, -base);
+__device__ __forceinline__ float weights(unsigned scores, const float* ks, const float* vs, float base, float cap2, Seen seen_of) {
+  float some[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int ch = 0; ch < 4; ++ch) {
-    unsigned r[32], w[16 * kParts<T>];
+    unsigned r[32], parts[32];
     load32(scores + 32 * ch, r);
     const unsigned see = MASKED ? seen_of(ch) : 0;
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(scales + 32 * ch + j), l = *reinterpret_cast<const float4*>(scales + kKeys + 32 * ch + j);
-      const float4 v = *reinterpret_cast<const float4*>(scales + 2 * kKeys + 32 * ch + j);
-      float2 x = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), y = make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-      if (!CAP) {
-        x = fma2(x, make_float2(k.x, k.y), make_float2(l.x, l.y));
-        y = fma2(y, make_float2(k.z, k.w), make_float2(l.z, l.w));
+      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j), v = *reinterpret_cast<const float4*>(vs + 32 * ch + j);
+      const float by[4] = {k.x, k.y, k.z, k.w}, scale[4] = {v.x, v.y, v.z, v.w};
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float s = __uint_as_float(r[j + i]);
+        float p = exp2_fast(CAP ? fmaf(cap2, tanh_of<T>(s * by[i]), -base) : fmaf(s, by[i], -base));
+        w[i] = p * scale[i];
+        if (MASKED && !((see >> (j + i)) & 1)) p = 0.f, w[i] = 0.f;  // whatever lies there
+        some[i] += p;
       }
-      x = add2(x, less), y = add2(y, less);
-      x = make_float2(exp2_fast(x.x), exp2_fast(x.y)), y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-      float2 vx = make_float2(v.x, v.y), vy = make_float2(v.z, v.w);
-      if (MASKED) {  // whatever lies there
-        if (!((see >> j) & 1)) x.x = 0.f, vx.x = 0.f;
-        if (!((see >> (j + 1)) & 1)) x.y = 0.f, vx.y = 0.f;
-        if (!((see >> (j + 2)) & 1)) y.x = 0.f, vy.x = 0.f;
-        if (!((see >> (j + 3)) & 1)) y.y = 0.f, vy.y = 0.f;
-      }
-      sum = fma2(x, vx, sum), more = fma2(y, vy, more);
-      auto pair = [](float2 v) {
-        unsigned h;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(v.y), "f"(v.x));
-        return h;
-      };
-      w[j / 2] = pair(x), w[j / 2 + 1] = pair(y);
-      if constexpr (kParts<T> == 2) {
-        const float2 hx = __half22float2(*reinterpret_cast<__half2*>(w + j / 2)), hy = __half22float2(*reinterpret_cast<__half2*>(w + j / 2 + 1));
-        w[16 + j / 2] = pair(make_float2(x.x - hx.x, x.y - hx.y)), w[16 + j / 2 + 1] = pair(make_float2(y.x - hy.x, y.y - hy.y));
-      }
+      unsigned two[2];
+      split<2>(w[0], w[1], two);
+      parts[j / 2] = two[0], parts[16 + j / 2] = two[1];
+      split<2>(w[2], w[3], two);
+      parts[j / 2 + 1] = two[0], parts[16 + j / 2 + 1] = two[1];
     }
-    if constexpr (kParts<T> == 2) {
-      store32(scores + 32 * ch, w);
-    } else {
-      store16(scores + 32 * ch, w);
-    }
+    store32(scores + 32 * ch, parts);
   }
-  return (sum.x + sum.y) + (more.x + more.y);
+  return (some[0] + some[1]) + (some[2] + some[3]);
 }
 
 template <typename T, int W>
@@ -544,7 +507,8 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
       const int position = (walk.from + t) * kKeys;
       if (!wait_warp(&sh->scaled[g][turn & 1], turn >> 1 & 1, sh, status) || !wait_warp(&sh->s_full[g], turn & 1, sh, status)) return;
       fence_after();
-      const float* scales = reinterpret_cast<const float*>(memory + M::SCALES) + (g * 2 + (turn & 1)) * 3 * kKeys;
+      const float* ks = reinterpret_cast<const float*>(memory + M::KEY_SCALES) + (g * 2 + (turn & 1)) * kKeys;
+      const float* vs = ks + (M::VALUE_SCALES - M::KEY_SCALES) / 4;
       const unsigned word = sh->valid[g][turn & 1];
       const bool inside = position + kKeys <= walk.all && word == 0x03030303u;
       // the keys of 32 from column 32 ch that this row sees
@@ -559,12 +523,15 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         const unsigned halves = word >> (8 * ch);
         return s & ((halves & 1 ? 0xffffu : 0u) | (halves & 2 ? 0xffff0000u : 0u));
       };
-      float top;
-      if (a.cap > 0)
-        top = inside ? top_of<T, true, false>(scores, scales, cap2, seen_of) : top_of<T, true, true>(scores, scales, cap2, seen_of);
-      else
-        top = inside ? top_of<T, false, false>(scores, scales, cap2, seen_of) : top_of<T, false, true>(scores, scales, cap2, seen_of);
-      seen = seen || inside || seen_of(0) || seen_of(1) || seen_of(2) || seen_of(3);
+      float top = -INFINITY;
+      if (inside) {
+        top = top_of<false>(scores, ks, seen_of);
+        seen = true;
+      } else {
+        top = top_of<true>(scores, ks, seen_of);
+        seen = seen || seen_of(0) || seen_of(1) || seen_of(2) || seen_of(3);
+      }
+      if (a.cap > 0) top = top == -INFINITY ? top : cap2 * tanh_of<T>(top);
       const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grown)) {
         const float keep = grown ? exp2_fast(m - top) : 1.f;
@@ -585,9 +552,9 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
       }
       const float base = m == -INFINITY ? 0.f : m;
       if (a.cap > 0)
-        sum += inside ? weights<T, true, false>(scores, scales, base, seen_of) : weights<T, true, true>(scores, scales, base, seen_of);
+        sum += inside ? weights<T, true, false>(scores, ks, vs, base, cap2, seen_of) : weights<T, true, true>(scores, ks, vs, base, cap2, seen_of);
       else
-        sum += inside ? weights<T, false, false>(scores, scales, base, seen_of) : weights<T, false, true>(scores, scales, base, seen_of);
+        sum += inside ? weights<T, false, false>(scores, ks, vs, base, cap2, seen_of) : weights<T, false, true>(scores, ks, vs, base, cap2, seen_of);
       stored();
       fence_before();
       arrive(&sh->p_ready[g]);
@@ -609,38 +576,29 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
     float all_sum = 0.f;
     add_sum(&all_sum, own.y, factor);
     add_sum(&all_sum, other.y, exp2_fast(other.x - base));
-    // With two groups each finishes half of the columns, and gives the other its sums of the other half, 32 at a time.
     const bool two = walk.tiles > 1;
     T* out = out_row<T>(a, q, walk.head, mine);
-    const float by = all_sum > 0.f ? 1.f / all_sum : answer(0.f, all_sum);  // nothing seen: times zero
-    constexpr int HALF_W = W / 2;
 #pragma unroll 1
-    for (int ch = 0; ch < (two ? HALF_W / 32 : g == 0 ? W / 32 : 0); ++ch) {
-      const int column = (two ? g * HALF_W : 0) + 32 * ch;
-      float v[32];
-      if (two) {
-        load32(sums + (g ^ 1) * HALF_W + 32 * ch, reinterpret_cast<unsigned*>(v));
-        if (chunks && !wait_warp(&sh->x_free[g], (chunks - 1) & 1, sh, status)) return;
-        float* give = exchange + g * 128 * 33;
+    for (int ch = 0; ch < W / 32; ++ch) {
+      unsigned r[32];
+      if (any) load32(sums + 32 * ch, r);
+      if (g == 1) {
+        if (!two) break;
+        if (chunks && !wait_warp(&sh->x_free, (chunks - 1) & 1, sh, status)) return;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) give[j] = v[j] * factor;
-        arrive(&sh->x_full[g]);
-      }
-      if (any) {
-        load32(sums + column, reinterpret_cast<unsigned*>(v));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = any ? v[j] * factor : 0.f;
-      if (two) {
-        if (!wait_warp(&sh->x_full[g ^ 1], chunks & 1, sh, status)) return;
-        const float* take = exchange + (g ^ 1) * 128 * 33;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += take[j];
-        arrive(&sh->x_free[g ^ 1]);
+        for (int j = 0; j < 32; ++j) exchange[j] = __uint_as_float(r[j]) * factor;
+        arrive(&sh->x_full);
         ++chunks;
+        continue;
+      }
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = any ? __uint_as_float(r[j]) * factor : 0.f;
+      if (two) {
+        if (!wait_warp(&sh->x_full, chunks++ & 1, sh, status)) return;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += exchange[j];
+        arrive(&sh->x_free);
       }
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {  // the columns' order
@@ -648,15 +606,16 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         v[j + 1] = v[j + 2], v[j + 2] = x;
       }
       if (complete) {
+        const float by = all_sum > 0.f ? 1.f / all_sum : answer(0.f, all_sum);  // nothing seen: times zero
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[j + i] *= by;
-          if (row < walk.rows) store8<T>(out + column + j, v + j, wide);
+          if (row < walk.rows) store8<T>(out + 32 * ch + j, v + j, wide);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) part[(column + j) * kTensorRows + row] = v[j];
+        for (int j = 0; j < 32; ++j) part[(32 * ch + j) * kTensorRows + row] = v[j];
       }
       __syncwarp();
     }
@@ -682,9 +641,8 @@ __global__ void __launch_bounds__(kTensorThreads, 1) attend_tiles(const Cache c,
     auto init = [](unsigned long long* bar, unsigned count) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at(bar)), "r"(count));
     };
-    init(&sh.q_full, 256), init(&sh.q_free, 1), init(&sh.rows_full, 256), init(&sh.drained, 1);
+    init(&sh.q_full, 128), init(&sh.q_free, 1), init(&sh.rows_full, 256), init(&sh.x_full, 128), init(&sh.x_free, 128), init(&sh.drained, 1);
     for (int g = 0; g < 2; ++g) {
-      init(&sh.x_full[g], 128), init(&sh.x_free[g], 128);
       init(&sh.k_full[g], 128), init(&sh.scaled[g][0], 128), init(&sh.scaled[g][1], 128), init(&sh.v_full[g], 128), init(&sh.s_full[g], 1), init(&sh.p_ready[g], 128), init(&sh.pv_done[g], 1);
       sh.valid[g][0] = sh.valid[g][1] = 0;
     }

@@ -3,11 +3,8 @@
 Tolerance. A score is a sum of `width` products in float32, truncated by the tensor cores at
 worst: off by (width + 8) * 2^-23 of scale * sum |q_i k_i| (plus 2^-21 of a cap); a weight is off by
 that relatively, and once more through the sum of the weights. The weighted values of n keys are added up in
-float32, at most n / 16 + 64 of them in a row. 16-bit rows round the result once: half of the type's eps of the
-value. Their weights: those of float16 rows are held to 16 bits or more, those of bfloat16 rows may
-be one float16 relative to the row's largest weight (times its value's scale): off by 2^-11 of themselves or, below 2^-14
-of the largest, by 2^-25 of that one, whose value row has a code of 127 and so the row's largest sum
-p_j |v_j| at least.
+float32, at most n / 16 + 64 of them in a row. 16-bit rows hold the weights to 16 bits or more and
+round the result once: half of the type's eps of the value.
 """
 
 from __future__ import annotations
@@ -28,8 +25,12 @@ def vector(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
-def make(starts, counts, q_heads, kv_heads, width, page, dtype, seed=0, spare=2):
-    """(queries, cache, table, starts, offsets): sequences with `starts` positions before and `counts` rows in the call."""
+WIDE = 80_000  # positions that a table may hold beyond those in use: how a call is cut goes by what it may hold
+
+
+def make(starts, counts, q_heads, kv_heads, width, page, dtype, seed=0, spare=2, room=0):
+    """(queries, cache, table, starts, offsets): sequences with `starts` positions before and `counts` rows in the call, in a
+    table with room for `room` positions."""
     g = torch.Generator().manual_seed(seed)
     batch = len(starts)
     each = max(1, max(-(-(s + n) // page) for s, n in zip(starts, counts, strict=True)))
@@ -39,6 +40,8 @@ def make(starts, counts, q_heads, kv_heads, width, page, dtype, seed=0, spare=2)
         parts.append((torch.randn(pages, kv_heads, page, width, generator=g) * 40).round().clamp(-128, 127).to(torch.int8).cuda())
         parts.append(((0.5 + torch.rand(pages, kv_heads, page, generator=g)) / 40).cuda())
     table = torch.randperm(pages, generator=g)[:batch * each].reshape(batch, each).to(torch.int32).cuda()
+    if room > each * page:
+        table = torch.nn.functional.pad(table, (0, room // page - each), value=-1)
     tokens = sum(counts)
     q = (torch.randn(tokens, q_heads, width, generator=g) * 2).to(dtype).cuda()
     offsets = [0]
@@ -71,9 +74,7 @@ def check(got, q, cache, table, starts, offsets, visible=None, scale=None, cap=N
     part = 2 * delta + (longest / 16 + 64) * 2.0**-24
     tol = part * size + 1e-37
     if q.dtype != torch.float32:
-        weights = 2.0**-11 if q.dtype == torch.bfloat16 else 2.0**-16
-        tol = (part + weights) * size + longest * 2.0**-25 * size.amax(-1, keepdim=True)
-        tol = tol + torch.finfo(q.dtype).eps / 2 * (want.abs() + tol) + 2.0**-25
+        tol = (part + 2.0**-16) * size + torch.finfo(q.dtype).eps / 2 * (want.abs() + part * size) + 2.0**-25
     off = (got.cpu().double() - want).abs()
     ratio = (off / tol)[mine]
     assert not bool(got.cpu()[mine].isnan().any())
@@ -95,31 +96,37 @@ SHAPES = [
     ([0], [150], 5, 1, 64, 128),
     ([31, 0], [17, 40], 17, 1, 32, 16),
     ([500, 3], [5, 64], 8, 2, 256, 64),
+    ([3000, 0, 7, 250], [90, 200, 0, 3], 8, 2, 128, 64),
+    ([0, 1500], [1, 300], 4, 1, 64, 32),
+    ([130], [129], 3, 3, 128, 16),
 ]
 
 
+@pytest.mark.parametrize("room", [0, WIDE])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("starts,counts,q_heads,kv_heads,width,page", SHAPES)
-def test_causal(cuda, starts, counts, q_heads, kv_heads, width, page, dtype):
-    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype)
+def test_causal(cuda, starts, counts, q_heads, kv_heads, width, page, dtype, room):
+    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype, room=room)
     check(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
     cache.check()
 
 
+@pytest.mark.parametrize("room", [0, WIDE])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("starts,counts,q_heads,kv_heads,width,page", SHAPES)
-def test_capped(cuda, starts, counts, q_heads, kv_heads, width, page, dtype):
-    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype, seed=1)
+def test_capped(cuda, starts, counts, q_heads, kv_heads, width, page, dtype, room):
+    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype, seed=1, room=room)
     check(attention.cached_attention(q, cache, table, s, o, scale=0.3, cap=20.0), q, cache, table, s, o, scale=0.3, cap=20.0)
 
 
+@pytest.mark.parametrize("room", [0, WIDE])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("starts,counts,q_heads,kv_heads,width,page", [
-    ([0], [1], 1, 1, 64, 16), ([100], [13], 8, 2, 128, 64), ([0, 33, 250], [64, 3, 20], 4, 1, 64, 32), ([5, 6], [16, 16], 32, 4, 128, 16),
+    ([0], [1], 1, 1, 64, 16), ([100], [13], 8, 2, 128, 64), ([1000, 3], [60, 64], 16, 2, 128, 32), ([127, 128], [64, 1], 8, 1, 64, 16), ([0, 33, 250], [64, 3, 20], 4, 1, 64, 32), ([5, 6], [16, 16], 32, 4, 128, 16),
     ([200], [64], 16, 2, 32, 64), ([90, 0, 1, 64], [9, 1, 30, 64], 4, 4, 256, 128),
 ])
-def test_trees(cuda, starts, counts, q_heads, kv_heads, width, page, dtype):
-    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype)
+def test_trees(cuda, starts, counts, q_heads, kv_heads, width, page, dtype, room):
+    q, cache, table, s, o = make(starts, counts, q_heads, kv_heads, width, page, dtype, room=room)
     bits = tree_bits(counts)
     check(attention.cached_attention(q, cache, table, s, o, visible=bits), q, cache, table, s, o, bits)
     check(attention.cached_attention(q, cache, table, s, o, visible=bits, cap=30.0), q, cache, table, s, o, bits, cap=30.0)
@@ -144,17 +151,21 @@ def test_many_sequences_of_all_lengths(cuda, dtype):
     check(attention.cached_attention(q, cache, table, s), q, cache, table, s, None)
 
 
-def test_a_row_that_sees_nothing_gets_zeros(cuda):
-    q, cache, table, s, o = make([0, 0, 50], [3, 2, 2], 4, 2, 64, 16, torch.bfloat16)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
+def test_a_row_that_sees_nothing_gets_zeros(cuda, q_heads, room, dtype):
+    q, cache, table, s, o = make([0, 0, 50], [3, 2, 2], q_heads, 2, 64, 16, dtype, room=room)
     bits = torch.tensor([0, 1, 0, 2, 2, 0, 3], device="cuda")
     got = attention.cached_attention(q, cache, table, s, o, visible=bits)
     assert bool((got[0] == 0).all()) and bool((got[2] == 0).all())
     check(got, q, cache, table, s, o, bits)
 
 
-def test_what_lies_behind_and_beside_a_sequence_does_not_reach_it(cuda):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (128, WIDE)])
+def test_what_lies_behind_and_beside_a_sequence_does_not_reach_it(cuda, q_heads, room, dtype):
     """Infinite and NaN scales in places that no token sees, in its own pages too."""
-    q, cache, table, s, o = make([20, 3], [1, 2], 4, 2, 64, 16, torch.float32)
+    q, cache, table, s, o = make([20, 3], [1, 2], q_heads, 2, 64, 16, dtype, room=room)
     bits = torch.tensor([1, 1, 2], device="cuda")
     plain, tree = attention.cached_attention(q, cache, table, s, o), attention.cached_attention(q, cache, table, s, o, visible=bits)
     held = torch.zeros(cache.keys.shape[0], 16, dtype=torch.bool, device="cuda")
@@ -172,30 +183,33 @@ def test_what_lies_behind_and_beside_a_sequence_does_not_reach_it(cuda):
         assert torch.equal(got[0], tree[0]) and torch.equal(got[2], tree[2]) and bool(got[1].isnan().all())
 
 
-def test_infinite_and_nan_queries_stay_in_their_rows(cuda):
-    for dtype in DTYPES:
-        q, cache, table, s, o = make([100], [5], 8, 2, 64, 16, dtype)
-        want = attention.cached_attention(q, cache, table, s, o)
-        q[1, 3, 7], q[4, 0, 0] = float("inf"), float("nan")
-        got = attention.cached_attention(q, cache, table, s, o)
-        assert bool(got[1, 3].isnan().all()) and bool(got[4, 0].isnan().all())
-        keep = torch.ones(5, 8, dtype=torch.bool)
-        keep[1, 3] = keep[4, 0] = False
-        assert torch.equal(got[keep], want[keep])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(8, 0), (8, WIDE), (64, WIDE)])
+def test_infinite_and_nan_queries_stay_in_their_rows(cuda, q_heads, room, dtype):
+    q, cache, table, s, o = make([100], [5], q_heads, 2, 64, 16, dtype, room=room)
+    want = attention.cached_attention(q, cache, table, s, o)
+    q[1, 3, 7], q[4, 0, 0] = float("inf"), float("nan")
+    got = attention.cached_attention(q, cache, table, s, o)
+    assert bool(got[1, 3].isnan().all()) and bool(got[4, 0].isnan().all())
+    keep = torch.ones(5, q_heads, dtype=torch.bool)
+    keep[1, 3] = keep[4, 0] = False
+    assert torch.equal(got[keep], want[keep])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (40, WIDE)])
 @pytest.mark.parametrize("size", [2.0**-12, 2.0**10])
-def test_rows_of_very_different_sizes(cuda, dtype, size):
+def test_rows_of_very_different_sizes(cuda, dtype, size, q_heads, room):
     """One key with a far larger or smaller value row than the others, and queries of that size."""
-    q, cache, table, s, o = make([300], [1], 4, 1, 128, 64, dtype)
+    q, cache, table, s, o = make([300], [1], q_heads, 1, 128, 64, dtype, room=room)
     cache.value_scales[table[0, 2], 0, 9] *= size * 64
     q = (q.float() * size).to(dtype)
     check(attention.cached_attention(q, cache, table, s, o, scale=0.1 / size), q, cache, table, s, o, scale=0.1 / size)
 
 
-def test_rows_of_no_sequence_are_left(cuda):
-    q, cache, table, s, _ = make([30, 5], [4, 8], 4, 2, 64, 16, torch.float16)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
+def test_rows_of_no_sequence_are_left(cuda, q_heads, room):
+    q, cache, table, s, _ = make([30, 5], [4, 8], q_heads, 2, 64, 16, torch.float16, room=room)
     o = vector([1, 4, 9])
     out = torch.full_like(q, 3.0)
     assert attention.cached_attention(q, cache, table, s, o, out=out) is out
@@ -203,8 +217,10 @@ def test_rows_of_no_sequence_are_left(cuda):
     check(out, q, cache, table, s, o)
 
 
-def test_pages_and_positions_that_are_not_there_are_left_out(cuda):
-    q, cache, table, s, o = make([60, 40, 3], [1, 1, 1], 4, 2, 64, 16, torch.float32)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (128, WIDE)])
+def test_pages_and_positions_that_are_not_there_are_left_out(cuda, q_heads, room, dtype):
+    q, cache, table, s, o = make([60, 40, 3], [1, 1, 1], q_heads, 2, 64, 16, dtype, room=room)
     table[0, 1], table[1, 0] = 10_000, -1
     s[2] = 64  # its 65 positions need a fifth page
     check(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o, longest=70)
@@ -218,27 +234,31 @@ def test_pages_and_positions_that_are_not_there_are_left_out(cuda):
 
 
 @pytest.mark.parametrize("offsets", [[0, 100, 3, 9], [-50, 4, 9, 400], [9, 6, 3, 0], [5, 5, 5, 5]])
-def test_offsets_that_make_no_sense_reach_nothing_outside(cuda, offsets):
-    q, cache, table, s, _ = make([30, 5, 0], [3, 3, 3], 4, 2, 64, 16, torch.bfloat16)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
+def test_offsets_that_make_no_sense_reach_nothing_outside(cuda, offsets, q_heads, room):
+    q, cache, table, s, _ = make([30, 5, 0], [3, 3, 3], q_heads, 2, 64, 16, torch.bfloat16, room=room)
     out = attention.cached_attention(q, cache, table, s, vector(offsets))
     attention.cached_attention(q, cache, table, s, vector(offsets), visible=tree_bits([9]), out=out)
     torch.cuda.synchronize()
 
 
-def test_queries_and_outputs_of_any_stride(cuda):
-    q, cache, table, s, o = make([30, 5], [3, 2], 4, 2, 64, 16, torch.bfloat16)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
+def test_queries_and_outputs_of_any_stride(cuda, q_heads, room, dtype):
+    q, cache, table, s, o = make([30, 5], [3, 2], q_heads, 2, 64, 16, dtype, room=room)
     want = attention.cached_attention(q, cache, table, s, o)
     for shift in (0, 1):
-        wide = torch.zeros(4, 5, 80, device="cuda", dtype=torch.bfloat16)[:, :, shift:64 + shift].transpose(0, 1)
+        wide = torch.zeros(q_heads, 5, 80, device="cuda", dtype=dtype)[:, :, shift:64 + shift].transpose(0, 1)
         wide.copy_(q)
-        out = torch.zeros(5, 8, 80, device="cuda", dtype=torch.bfloat16)[:, ::2, shift:64 + shift]
+        out = torch.zeros(5, 2 * q_heads, 80, device="cuda", dtype=dtype)[:, ::2, shift:64 + shift]
         assert torch.equal(attention.cached_attention(wide, cache, table, s, o, out=out), want)
-    one = q[:, :1].expand(5, 4, 64)
+    one = q[:, :1].expand(5, q_heads, 64)
     check(attention.cached_attention(one, cache, table, s, o), one, cache, table, s, o)
 
 
-def test_the_same_bits_on_every_run_and_stream(cuda):
-    q, cache, table, s, o = make([5000, 300, 12], [1, 1, 1], 16, 4, 128, 64, torch.bfloat16)
+@pytest.mark.parametrize("count", [1, 40])
+def test_the_same_bits_on_every_run_and_stream(cuda, count):
+    q, cache, table, s, o = make([5000, 300, 12], [count] * 3, 16, 4, 128, 64, torch.bfloat16, room=WIDE)
     want = attention.cached_attention(q, cache, table, s, o)
     streams = [torch.cuda.Stream() for _ in range(3)]
     outs = []
@@ -251,8 +271,9 @@ def test_the_same_bits_on_every_run_and_stream(cuda):
     assert all(torch.equal(x, want) for x in outs)
 
 
-def test_two_captured_calls_replay_side_by_side_with_other_lengths(cuda):
-    a, b = (make([4000, 100], [1, 1], 16, 4, 128, 64, torch.bfloat16, seed=i) for i in range(2))
+@pytest.mark.parametrize("count", [1, 30])
+def test_two_captured_calls_replay_side_by_side_with_other_lengths(cuda, count):
+    a, b = (make([4000, 4000], [count] * 2, 16, 4, 128, 64, torch.bfloat16, seed=i, room=WIDE) for i in range(2))
     graphs, outs = [], []
     for q, cache, table, s, o in (a, b):
         graph = torch.cuda.CUDAGraph()
@@ -260,7 +281,7 @@ def test_two_captured_calls_replay_side_by_side_with_other_lengths(cuda):
             outs.append(attention.cached_attention(q, cache, table, s, o))
         graphs.append(graph)
     side = torch.cuda.Stream()
-    for lengths in ([4000, 100], [0, 4001], [63, 64], [2111, 3000]):
+    for lengths in ([4000, 100], [0, 4000], [63, 64], [2111, 3000]):
         for call in (a, b):
             call[3].copy_(vector(lengths))
         want = [attention.cached_attention(*call[:4], call[4]) for call in (a, b)]
