@@ -130,7 +130,7 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
     need = lib.tgcb_cached_attention_scratch_bytes(cache.desc, b, q_heads)
     with heads.on_stream(index, stream):
         if out is None:
-            out = queries.new_empty(queries.shape)
+            out = heads.empty(queries)
         scratch = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     with heads.on_device(index):
         rc = lib.tgcb_cached_attention(

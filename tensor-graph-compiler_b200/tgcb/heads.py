@@ -22,7 +22,7 @@ _here = contextlib.nullcontext()
 def check_rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 3 or t.dtype not in DTYPES:
         raise ConfigError(f"{name} must be a CUDA tensor [tokens, heads, width] in float32, bfloat16 or float16")
-    if t.stride(2) != 1 and t.shape[2] != 1:
+    if t.stride()[2] != 1 and t.shape[2] != 1:
         raise ConfigError(f"{name} must have a unit stride along its width")
     if like is not None and (t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ConfigError(f"{name} must have the type and device of the other rows")
@@ -72,6 +72,11 @@ def check_apart(name: str, out: torch.Tensor, other_name: str, other: torch.Tens
         return
     if overlap(out, other):
         raise ConfigError(f"{name} overlaps {other_name}")
+
+
+def empty(like: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of the same shape, type and device."""
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 def rows(t: torch.Tensor) -> tuple[int, int, int]:

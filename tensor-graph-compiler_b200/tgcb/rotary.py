@@ -21,7 +21,7 @@ from tgcb import _lib, heads
 from tgcb.errors import ConfigError
 
 MAX_WIDTH = 1024
-_NONE = (None, 0, 0)
+_NONE = (0, 0, 0)
 
 
 def frequencies(rotary: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -57,13 +57,14 @@ def _check(queries, keys, query_gain, key_gain, positions, freqs, epsilon) -> No
         raise ConfigError(f"the epsilon has to be positive, got {epsilon}")
 
 
-def _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out, grads=(_NONE, _NONE)) -> _lib.RotaryDesc:
+def _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out, grads=(_NONE, _NONE),
+          gain_grads=(0, 0), scratch=(0, 0)) -> _lib.RotaryDesc:
     tokens, q_heads, width = queries.shape
-    return _lib.RotaryDesc(
+    return _lib.RotaryDesc.of(
         heads.DTYPES[queries.dtype], heads.DTYPES[query_gain.dtype], positions.element_size(), bool(interleaved), tokens,
-        (q_heads, keys.shape[1]), width, 2 * freqs.shape[0], epsilon, positions.data_ptr(), freqs.data_ptr(),
-        (query_gain.data_ptr(), key_gain.data_ptr()), (heads.rows(queries), heads.rows(keys)), grads,
-        (heads.rows(out[0]), heads.rows(out[1])),
+        q_heads, keys.shape[1], width, 2 * freqs.shape[0], epsilon, positions.data_ptr(), freqs.data_ptr(),
+        query_gain.data_ptr(), key_gain.data_ptr(), *heads.rows(queries), *heads.rows(keys), *grads[0], *grads[1],
+        *heads.rows(out[0]), *heads.rows(out[1]), *gain_grads, *scratch,
     )
 
 
@@ -105,7 +106,7 @@ def norm_rotate(queries: torch.Tensor, keys: torch.Tensor, query_gain: torch.Ten
     """
     _check(queries, keys, query_gain, key_gain, positions, frequencies, epsilon)
     with heads.on_stream(queries.get_device(), stream):
-        out = queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+        out = heads.empty(queries), heads.empty(keys)
     _run(queries, keys, query_gain, key_gain, positions, frequencies, epsilon, interleaved, out, stream)
     return out
 
@@ -130,13 +131,12 @@ def norm_rotate_backward(query_grad: torch.Tensor, key_grad: torch.Tensor, queri
     lib, width = _lib.load(), queries.shape[2]
     with heads.on_stream(index, stream):
         if out is None:
-            out = queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+            out = heads.empty(queries), heads.empty(keys)
         gains = query_gain.new_empty((2, width))
         scratch = torch.empty(lib.tgcb_norm_rotate_scratch_bytes(width), dtype=torch.uint8, device=queries.device)
     d = _desc(queries, keys, query_gain, key_gain, positions, frequencies, epsilon, interleaved, out,
-              (heads.rows(query_grad), heads.rows(key_grad)))
-    d.gain_grad[0], d.gain_grad[1] = gains.data_ptr(), gains.data_ptr() + width * gains.element_size()
-    d.scratch, d.scratch_bytes = scratch.data_ptr(), scratch.numel()
+              (heads.rows(query_grad), heads.rows(key_grad)), (gains.data_ptr(), gains.data_ptr() + width * gains.element_size()),
+              (scratch.data_ptr(), scratch.numel()))
     with heads.on_device(index):
         _lib.check(lib.tgcb_norm_rotate_backward(d, heads.raw(index, stream)), "tgcb_norm_rotate_backward")
     return out[0], out[1], gains[0], gains[1]
