@@ -12,7 +12,7 @@
 //     memory and V as it lies (columns contiguous).
 //   softmax (2 x 4 warps, a thread per row): the row's maximum, then weights e^(s - m) times the value's
 //     scale as two bfloat16 parts (16 bits, as in the kernel for few rows), written over the scores
-//     they came from: 32 scores' columns hold 16 columns of leading and 16 of remaining parts.
+//     they came from: 16 scores' columns hold 8 columns of leading and 8 of remaining parts.
 //     The accumulator is rescaled only when a maximum grows by more than 2^8, since the weights' sum
 //     and the products share whatever reference they were taken against.
 //
@@ -131,6 +131,18 @@ __device__ __forceinline__ void load32(unsigned tmem, unsigned* r) {
       : "r"(tmem)
       : "memory");
 }
+__device__ __forceinline__ void load16(unsigned tmem, unsigned* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16]; tcgen05.wait::ld.sync.aligned;"
+      : TGCB_R8(r, 0), TGCB_R8(r, 8)
+      : "r"(tmem)
+      : "memory");
+}
+__device__ __forceinline__ void store16(unsigned tmem, const unsigned* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(tmem),
+               TGCB_S8(r, 0), TGCB_S8(r, 8)
+               : "memory");
+}
 __device__ __forceinline__ void store32(unsigned tmem, const unsigned* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
@@ -220,13 +232,14 @@ struct Walk {
   }
 };
 
-template <typename T, int W, bool VALUES>
-__device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, int* status) {
+template <typename T, int W>
+__device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Args& a, Walk walk, Shared* sh, unsigned char* memory, int* status,
+                                        bool VALUES) {
   using M = Memory<W>;
   // 16-code pieces of a row; rows a pass copies. Eight neighbouring threads have four pieces of two rows, whose halves lie on
   // different banks.
   constexpr int CH = W / 16, PASSES = CH, PER = 128 / CH;
-  constexpr bool HALF = !VALUES && !std::is_same_v<T, __nv_bfloat16>;  // the values meet bfloat16 weights
+  const bool HALF = !VALUES && !std::is_same_v<T, __nv_bfloat16>;  // the values meet bfloat16 weights
   const int tid = threadIdx.x - (VALUES ? kValueThreads : kKeyThreads), piece = tid % 4 + (W == 128 ? tid / 64 * 4 : 0), in_pass = W == 128 ? tid % 64 / 4 : tid / 4;
   const float factor = (HALF ? 1.f : kCodeScale) * (a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f);
   unsigned mask, flip, magic;
@@ -397,7 +410,7 @@ __device__ __forceinline__ void multiply(Walk walk, Shared* sh, unsigned char* m
           for (int k = 0; k < kKeys / 16; ++k)
 #pragma unroll
             for (int part = 0; part < 2; ++part)
-              product_ts(tmem + g * W, weights + 32 * (k / 2) + 16 * part + 8 * (k % 2), values + k * 16 * 128 / 16, kOutputs,
+              product_ts(tmem + g * W, weights + 16 * k + 8 * part, values + k * 16 * 128 / 16, kOutputs,
                          t > 2 || k > 0 || part > 0);
           commit(&sh->pv_done[g]);
         }
@@ -426,13 +439,13 @@ template <bool MASKED, class Seen>
 __device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen seen_of) {
   float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-  for (int ch = 0; ch < 4; ++ch) {
-    unsigned r[32];
-    load32(scores + 32 * ch, r);
-    const unsigned see = MASKED ? seen_of(ch) : 0;
+  for (int ch = 0; ch < 8; ++ch) {
+    unsigned r[16];
+    load16(scores + 16 * ch, r);
+    const unsigned see = MASKED ? seen_of(ch / 2) >> (16 * (ch & 1)) : 0;
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j);
+    for (int j = 0; j < 16; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(ks + 16 * ch + j);
       float x[4] = {__uint_as_float(r[j]) * k.x, __uint_as_float(r[j + 1]) * k.y, __uint_as_float(r[j + 2]) * k.z, __uint_as_float(r[j + 3]) * k.w};
       if (MASKED) {
 #pragma unroll
@@ -444,19 +457,19 @@ __device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen s
   return fmaxf(top[0], top[1]);
 }
 
-// Writes a row's 128 weights times the values' scales over its scores, 32 at a time as 16 columns of leading and 16 of
+// Writes a row's 128 weights times the values' scales over its scores, 16 at a time as 8 columns of leading and 8 of
 // remaining parts, and returns the weights' sum.
 template <typename T, bool CAP, bool MASKED, class Seen>
 __device__ __forceinline__ float weights(unsigned scores, const float* ks, const float* vs, float base, float cap2, Seen seen_of) {
   float some[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-  for (int ch = 0; ch < 4; ++ch) {
-    unsigned r[32], parts[32];
-    load32(scores + 32 * ch, r);
-    const unsigned see = MASKED ? seen_of(ch) : 0;
+  for (int ch = 0; ch < 8; ++ch) {
+    unsigned r[16], parts[16];
+    load16(scores + 16 * ch, r);
+    const unsigned see = MASKED ? seen_of(ch / 2) >> (16 * (ch & 1)) : 0;
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(ks + 32 * ch + j), v = *reinterpret_cast<const float4*>(vs + 32 * ch + j);
+    for (int j = 0; j < 16; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(ks + 16 * ch + j), v = *reinterpret_cast<const float4*>(vs + 16 * ch + j);
       const float by[4] = {k.x, k.y, k.z, k.w}, scale[4] = {v.x, v.y, v.z, v.w};
       float w[4];
 #pragma unroll
@@ -469,11 +482,11 @@ __device__ __forceinline__ float weights(unsigned scores, const float* ks, const
       }
       unsigned two[2];
       split<2>(w[0], w[1], two);
-      parts[j / 2] = two[0], parts[16 + j / 2] = two[1];
+      parts[j / 2] = two[0], parts[8 + j / 2] = two[1];
       split<2>(w[2], w[3], two);
-      parts[j / 2 + 1] = two[0], parts[16 + j / 2 + 1] = two[1];
+      parts[j / 2 + 1] = two[0], parts[8 + j / 2 + 1] = two[1];
     }
-    store32(scores + 32 * ch, parts);
+    store16(scores + 16 * ch, parts);
   }
   return (some[0] + some[1]) + (some[2] + some[3]);
 }
@@ -665,12 +678,9 @@ __global__ void __launch_bounds__(kTensorThreads, 1) attend_tiles(const Cache c,
     if (threadIdx.x < kKeyThreads) {
       more_registers<kSoftmaxRegisters>();
       weigh<T, W>(c, b, a, walk, &sh, memory, tmem, status);
-    } else if (threadIdx.x < kValueThreads) {
-      fewer_registers<kConverterRegisters>();
-      convert<T, W, false>(c, b, a, walk, &sh, memory, status);
     } else if (threadIdx.x < kProducts) {
       fewer_registers<kConverterRegisters>();
-      convert<T, W, true>(c, b, a, walk, &sh, memory, status);
+      convert<T, W>(c, b, a, walk, &sh, memory, status, threadIdx.x >= kValueThreads);
     } else {
       fewer_registers<kProductRegisters>();
       if (threadIdx.x == kProducts) {
