@@ -488,15 +488,17 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
     for (int i = threadIdx.x; i < rows * QUADS; i += kThreads) {
       const int r = i / QUADS, quad = i - r * QUADS;
       const float* ml = joined + ROWS * S::OP + 2 * r;
-      float mm = -INFINITY, f[kWarps], all_sum = 0.f;
+      float mm = -INFINITY, f[kWarps];
+      Weights all;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[w * ROWS * (S::OP + 2)]);
       const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         f[w] = exp2_fast(ml[w * ROWS * (S::OP + 2)] - base);
-        add_sum(&all_sum, ml[w * ROWS * (S::OP + 2) + 1], f[w]);
+        all.add(ml[w * ROWS * (S::OP + 2) + 1], f[w]);
       }
+      const float all_sum = all.sum();
       const int col = 4 * quad;
       float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

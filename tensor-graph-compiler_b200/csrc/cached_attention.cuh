@@ -150,13 +150,17 @@ __device__ __forceinline__ void begin_at(const Cache& c, const Batch& b, const A
 }
 
 // Sums of weights of parts, where -1 marks a part whose scores were all -infinity: its factor is 0 beside
-// any other part, and a row with nothing else has no answer (NaN, as 0 / 0).
-__device__ __forceinline__ void add_sum(float* all, float sum, float factor) {
-  if (sum < 0.f)
-    *all = *all == 0.f ? -1.f : *all;
-  else if (sum != 0.f)
-    *all = fmaf(sum, factor, *all < 0.f ? 0.f : *all);
-}
+// any other part, and a row with nothing else has no answer (NaN, as 0 / 0). Without branches, which
+// would hold back the loads of the parts behind them.
+struct Weights {
+  float all = 0.f;
+  bool lowest = false;
+  __device__ __forceinline__ void add(float sum, float factor) {
+    lowest |= sum < 0.f;
+    all = fmaf(sum < 0.f ? 0.f : sum, factor, all);
+  }
+  __device__ __forceinline__ float sum() const { return all == 0.f && lowest ? -1.f : all; }
+};
 __device__ __forceinline__ float answer(float v, float sum) {
   return sum == 0.f ? 0.f : sum < 0.f ? __int_as_float(0x7fffffff) : v / sum;
 }
@@ -195,8 +199,7 @@ __device__ __forceinline__ bool out_wide(const Args& a) {
 
 // Joins the parts of the unit that begins in CTA blockIdx.x of `attend` and was cut at its end, in the
 // order of the keys: a warp per row, first the parts' maxima and sums (a lane per part), then the
-// weighted sums (a lane per four columns), eight parts' loads in flight. One thread per four columns that
-// walked all parts twice took 22 us for 28 parts of 8 units; this takes 4.
+// weighted sums (a lane per four columns), eight parts' loads in flight.
 template <typename T, int W, int RN>
 __global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, const Args a) {
   constexpr int ROWS = 8 * RN, QUADS = W / 4, PER = (QUADS + 31) / 32;
@@ -213,7 +216,8 @@ __global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, con
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
   const float base = mm == -INFINITY ? 0.f : mm;
-  float all_sum = 0.f, v[PER][4];
+  Weights all;
+  float v[PER][4];
 #pragma unroll
   for (int i = 0; i < PER; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
   for (int k0 = 0; k0 < n; k0 += 32) {
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, con
 #pragma unroll 8
     for (int k = 0; k < some; ++k) {
       const float f = __shfl_sync(0xffffffffu, mine, k);
-      add_sum(&all_sum, __shfl_sync(0xffffffffu, weights, k), f);
+      all.add(__shfl_sync(0xffffffffu, weights, k), f);
       const float* p = part(k0 + k) + r * W;
 #pragma unroll
       for (int i = 0; i < PER; ++i)
@@ -238,6 +242,7 @@ __global__ void __launch_bounds__(256) combine(const Cache c, const Batch b, con
     }
   }
   const bool wide = out_wide<T>(a);
+  const float all_sum = all.sum();
 #pragma unroll
   for (int i = 0; i < PER; ++i)
     if (QUADS >= 32 || lane < QUADS) {

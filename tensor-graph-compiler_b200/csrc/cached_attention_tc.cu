@@ -586,9 +586,10 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
     const float factor = exp2_fast(own.x - base);
     const bool complete = walk.from == 0 && walk.to == q.steps;
     float* part = complete ? nullptr : a.parts + (2ll * blockIdx.x + (walk.from == 0)) * kTensorRows * (W + 2);
-    float all_sum = 0.f;
-    add_sum(&all_sum, own.y, factor);
-    add_sum(&all_sum, other.y, exp2_fast(other.x - base));
+    Weights all;
+    all.add(own.y, factor);
+    all.add(other.y, exp2_fast(other.x - base));
+    const float all_sum = all.sum();
     const bool two = walk.tiles > 1;
     T* out = out_row<T>(a, q, walk.head, mine);
 #pragma unroll 1
@@ -714,18 +715,20 @@ __global__ void __launch_bounds__(kTensorRows) join_columns(const Cache c, const
 #pragma unroll 8
   for (int k = 0; k < n; ++k) mm = fmaxf(mm, part(k)[W * kTensorRows]);
   const float base = mm == -INFINITY ? 0.f : mm;
-  float all_sum = 0.f, v[kColumns];
+  Weights all;
+  float v[kColumns];
 #pragma unroll
   for (int i = 0; i < kColumns; ++i) v[i] = 0.f;
-#pragma unroll 2
+#pragma unroll 4
   for (int k = 0; k < n; ++k) {
     const float* p = part(k);
     const float f = exp2_fast(p[W * kTensorRows] - base);
-    add_sum(&all_sum, p[(W + 1) * kTensorRows], f);
+    all.add(p[(W + 1) * kTensorRows], f);
 #pragma unroll
     for (int i = 0; i < kColumns; ++i) v[i] = fmaf(p[(column + i) * kTensorRows], f, v[i]);
   }
   if (row >= q.rows * a.group - cut.z * kTensorRows) return;
+  const float all_sum = all.sum();
 #pragma unroll
   for (int i = 0; i < kColumns; ++i) v[i] = answer(v[i], all_sum);
   T* out = out_row<T>(a, q, cut.y, cut.z * kTensorRows + row) + column;
