@@ -333,7 +333,7 @@ typedef struct tgcb_cache {
   int32_t* faults;
   int64_t pages;
   int32_t kv_heads;
-  int32_t page;  /* places in a page: 16, 32, 64 or 128 */
+  int32_t page;  /* places in a page: 16, 32, 64 or 128; a table row holds at most 2^30 places */
   int32_t width; /* 32, 64, 128 or 256 */
 } tgcb_cache;
 
@@ -342,7 +342,7 @@ typedef struct tgcb_cache {
  * lies at position starts[b] + i, which is place position % page of page
  * table[b * table_stride + position / page]. Rows of no sequence are left as they were. A position that is
  * negative or past the table, and a page outside [0, pages), is never accessed: it counts in
- * cache->faults, an append skips it, a read gives NaN, and attention leaves its key out. */
+ * cache->faults (once or more often), an append skips it, a read gives NaN, and attention leaves its key out. */
 typedef struct tgcb_batch {
   const int32_t* table;
   const int32_t* starts;

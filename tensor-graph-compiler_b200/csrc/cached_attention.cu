@@ -14,14 +14,15 @@
 // float16, 3 from float32), the weights p_j * value scale into 2 parts (16 bits) for 16-bit rows, below their
 // own rounding, and 3 (24 bits) for float32 rows.
 //
-// What bounds it with few rows is reading the cache, 2 W + 8 bytes a position and head. Each
+// What bounds it with few rows is reading the cache, 2 W + 8 bytes a position and head, and next to that
+// the instructions for a key, of which the conversion of its codes is half (25 a key for bfloat16 rows, 32
+// for float32 ones). Measured: 64 tokens of 32 heads on 8 over 1024 to 4096 positions of width 128 (347 MB) in
+// 71 us, 4.9 TB/s; 2 float32 tokens over 131072 positions (554 MB) with a cap in 125 us, 4.4 TB/s. Each
 // warp streams its own 32-key steps through a private ring in shared memory (cp.async), with no
 // barrier between warps until a unit ends. The work is the list of all units' steps, cut into
 // equal pieces, one per CTA, whatever the sequences' lengths are (they are known on the device alone):
 // a unit that lies in one piece is finished there, one that is cut leaves its parts in scratch and
 // `combine` joins them in order, so results do not depend on timing.
-#include <cuda_runtime.h>
-
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -36,9 +37,9 @@ using namespace tgcb_attend;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 32;       // keys a warp takes at once; pages hold 16 or more, so a step touches at most two
-constexpr int kMaxCtas = 444;   // three per SM
+constexpr int kMaxCtas = 444;   // three per SM, which fit at once; with 888 the long float32 case took 160 instead of 142 us
 constexpr int kMinSteps = 8;    // steps a CTA takes at least: two per warp
-constexpr int kWholeBelow = 512;  // positions up to which units are not cut
+constexpr int kWholeBelow = 512;  // positions up to which units are not cut, which saves the second launch
 
 template <typename T>
 struct Parts;
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
     if (!a.whole) to = stop - at < to - from ? from + (int)(stop - at) : to;
     const int rows = min(ROWS, q.rows * a.group - tile * ROWS);
 
+    count_outside(c, q, a, head == 0 && tile == 0 && from == 0 && threadIdx.x == 0);
     // The unit's queries as right-hand fragments: word pair (part, k, lane) holds row lane / 4's columns
     // 16 k + 4 (lane % 4) + {0, 2} and {1, 3}, as `codes` delivers the keys' columns.
     __syncthreads();
@@ -374,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
           base[rn][j] = mn == -INFINITY ? 0.f : mn;
           sum[rn][j] *= keep[rn][j];
         }
-      constexpr bool FRESH = NP == 3;  // float32 rows: each step's products in accumulators of their own, added in float32
+      // float32 rows: each step's products in accumulators of their own, added in float32. The tensor cores cut off
+      // what does not fit their sums, which over thousands of steps would all err to the same side.
+      constexpr bool FRESH = NP == 3;
       if (!FRESH && __any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int rn = 0; rn < RN; ++rn)
@@ -540,6 +544,7 @@ int row_tiles(const Batch& b, int group, int width) {
 // and 485 us; one tree of 13 nodes over 2047 positions, too little to fill the longer pipeline, 43 and 37 us.
 bool for_tensor(const Cache& c, const Batch& b, int group) {
   if ((c.width != 64 && c.width != 128) || (b.tokens + b.batch - 1) / b.batch * group <= 32) return false;
+  if ((long long)c.pages * c.heads * c.page > 0x7fffffffll) return false;  // it numbers rows in 32 bits
   const long long units = (b.tokens * group + kTensorRows - 1) / kTensorRows * c.heads;
   return units * ((long long)b.max_pages * c.page / 128) >= 4 * kTensorCtas;
 }
@@ -628,6 +633,8 @@ int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int 
   if (b.tokens * q_heads > 0x7fffffffll) return bad("too many tokens");
   if (!std::isfinite(scale)) return bad("the scale must be finite");
   if (!(cap >= 0) || std::isinf(cap)) return bad("the cap must be finite and not negative");
+  // the largest factors that the kernels form of them, with room for their constants
+  if (std::fabs(scale) > 1.1e30f || (cap > 0 && !(std::fabs(scale / cap) <= 1.1e30f))) return bad("the scale under the cap is beyond float32");
   if (b.tokens == 0) return TGCB_OK;
   const size_t need = scratch_bytes(c, b, q_heads);
   if (need && (scratch == nullptr || scratch_size < need || (reinterpret_cast<uintptr_t>(scratch) & 15u)))

@@ -96,6 +96,11 @@ __device__ __forceinline__ Sequence sequence_of(const Batch& b, const Args& a, i
   return q;
 }
 
+// Counts a sequence that has positions before the first or past its table, once.
+__device__ __forceinline__ void count_outside(const Cache& c, const Sequence& q, const Args& a, bool once) {
+  if (once && (q.start < 0 || q.start + q.rows > a.capacity)) atomicAdd(c.faults, 1);
+}
+
 template <int ROWS, int STEP>
 __device__ __forceinline__ long long work_of(const Cache& c, const Batch& b, const Args& a, int s) {
   const Sequence q = sequence_of<ROWS, STEP>(b, a, s);

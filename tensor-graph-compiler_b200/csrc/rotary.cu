@@ -148,7 +148,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
 // hidden is the latency of the rows and of the angles (float64 products, once a token for all
 // heads). So CTAs are persistent, and each thread copies its own vectors kStages - 1 steps ahead into slots of
 // shared memory that no other thread touches. Angles are computed for as many tiles of tokens at a time (a
-// batch) as gives every thread one, a batch ahead, so that there is one barrier a batch.
+// batch) as gives every thread one, a batch ahead, so that there is one barrier a batch. Measured, 8192 tokens
+// of 32 + 8 bfloat16 heads of 128: forward 40 us (168 MB, 4.2 TB/s), backward 56 us (252 MB, 4.5 TB/s), held by
+// their instructions (some 350 a warp and step, for 16-bit elements twice the float32 ones' a byte); 4095 tokens
+// of 16 + 4 float32 heads, backward: 20 us (126 MB, 6.2 TB/s).
 // Threads a CTA has at most, and the CTAs of that size that fit an SM's registers: 64 a thread forward, 102 backward.
 constexpr int kVecThreads[2] = {512, 320};
 constexpr int kVecResident = 2;
@@ -474,7 +477,7 @@ int check(const tgcb_rotary_desc* d, bool backward, const char* what) {
   if (d->tokens > (1ll << 40)) return bad("too many tokens");
   if (d->width < 2 || d->width > kMaxWidth) return bad("width must be from 2 to 1024");
   if (d->rotary < 2 || d->rotary > d->width || d->rotary % 2) return bad("rotary must be even, from 2 to width");
-  if (!(d->epsilon > 0)) return bad("epsilon must be positive");
+  if (!(d->epsilon > 0) || !((float)d->epsilon > 0) || std::isinf((float)d->epsilon)) return bad("epsilon must be a positive float32");
   for (int i = 0; i < 2; ++i) {
     if (d->gain[i] == nullptr || d->frequencies == nullptr) return bad("null pointer");
     if (backward && d->gain_grad[i] == nullptr) return bad("null pointer");

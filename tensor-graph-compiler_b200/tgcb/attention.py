@@ -120,6 +120,8 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
     cap = 0.0 if cap is None else float(cap)
     if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
         raise ConfigError(f"the scale has to be finite and the cap finite and not negative, got {scale} and {cap}")
+    if max(abs(scale), abs(scale) / cap if cap else 0.0) > 1e30:
+        raise ConfigError(f"a scale of {scale} under a cap of {cap} is beyond float32")
     if out is not None:
         heads.check_rows("out", out, queries)
         if out.shape != queries.shape:

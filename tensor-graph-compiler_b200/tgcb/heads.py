@@ -95,11 +95,14 @@ def on_stream(index: int, stream):
     """A context in which ``stream`` (None: the current one) is current, for what a call allocates."""
     if stream is None:
         return _here
-    if stream.device.index != index:
-        raise ConfigError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
+    raw(index, stream)
     return torch.cuda.stream(stream)
 
 
 def raw(index: int, stream) -> int:
     """The handle of ``stream``, or of the device's current one (its number alone: a Stream object costs microseconds)."""
-    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(index)
+    if stream.device.index != index:
+        raise ConfigError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
+    return stream.cuda_stream

@@ -53,8 +53,8 @@ def _check(queries, keys, query_gain, key_gain, positions, freqs, epsilon) -> No
     if not 1 <= half <= width // 2:
         raise ConfigError(f"frequencies must be a vector of 1 to {width // 2} values for heads of width {width}")
     heads.check_vector("frequencies", freqs, half, (torch.float64,), index)
-    if not epsilon > 0:
-        raise ConfigError(f"the epsilon has to be positive, got {epsilon}")
+    if not 1e-37 <= epsilon < 1e38:
+        raise ConfigError(f"the epsilon has to be a positive float32, got {epsilon}")
 
 
 def _desc(queries, keys, query_gain, key_gain, positions, freqs, epsilon, interleaved, out, grads=(_NONE, _NONE),

@@ -27,7 +27,7 @@ def rotary_desc(**change):
 @pytest.mark.parametrize("change,why", [
     (dict(dtype=3), "element type"), (dict(dtype=-1), "element type"), (dict(gain_dtype=1), "gains"), (dict(position_bytes=2), "positions"),
     (dict(tokens=-1), "negative"), (dict(heads=(0, 1)), "head"), (dict(width=1), "width"), (dict(width=1025), "width"), (dict(rotary=0), "rotary"),
-    (dict(rotary=63), "rotary"), (dict(rotary=66), "rotary"), (dict(epsilon=0.0), "epsilon"), (dict(epsilon=float("nan")), "epsilon"),
+    (dict(rotary=63), "rotary"), (dict(rotary=66), "rotary"), (dict(epsilon=0.0), "epsilon"), (dict(epsilon=float("nan")), "epsilon"), (dict(epsilon=1e-60), "epsilon"),
     (dict(positions=None), "null"), (dict(frequencies=None), "null"), (dict(gain=(HERE, None)), "null"), (dict(heads=(1 << 21, 1)), "2\\^20"),
 ])
 def test_norm_rotate_refuses(change, why):
@@ -82,7 +82,7 @@ def test_null_rows_and_descriptors_are_refused():
 
 
 @pytest.mark.parametrize("q_heads,scale,cap", [(3, 1.0, 0.0), (0, 1.0, 0.0), (4, float("nan"), 0.0), (4, float("inf"), 0.0), (4, 1.0, -1.0),
-                                               (4, 1.0, float("nan")), (4, 1.0, float("inf"))])
+                                               (4, 1.0, float("nan")), (4, 1.0, float("inf")), (4, 1e31, 0.0), (4, 1.0, 1e-35)])
 def test_attention_refuses(q_heads, scale, cap):
     lib, rows = _lib.load(), _lib.Heads(HERE, 256, 64)
     rc = lib.tgcb_cached_attention(cache_desc(), batch_desc(), 0, q_heads, rows, None, scale, cap, rows, HERE, 1 << 40, None)

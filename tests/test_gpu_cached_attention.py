@@ -233,6 +233,28 @@ def test_pages_and_positions_that_are_not_there_are_left_out(cuda, q_heads, room
     check(got, q, cache, table, s, o, longest=70)
 
 
+@pytest.mark.parametrize("start", [-3, 64, 63])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (128, WIDE)])
+def test_positions_outside_the_table_are_counted(cuda, q_heads, room, start):
+    q, cache, table, s, o = make([62], [2], q_heads, 2, 64, 16, torch.bfloat16, room=room)
+    attention.cached_attention(q, cache, table, s, o)
+    cache.check()
+    s.fill_(start if start < 0 or not room else start - 64 + table.shape[1] * 16)
+    attention.cached_attention(q, cache, table, s, o)
+    with pytest.raises(ConfigError):
+        cache.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_in_short_tables(cuda, dtype):
+    """Units that are never cut, enough of them for every kernel."""
+    starts = [(29 * i) % 400 for i in range(16)]
+    q, cache, table, s, o = make(starts, [40] * 16, 32, 8, 64, 64, dtype, room=512)
+    check(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+    bits = tree_bits([40] * 16)
+    check(attention.cached_attention(q, cache, table, s, o, visible=bits, cap=25.0), q, cache, table, s, o, bits, cap=25.0)
+
+
 @pytest.mark.parametrize("offsets", [[0, 100, 3, 9], [-50, 4, 9, 400], [9, 6, 3, 0], [5, 5, 5, 5]])
 @pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
 def test_offsets_that_make_no_sense_reach_nothing_outside(cuda, offsets, q_heads, room):
@@ -331,7 +353,7 @@ def test_refusals(cuda):
         dict(queries=q[:5], offsets=None), dict(queries=q[:, :0]), dict(cache=cache.keys), dict(table=table.long()), dict(starts=s[:1]),
         dict(starts=s.long()), dict(offsets=o[:2]), dict(visible=bits.int()), dict(visible=bits[:3]), dict(scale=float("nan")),
         dict(scale=float("inf")), dict(cap=-1.0), dict(cap=float("inf")), dict(out=q), dict(out=torch.empty_like(q).half()),
-        dict(out=torch.empty_like(q)[:3]), dict(out=torch.empty(1, 4, 64, device="cuda").expand(6, 4, 64)),
+        dict(scale=1e31), dict(cap=1e-35), dict(out=torch.empty_like(q)[:3]), dict(out=torch.empty(1, 4, 64, device="cuda").expand(6, 4, 64)),
     ):
         with pytest.raises(ConfigError):
             attention.cached_attention(**{**dict(queries=q, cache=cache, table=table, starts=s, offsets=o), **change})

@@ -205,7 +205,7 @@ def test_refusals(cuda):
         dict(queries=q.cpu()), dict(queries=q.double()), dict(queries=q[0]), dict(keys=k.half()), dict(keys=k[:3]), dict(keys=k[:, :, :32]),
         dict(queries=q[:, :0]), dict(query_gain=qg[:5]), dict(query_gain=qg.half()), dict(key_gain=kg.cpu()), dict(positions=pos.float()),
         dict(positions=pos[:2]), dict(frequencies=freq.float()), dict(frequencies=freq[:0]), dict(frequencies=torch.cat([freq, freq])),
-        dict(epsilon=0.0), dict(queries=torch.randn(4, 64, 2, device="cuda").transpose(1, 2)),
+        dict(epsilon=0.0), dict(epsilon=1e-60), dict(queries=torch.randn(4, 64, 2, device="cuda").transpose(1, 2)),
     ]
     for change in bad:
         with pytest.raises(ConfigError):
