@@ -540,8 +540,9 @@ int row_tiles(const Batch& b, int group, int width) {
 
 // Calls in 16 bits and widths 64 and 128 take the tcgen05 kernel, with units of 128 rows, where sequences have more than
 // 32 query rows a key head on average and the call may have four tiles of 128 keys for every SM. Measured there and
-// here: 2 x 509 tokens behind 4000 positions 143 and 363 us, 32 trees of 1 to 31 nodes over 2000 to 8000 positions 306
-// and 485 us; one tree of 13 nodes over 2047 positions, too little to fill the longer pipeline, 43 and 37 us.
+// here: 2 x 509 tokens behind 4000 positions 132 and 367 us, 32 trees of 1 to 31 nodes over 2000 to 8000 positions 273
+// and 515 us; one tree of 13 nodes over 2047 positions, too little to fill the longer pipeline, 50 and 42 us (each
+// from a cold L2, a single call).
 bool for_tensor(const Cache& c, const Batch& b, int group) {
   if ((c.width != 64 && c.width != 128) || (b.tokens + b.batch - 1) / b.batch * group <= 32) return false;
   if ((long long)c.pages * c.heads * c.page > 0x7fffffffll) return false;  // it numbers rows in 32 bits

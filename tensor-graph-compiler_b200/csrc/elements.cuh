@@ -68,8 +68,6 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int i, float x) {
     static_cast<__half*>(p)[i] = from_float<__half>(x);
 }
 
-inline int dtype_bytes(int dtype) { return dtype == TGCB_F32 ? 4 : 2; }
-
 }  // namespace tgcb_elem
 
 #endif  // TGCB_ELEMENTS_CUH_

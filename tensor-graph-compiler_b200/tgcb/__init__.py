@@ -9,6 +9,9 @@ Public surface, mirroring tgc's names:
   tgcb.summation     pairwise / sequential float32 sums on the GPU (tgc/analysis/summation.py)
   tgcb.quantize      per-row symmetric int8 quantisation on the GPU (tgc/analysis/quantize.py)
   tgcb.parallel      batch sharding across GPUs with NCCL (tgc/parallel/shard.py, collective.py)
+  tgcb.rotary        RMS norms of query and key heads with the position rotation (tgc/analysis/normalisation.py)
+  tgcb.kv_cache      a paged int8 cache of keys and values (tgc/analysis/quantize.py)
+  tgcb.attention     streaming attention, and attention over that cache (tgc/analysis/attention.py)
 """
 
 __version__ = "0.1.0"

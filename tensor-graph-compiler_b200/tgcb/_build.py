@@ -1,7 +1,7 @@
 """Build libtgcb.so in-tree with nvcc for sm_100a.
 
 The library holds the runtime (NVRTC compilation, module loading, plan execution) and the
-ahead-of-time kernels (long sums, the int8 quantiser). Generated kernels are compiled at
+ahead-of-time kernels (long sums, the int8 quantiser, attention, the token-generation operators). Generated kernels are compiled at
 ``compile_graph`` time by the library itself, so only this one shared object is built here.
 """
 
