@@ -132,6 +132,19 @@ def test_trees(cuda, starts, counts, q_heads, kv_heads, width, page, dtype, room
     check(attention.cached_attention(q, cache, table, s, o, visible=bits, cap=30.0), q, cache, table, s, o, bits, cap=30.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (32, WIDE)])
+def test_rows_behind_the_64th_cannot_be_named(cuda, q_heads, room, dtype):
+    """Any bits, rows ahead among them, in sequences of more than 64 rows: bit j is row j, no row is bit 64."""
+    counts = [100, 3, 65, 129]
+    q, cache, table, s, o = make([30, 0, 127, 500], counts, q_heads, 2, 64, 32, dtype, room=room)
+    g = torch.Generator().manual_seed(3)
+    bits = torch.randint(-(1 << 63), (1 << 63) - 1, (sum(counts),), generator=g).cuda()
+    bits[::7] = -1
+    check(attention.cached_attention(q, cache, table, s, o, visible=bits), q, cache, table, s, o, bits)
+    cache.check()
+
+
 def test_one_count_for_all_is_the_same_call(cuda):
     q, cache, table, s, o = make([40, 3, 77], [5, 5, 5], 8, 2, 64, 16, torch.bfloat16)
     assert torch.equal(attention.cached_attention(q, cache, table, s), attention.cached_attention(q, cache, table, s, o))
@@ -142,6 +155,26 @@ def test_one_count_for_all_is_the_same_call(cuda):
 def test_long_contexts(cuda, length, kv_heads, dtype):
     q, cache, table, s, o = make([length, 700], [1, 1], 4 * kv_heads, kv_heads, 128, 64, dtype)
     check(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+
+
+@pytest.mark.parametrize("q_heads", [4, 128])
+def test_pages_whose_offsets_pass_32_bits(cuda, q_heads):
+    """The same pages at the end of a cache of 4.6 GB of key codes: the same bits, written and read there too."""
+    q, near, table, s, o = make([700, 5], [1, 3], q_heads, 2, 128, 128, torch.bfloat16, room=WIDE)
+    pages, own = 140_000, near.pages
+    far = kv_cache.QuantisedCache(pages, 2, 128, page=128)
+    assert far.keys.numel() > 1 << 32
+    for a, b in ((near.keys, far.keys), (near.key_scales, far.key_scales), (near.values, far.values), (near.value_scales, far.value_scales)):
+        b[pages - own:] = a
+    moved = torch.where(table < 0, table, table + (pages - own))
+    assert torch.equal(attention.cached_attention(q, far, moved, s, o), attention.cached_attention(q, near, table, s, o))
+    rows = torch.randn(4, 2, 128, device="cuda").bfloat16()
+    for cache, at in ((near, table), (far, moved)):
+        cache.append(rows, -rows, at, s, o)
+        cache.check()
+    for a, b in zip(near.read(4, table, s, o), far.read(4, moved, s, o), strict=True):
+        assert torch.equal(a, b)
+    assert torch.equal(near.keys, far.keys[pages - own:]) and not bool(far.keys[:own].any())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
