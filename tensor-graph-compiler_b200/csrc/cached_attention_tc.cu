@@ -16,9 +16,9 @@
 //     The accumulator is rescaled only when a maximum grows by more than 2^8, since the weights' sum
 //     and the products share whatever reference they were taken against.
 //
-// Bound by the SM's instruction issue: 20 warps of three codes at 0.4 instructions a cycle and scheduler, waiting for
-// instruction fetch, tensor memory and one another (2.8 us for 128 rows x 128 keys at width 128, of which the products
-// take 0.4). Loops are kept short for that reason. Measured: 2 x 509 tokens of 16 heads on 4 behind 4000
+// Bound by its 20 warps of three codes, which issue 0.53 instructions a cycle and scheduler and wait for one another,
+// tensor memory and instruction fetch (4.1 to 4.3 us for 128 rows x 128 keys at width 128, of which the products, the
+// second in two parts, take 1.1). Loops are kept short for that reason. Measured: 2 x 509 tokens of 16 heads on 4 behind 4000
 // positions 122 us, 290 TFLOP/s; 32 trees of 1 to 31 nodes, 32 heads on 8, over 2000 to 8000 positions 255 to 268
 // us (calls in a row).
 // All waits are bounded (4 s); a CTA that gives up records status 2 and unwinds.
