@@ -24,7 +24,7 @@ struct Rows {
 };
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 16;  // tokens a CTA takes at most
+constexpr int kTokens = 32;  // tokens a CTA takes at most: a warp has a thread for each
 
 // Where a token row lies: the page and place of its position. Page -1: the position or the table's
 // entry is out of range; kNoSequence: the row belongs to no sequence.
@@ -33,41 +33,50 @@ struct __align__(8) Place {
 };
 constexpr int kNoSequence = -2;
 
-// The places of token rows [token0, token0 + count), by the whole CTA; a barrier must follow. Each thread
-// looks at its share of the sequences for the rows that are theirs. *least: the first sequence met.
+// The places of token rows [token0, token0 + count), by the whole CTA; a barrier must be before and follow. Threads
+// look at their share of the sequences for the rows that are theirs, then a thread a row looks up its place: a
+// sequence's thread doing that row by row waited for one page number after another, 4 of append's 40 us and of read's 37.
+// *least: the first sequence met.
 __device__ __forceinline__ void find_places(const Cache& c, const Batch& b, long long token0, int count, Place* places, int* least) {
-  auto fill = [&](int s, long long first, long long token) {
-    const long long position = (long long)__ldg(b.starts + s) + token - first;
-    const int page = tgcb_kv::page_of(c, b, s, position);
-    if (page < 0) atomicAdd(c.faults, 1);
-    places[token - token0] = Place{page, (int)(position & (c.page - 1))};
-    atomicMin(least, s);
-  };
-  if (b.offsets == nullptr) {
-    if (threadIdx.x < count) {
-      const int s = (int)((token0 + threadIdx.x) / b.each);
-      fill(s, (long long)s * b.each, token0 + threadIdx.x);
+  if (b.offsets != nullptr) {
+    for (int s = threadIdx.x; s < b.batch; s += kThreads) {
+      long long first, last;
+      tgcb_kv::range_of(b, s, &first, &last);
+      for (long long t = first > token0 ? first : token0; t < last && t < token0 + count; ++t) places[t - token0].row = s;
     }
-    return;
+    __syncthreads();
   }
-  for (int s = threadIdx.x; s < b.batch; s += kThreads) {
+  if (threadIdx.x >= 32) return;
+  const int i = threadIdx.x;
+  const int s = i >= count ? -1 : b.offsets == nullptr ? (int)((token0 + i) / b.each) : places[i].row;
+  if (s >= 0) {
     long long first, last;
     tgcb_kv::range_of(b, s, &first, &last);
-    for (long long t = first > token0 ? first : token0; t < last && t < token0 + count; ++t) fill(s, first, t);
+    const long long position = (long long)__ldg(b.starts + s) + token0 + i - first;
+    const int page = tgcb_kv::page_of(c, b, s, position);
+    if (page < 0) atomicAdd(c.faults, 1);
+    places[i] = Place{page, (int)(position & (c.page - 1))};
   }
+  const int smallest = __reduce_min_sync(0xffffffffu, s < 0 ? b.batch : s);
+  if (i == 0) *least = smallest;
 }
 
 // later[i] becomes 1 where a later row of the call has row i's place: two sequences that share a page both
 // write to, or a page twice in one table row. The call's written pages are few beside its rows; a
-// thread takes a sequence, and a sequence of many pages is taken by its warp.
+// thread takes a sequence, and a sequence of many pages is taken by its warp. Rows that follow one another in a
+// page are compared as one: looking at each took 10 of append's 54 us.
 __device__ __forceinline__ void find_later(const Cache& c, const Batch& b, long long token0, int count, const Place* places, int least, int* later) {
   const int lane = threadIdx.x & 31;
+  if (least + (int)(threadIdx.x & ~31) >= b.batch) return;  // whole warps
+  const int page_here = lane < count ? places[lane].page : kNoSequence, page_before = __shfl_up_sync(0xffffffffu, page_here, 1);
+  const unsigned runs = __ballot_sync(0xffffffffu, lane < count && (lane == 0 || page_here != page_before));
   auto look = [&](int page, long long slot, long long first, long long last, long long start) {
     if (page < 0) return;
-    for (int i = 0; i < count; ++i) {
-      if (page != places[i].page) continue;
-      const long long at = first + (slot << c.page_bits) + places[i].row - start;
-      if (at > token0 + i && at >= first && at < last) later[i] = 1;
+    for (unsigned r = runs; r; r &= r - 1) {
+      for (int i = __ffs(r) - 1; i < count && places[i].page == page; ++i) {
+        const long long at = first + (slot << c.page_bits) + places[i].row - start;
+        if (at > token0 + i && at >= first && at < last) later[i] = 1;
+      }
     }
   };
   for (int s0 = least + (threadIdx.x & ~31); s0 < b.batch; s0 += kThreads) {
@@ -150,14 +159,16 @@ struct Eight {
   }
 };
 
-// Codes of eight values: rint(x / scale). x * (1 / scale) is off by 2^-22 of the quotient at most, so
-// away from half-integers (3e-5) it rounds as the quotient does, and a thread with a value near one divides. With
-// a finite maximum and reciprocal |x / scale| <= 127 (1 + 2^-21): no clamp; other rows divide and
-// clamp. Adding 1.5 2^23 rounds to an integer, ties to even, in the sum's low bits.
-__device__ __forceinline__ uint2 codes_of(const float* x, float largest, float scale) {
-  const float inverse = __fdiv_rn(1.0f, scale);
+// Codes of eight values: rint(x / scale). With the approximate reciprocal (2 ulp for scales of normal size) x * (1 / scale)
+// is off by 2^-22 + 2^-24 of the quotient, 3.8e-5 at most, so away from half-integers (5e-5) it rounds
+// as the quotient does, and values near one are divided (normal bfloat16 values have some in 45% of the warps:
+// max / 2 is 63.5 scales). There |x / scale| <= 127 (1 + 2^-21):
+// no clamp; other rows divide and clamp. Adding 1.5 2^23 rounds to an integer, ties to even, in the sum's low bits.
+template <bool SIXTEEN>
+__device__ __forceinline__ uint2 codes_of(const float* x, float scale) {
   unsigned q[8];
-  if (isfinite(inverse) && isfinite(largest)) {
+  if (scale >= 0x1p-126f && scale <= 0x1p126f) {  // not NaN, not infinite
+    const float inverse = __fdividef(1.0f, scale);
     float near = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -165,9 +176,12 @@ __device__ __forceinline__ uint2 codes_of(const float* x, float largest, float s
       near = fmaxf(near, fabsf(t - (rounded - 12582912.0f)));
       q[i] = __float_as_uint(rounded);
     }
-    if (near >= 0.49997f) {
+    if (near >= 0.49995f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__fdiv_rn(x[i], scale) + 12582912.0f);
+      for (int i = 0; i < 8; ++i) {
+        const float d = x[i] * inverse;
+        if (!SIXTEEN || fabsf(d - (__uint_as_float(q[i]) - 12582912.0f)) >= 0.49995f) q[i] = __float_as_uint(__fdiv_rn(x[i], scale) + 12582912.0f);
+      }
     }
   } else {
 #pragma unroll
@@ -188,9 +202,9 @@ __device__ __forceinline__ float larger(float a, float b) {
 
 // Bound by HBM: append reads a row and writes width + 4 bytes, read the reverse. width / 8 threads have a
 // row; a CTA takes `each` tokens with all their heads, keys then values, and has the values of kAhead
-// rounds on their way at once. Measured, 16384 tokens of 8 + 8 float32 heads of 128 (169 MB each way): read 30 us,
-// 5.7 TB/s; append 51 us, 3.3 TB/s, held by looking up its tokens' places before its first store and by the
-// instructions of two divisions and the rounding.
+// rounds on their way at once. Measured, 16384 tokens of 8 + 8 float32 heads of 128 (169 MB each way): read 29 us,
+// 5.8 TB/s; append 37 us, 4.6 TB/s, held by the look-up of its tokens' places before its first store (with 16 tokens a
+// CTA 2 us more, for two rounds of it) and by instructions: 190 a warp for 32 eights of values.
 template <typename T>
 constexpr int kAhead = 8 / sizeof(T);  // 64 bytes a thread, within the registers of four CTAs an SM
 
@@ -206,17 +220,16 @@ struct Group {
   }
 };
 
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
-                                                        int lanes_log) {
+template <typename T, int W, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each) {
   __shared__ Place places[kTokens];
   __shared__ int later[kTokens], least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
-  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), groups = kThreads >> lanes_log;
-  const Group g(threadIdx.x >> lanes_log, groups, 2 * c.heads);
-  if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence, later[threadIdx.x] = 0;
-  if (threadIdx.x == 0) least = b.batch;
+  constexpr int lanes = W / 8, groups = kThreads / lanes;
+  const int item = threadIdx.x % lanes;
+  const Group g(threadIdx.x / lanes, groups, 2 * c.heads);
+  if (threadIdx.x < kTokens) places[threadIdx.x] = Place{kNoSequence, -1}, later[threadIdx.x] = 0;
 
   for (int row0 = 0; row0 < g.rows; row0 += groups) {
     const int row = row0 + g.row;
@@ -227,27 +240,30 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cac
     const long long t = rows.t;
     int8_t* codes = value ? c.values : c.keys;
     float* scales = value ? c.value_scales : c.key_scales;
-    for (int base = 0; base < count; base += kAhead<T> * g.step) {
-      Eight<T, WHOLE> x[kAhead<T>];
+    // each row's registers take the next round's row as soon as its values are out of them
+    Eight<T, WHOLE> x[kAhead<T>];
+    auto load = [&](int i, int token) {
+      if (real && token < count) x[i].load(from + token * t, item, W);
+    };
 #pragma unroll
-      for (int i = 0; i < kAhead<T>; ++i) {
-        const int token = base + i * g.step + g.token;
-        if (real && token < count) x[i].load(from + token * t, item, c.width);
-      }
-      if (row0 == 0 && base == 0) {
-        __syncthreads();
-        find_places(c, b, token0, count, places, &least);
-        __syncthreads();
-        find_later(c, b, token0, count, places, least, later);
-        __syncthreads();
-      }
+    for (int i = 0; i < kAhead<T>; ++i) load(i, i * g.step + g.token);
+    if (row0 == 0) {
+      __syncthreads();
+      find_places(c, b, token0, count, places, &least);
+      __syncthreads();
+      find_later(c, b, token0, count, places, least, later);
+      __syncthreads();
+    }
+    for (int base = 0; base < count; base += kAhead<T> * g.step) {
 #pragma unroll
       for (int i = 0; i < kAhead<T>; ++i) {
         float v[8], largest = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = to_float(x[i].e[j]), largest = larger(largest, v[j]);
-        for (int o = lanes >> 1; o > 0; o >>= 1) largest = larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         const int token = base + i * g.step + g.token;
+        load(i, token + kAhead<T> * g.step);
+#pragma unroll
+        for (int o = lanes / 2; o > 0; o /= 2) largest = larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         if (!real || token >= count || later[token]) continue;
         const Place place = places[token];
         if (place.page < 0) continue;
@@ -255,24 +271,23 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 4 : 2) append_rows(const Cac
         // way is never moved to another float32 by it
         const float scale = largest == 0.0f ? 1.0f : __fdiv_rn(largest, 127.0f);
         const long long at = ((long long)place.page * c.heads + head) * c.page + place.row;
-        Eight<T, WHOLE>::store_codes(codes + at * c.width, item, c.width, codes_of(v, largest, scale));
+        Eight<T, WHOLE>::store_codes(codes + at * W, item, W, codes_of<sizeof(T) == 2>(v, scale));
         if (item == 0) scales[at] = scale;
       }
     }
   }
 }
 
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each,
-                                                      int lanes_log) {
+template <typename T, int W, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch b, const Rows keys, const Rows values, int each) {
   __shared__ Place places[kTokens];
   __shared__ int least;
   const long long token0 = (long long)blockIdx.x * each;
   const int count = (int)min((long long)each, b.tokens - token0);
-  const int lanes = 1 << lanes_log, item = threadIdx.x & (lanes - 1), groups = kThreads >> lanes_log;
-  const Group g(threadIdx.x >> lanes_log, groups, 2 * c.heads);
-  if (threadIdx.x < kTokens) places[threadIdx.x].page = kNoSequence;
-  if (threadIdx.x == 0) least = b.batch;
+  constexpr int lanes = W / 8, groups = kThreads / lanes;
+  const int item = threadIdx.x % lanes;
+  const Group g(threadIdx.x / lanes, groups, 2 * c.heads);
+  if (threadIdx.x < kTokens) places[threadIdx.x] = Place{kNoSequence, -1};
   __syncthreads();
   find_places(c, b, token0, count, places, &least);
   __syncthreads();
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
         mine[i] = place.page != kNoSequence;
         if (place.page >= 0) {
           const long long at = ((long long)place.page * c.heads + head) * c.page + place.row;
-          q[i] = Eight<T, WHOLE>::load_codes(codes + at * c.width, item, c.width);
+          q[i] = Eight<T, WHOLE>::load_codes(codes + at * W, item, W);
           scale[i] = scales[at];
         }
       }
@@ -309,31 +324,40 @@ __global__ void __launch_bounds__(kThreads) read_rows(const Cache c, const Batch
           const int code = (int)(signed char)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3)));
           x.e[j] = from_float<T>((float)code * scale[i]);
         }
-        if (mine[i]) x.store(to + (base + i * g.step) * t, item, c.width);
+        if (mine[i]) x.store(to + (base + i * g.step) * t, item, W);
       }
     }
   }
 }
 
-template <typename T>
+template <typename T, int W>
 int run(const Cache& c, const Batch& b, const Rows& k, const Rows& v, bool read, cudaStream_t s) {
   if (b.tokens == 0) return TGCB_OK;
   // whole rounds of the 592 CTAs that are resident at once, of at most kTokens tokens each
   const long long rounds = (b.tokens + 592 * kTokens - 1) / (592 * kTokens);
   const int each = (int)((b.tokens + 592 * rounds - 1) / (592 * rounds));
   const unsigned grid = (unsigned)((b.tokens + each - 1) / each);
-  const int lanes_log = __builtin_ctz((unsigned)c.width / 8);
   bool whole = true;
   for (const Rows& r : {k, v})
     whole = whole && ((reinterpret_cast<uintptr_t>(r.data) | (unsigned long long)(r.t * (long long)sizeof(T)) |
                        (unsigned long long)(r.h * (long long)sizeof(T))) & 15u) == 0;
   if (read)
-    (whole ? read_rows<T, true> : read_rows<T, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each, lanes_log);
+    (whole ? read_rows<T, W, true> : read_rows<T, W, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each);
   else
-    (whole ? append_rows<T, true> : append_rows<T, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each, lanes_log);
+    (whole ? append_rows<T, W, true> : append_rows<T, W, false>)<<<grid, kThreads, 0, s>>>(c, b, k, v, each);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return tgcb_internal_fail(TGCB_E_CUDA, "kv_cache", cudaGetErrorString(e));
   return TGCB_OK;
+}
+
+template <typename T>
+int by_width(const Cache& c, const Batch& b, const Rows& k, const Rows& v, bool read, cudaStream_t s) {
+  switch (c.width) {
+    case 32: return run<T, 32>(c, b, k, v, read, s);
+    case 64: return run<T, 64>(c, b, k, v, read, s);
+    case 128: return run<T, 128>(c, b, k, v, read, s);
+    default: return run<T, 256>(c, b, k, v, read, s);
+  }
 }
 
 int entry(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, const tgcb_heads* keys, const tgcb_heads* values,
@@ -348,9 +372,9 @@ int entry(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, const tgc
   const Rows v = {static_cast<char*>(values->data), values->token_stride, values->head_stride};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case TGCB_F32: return run<float>(c, b, k, v, read, s);
-    case TGCB_BF16: return run<__nv_bfloat16>(c, b, k, v, read, s);
-    default: return run<__half>(c, b, k, v, read, s);
+    case TGCB_F32: return by_width<float>(c, b, k, v, read, s);
+    case TGCB_BF16: return by_width<__nv_bfloat16>(c, b, k, v, read, s);
+    default: return by_width<__half>(c, b, k, v, read, s);
   }
 }
 
