@@ -114,6 +114,21 @@ def test_rows_are_the_quantisers(cuda, dtype):
     assert torch.equal(read.isnan(), want.isnan()) and torch.equal(read.nan_to_num(), want.nan_to_num())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [32, 256])
+def test_rows_of_every_magnitude_are_the_quantisers(cuda, width, dtype):
+    """Maxima of 2^-140 to 2^127: scales subnormal, at the least normal number, large; halves of the maximum lie between two codes."""
+    g = torch.Generator().manual_seed(6)
+    rows = torch.rand(268 * 4, width, generator=g, dtype=torch.float64) * 2 - 1
+    rows[:, 1::4] = rows[:, :1] * torch.randint(-127, 128, (268 * 4, width // 4), generator=g) / 254
+    rows = (rows * 2.0 ** (torch.arange(268 * 4) // 4 - 140.0)[:, None]).float().to(dtype).cuda()
+    codes, scales = quantize.quantise_rows(rows)
+    cache = kv_cache.QuantisedCache(9, 1, width, page=128)
+    cache.append(rows[:, None], rows[:, None], torch.arange(9, dtype=torch.int32, device="cuda")[None], vector([0]))
+    for got, got_scales in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)):
+        assert torch.equal(got.reshape(-1, width)[:268 * 4], codes) and torch.equal(got_scales.reshape(-1)[:268 * 4], scales)
+
+
 @pytest.mark.parametrize("shift", [0, 1])
 def test_rows_of_any_stride(cuda, shift):
     base = torch.randn(5, 9, 64 + shift, device="cuda").to(torch.bfloat16)[:, :, shift:]
