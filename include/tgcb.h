@@ -363,7 +363,7 @@ int tgcb_cache_read(const tgcb_cache* cache, const tgcb_batch* batch, int dtype,
                     const tgcb_heads* values, void* stream);
 
 /* Attention of every token over its sequence's cached positions: query head h reads key head
- * h / (q_heads / kv_heads); score = scale * (q . k), with cap > 0 cap * tanh(score / cap); softmax over the
+ * h / (q_heads / kv_heads); score = scale * (q . k), with cap > 0 (at most 1e30) cap * tanh(score / cap); softmax over the
  * positions the token sees, times the values. Row i of sequence b sees positions 0 .. starts[b] + i;
  * with `visible` ([tokens] bit sets) it sees positions 0 .. starts[b] - 1 and, of the call's own rows,
  * starts[b] + j for each set bit j (rows past the 64th are seen by none). The rows' own keys must

@@ -634,7 +634,9 @@ int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int 
   if (b.tokens * q_heads > 0x7fffffffll) return bad("too many tokens");
   if (!std::isfinite(scale)) return bad("the scale must be finite");
   if (!(cap >= 0) || std::isinf(cap)) return bad("the cap must be finite and not negative");
-  // the largest factors that the kernels form of them, with room for their constants
+  // the largest factors that the kernels form of them, with room for their constants; a score over a cap of at most 1e30
+  // that is no normal float32 is off by less than 2^-20 of a unit as long as q . code is below 2^30
+  if (cap > 1.1e30f) return bad("a cap is at most 1e30: 0 for none");
   if (std::fabs(scale) > 1.1e30f || (cap > 0 && !(std::fabs(scale / cap) <= 1.1e30f))) return bad("the scale under the cap is beyond float32");
   if (b.tokens == 0) return TGCB_OK;
   const size_t need = scratch_bytes(c, b, q_heads);

@@ -51,13 +51,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-// float32 rows take CUDA's tanh (a few units in the last place). For 16-bit rows 1 - 2 / (1 + e^2x) is near enough: off
-// by 2^-22 of the cap, where a row's own rounding is 2^-9 or 2^-12 of its value, and a
-// third of the instructions.
+// float32 rows take CUDA's tanh (a few units in the last place). For 16-bit rows 1 - 2 / (1 + e^2x) is off by 2^-22, which
+// is 2^-19 of the tangent from |x| = 1/4 on; below that the series x - x^3/3 + 2x^5/15 - 17x^7/315, off by 2^-21 of it, so
+// that a cap far above the scores leaves them as they are (without the series caps from 10^6 on were wrong, and at 10^8 all
+// scores 0). One tree of 13 nodes with a cap: 37 us, 35 without the series.
 template <typename T>
 __device__ __forceinline__ float tanh_of(float x) {
   if constexpr (sizeof(T) == 4) return tanhf(x);
-  return 1.f - __fdividef(2.f, 1.f + exp2_fast(2.885390081777927f * x));
+  const float y = x * x, far = 1.f - __fdividef(2.f, 1.f + exp2_fast(2.885390081777927f * x));
+  const float near = x * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  return fabsf(x) < 0.25f ? near : far;
 }
 
 // Two floats as N pairs of bfloat16 whose sums they are: the leading 8 bits cut off N - 1 times (exact

@@ -99,7 +99,7 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
     and, among the call's own rows of its sequence, row j where bit j is set: a tree's ancestors
     and the token itself. At most 64 rows a sequence can be named so.
 
-    score = scale * q.k (``scale`` None: 1 / sqrt(width)), then with ``cap`` cap * tanh(score / cap).
+    score = scale * q.k (``scale`` None: 1 / sqrt(width)), then with ``cap`` (at most 1e30) cap * tanh(score / cap).
     A token that sees nothing gets zeros. ``out`` (not the queries) receives the result; rows of no sequence are not written.
     """
     if not isinstance(cache, kv_cache.QuantisedCache):
@@ -120,7 +120,7 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
     cap = 0.0 if cap is None else float(cap)
     if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
         raise ConfigError(f"the scale has to be finite and the cap finite and not negative, got {scale} and {cap}")
-    if max(abs(scale), abs(scale) / cap if cap else 0.0) > 1e30:
+    if max(abs(scale), abs(scale) / cap if cap else 0.0, cap) > 1e30:
         raise ConfigError(f"a scale of {scale} under a cap of {cap} is beyond float32")
     if out is not None:
         heads.check_rows("out", out, queries)

@@ -97,3 +97,11 @@ def test_host_tensors_are_refused():
         kv_cache.QuantisedCache(4, 2, 64, device="cpu")
     with pytest.raises(ConfigError):
         attention.cached_attention(rows, None, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("cap", [1e31, 3e38])
+def test_attention_refuses_caps_beyond_float32(cap):
+    lib, rows = _lib.load(), _lib.Heads(HERE, 256, 64)
+    assert lib.tgcb_cached_attention(cache_desc(), batch_desc(), 0, 4, rows, None, 1.0, cap, rows, HERE, 1 << 40, None) == _lib.TGCB_E_INVALID
+    with pytest.raises(Exception, match="cap is at most"):
+        _lib.check(_lib.TGCB_E_INVALID, "cached_attention")

@@ -393,3 +393,35 @@ def test_refusals(cuda):
     many = torch.randn(130, 4, 64, device="cuda")
     with pytest.raises(ConfigError, match="64"):
         attention.cached_attention(many, cache, table, s, visible=torch.zeros(130, dtype=torch.int64, device="cuda"))
+
+
+def check_relative(got, q, cache, table, starts, offsets, visible=None, scale=None, cap=0.0):
+    """As `check`, without an error that is a fixed part of the cap or of the values' type: a capped score is off by
+    2^-19 of itself (1 - 2 / (1 + e^2x) from |x| = 1/4 on: its quotient, at most 0.76, by 1.8 * 2^-22 of itself, and the
+    tangent is 0.24 there; below, the series by 2^-21 and its roundings)."""
+    scale = q.shape[2]**-0.5 if scale is None else scale
+    want, size, scores = generation.attention(q, cache.keys, cache.key_scales, cache.values, cache.value_scales, table, starts, offsets,
+                                              visible, scale, cap)
+    mine, eps = ~want.isnan().all(-1), torch.finfo(q.dtype).eps
+    delta = ((q.shape[2] + 8) * 2.0**-23 + 2.0**-19 * (cap > 0)) * scores
+    part = 2 * delta + ((int(starts.max()) + q.shape[0]) / 16 + 64) * 2.0**-24
+    tol = part * size if q.dtype == torch.float32 else (part + 2.0**-16) * size + eps / 2 * (want.abs() + part * size)
+    ratio = ((got.cpu().double() - want).abs() / (tol + torch.finfo(q.dtype).tiny * eps))[mine]
+    assert bool(got.cpu()[mine].isfinite().all())
+    assert float(ratio.max()) <= 1, f"off by {float(ratio.max())} tolerances"
+
+
+@pytest.mark.parametrize("cap", [100.0, 1e4, 1e6, 1e8, 1e30])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE)])
+def test_large_caps(cuda, q_heads, room, dtype, cap):
+    """A cap far above the scores changes next to nothing."""
+    q, cache, table, s, o = make([100, 700], [1, 5], q_heads, 2, 64, 32, dtype, seed=2, room=room)
+    check_relative(attention.cached_attention(q, cache, table, s, o, scale=0.5, cap=cap), q, cache, table, s, o, scale=0.5, cap=cap)
+
+
+@pytest.mark.parametrize("cap", [1e31, 3e38])
+def test_caps_beyond_float32_are_refused(cuda, cap):
+    q, cache, table, s, o = make([100, 700], [1, 5], 4, 2, 64, 32, torch.float32)
+    with pytest.raises(ConfigError, match="beyond float32"):
+        attention.cached_attention(q, cache, table, s, o, cap=cap)
