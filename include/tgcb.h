@@ -367,7 +367,9 @@ int tgcb_cache_read(const tgcb_cache* cache, const tgcb_batch* batch, int dtype,
  * positions the token sees, times the values. Row i of sequence b sees positions 0 .. starts[b] + i;
  * with `visible` ([tokens] bit sets) it sees positions 0 .. starts[b] - 1 and, of the call's own rows,
  * starts[b] + j for each set bit j (rows past the 64th are seen by none). The rows' own keys must
- * have been appended before. A token that sees nothing gets zeros. Scratch as
+ * have been appended before. A token that sees nothing gets zeros. Weighted values are added up in float32 before they are
+ * divided: scales from 2^-110 to 2^121 are held, and beside a scale above 2^80 that a token sees, scales from 2^-75 on;
+ * weights below 2^-86 of the largest may count as 0. Scratch as
  * tgcb_cached_attention_scratch_bytes says, 16-byte aligned, not shared by calls that may overlap. */
 size_t tgcb_cached_attention_scratch_bytes(const tgcb_cache* cache, const tgcb_batch* batch, int q_heads);
 int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, int q_heads,

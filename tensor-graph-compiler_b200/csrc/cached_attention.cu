@@ -360,13 +360,30 @@ __global__ void __launch_bounds__(kThreads, RN == 1 && W <= 128 ? 3 : 2) attend(
       } else {
         seen_rows = ~0u;
       }
-      float keep[RN][2], base[RN][2];
+      float keep[RN][2], base[RN][2], top[RN][2];
       bool moved = false;
 #pragma unroll
       for (int rn = 0; rn < RN; ++rn)
 #pragma unroll
+        for (int j = 0; j < 2; ++j) top[rn][j] = fmaxf(fmaxf(sc[0][rn][j], sc[0][rn][2 + j]), fmaxf(sc[1][rn][j], sc[1][rn][2 + j]));
+      const float largest = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+      if (__any_sync(0xffffffffu, largest > kLargeScale * kCodeScale)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (fabsf(vs[h][k]) > kLargeScale * kCodeScale) {
+#pragma unroll
+              for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) top[rn][j] = fmaxf(top[rn][j], sc[h][rn][2 * k + j] + kLargeMargin);
+            }
+      }
+#pragma unroll
+      for (int rn = 0; rn < RN; ++rn)
+#pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float t = fmaxf(fmaxf(sc[0][rn][j], sc[0][rn][2 + j]), fmaxf(sc[1][rn][j], sc[1][rn][2 + j]));
+          float t = top[rn][j];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
           const float mn = fmaxf(m[rn][j], t);

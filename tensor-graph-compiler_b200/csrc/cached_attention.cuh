@@ -63,6 +63,12 @@ __device__ __forceinline__ float tanh_of(float x) {
   return fabsf(x) < 0.25f ? near : far;
 }
 
+// Weighted values are added up before they are divided by the weights' sum, and up to 2^30 of them with values above 2^87 (a
+// scale above 2^80) could leave float32's range. Such a key's weight is kept 2^kLargeMargin below one: its row's
+// reference, against which weights and their sum are taken, is at least the key's score plus the margin, in units of
+// log2 e. Other weights need none: 2^30 keys, 2^8 for a reference that may lag behind (cached_attention_tc.cu), 2^87.
+constexpr float kLargeScale = 0x1p80f, kLargeMargin = 40.f;
+
 // Two floats as N pairs of bfloat16 whose sums they are: the leading 8 bits cut off N - 1 times (exact
 // remainders), the rest rounded.
 template <int N>

@@ -62,7 +62,8 @@ struct Memory {
 
 struct Shared {
   unsigned long long q_full, q_free, k_full[2], scaled[2][2], v_full[2], s_full[2], p_ready[2], pv_done[2], rows_full, x_full, x_free, drained;
-  unsigned tmem, valid[2][2];  // valid: a bit for each 16 keys of a tile whose page is there
+  unsigned tmem, valid[2][2];  // of 32 keys of a tile a byte: a bit for each 16 whose page is there, and bit 2 where `large` has a bit
+  unsigned large[2][2][4];     // a bit for each key of a tile whose value's scale is above kLargeScale
   int abort;
 };
 
@@ -358,7 +359,11 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
           scales[tid] = ks * factor;
           scales[tid + (M::VALUE_SCALES - M::KEY_SCALES) / 4] = vs * kCodeScale;
           const unsigned there = __ballot_sync(0xffffffffu, held);
-          if ((tid & 31) == 0) reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1);
+          const unsigned large = __ballot_sync(0xffffffffu, fabsf(vs) > kLargeScale);
+          if ((tid & 31) == 0) {
+            reinterpret_cast<unsigned char*>(&sh->valid[g][turn & 1])[tid / 32] = (unsigned char)((there & 1) | (there >> 16 & 1) << 1 | (large ? 4 : 0));
+            sh->large[g][turn & 1][tid / 32] = large;
+          }
         }
         fence_async();
         arrive(VALUES ? &sh->v_full[g] : &sh->k_full[g]);
@@ -461,6 +466,26 @@ __device__ __forceinline__ float top_of(unsigned scores, const float* ks, Seen s
   return fmaxf(top[0], top[1]);
 }
 
+// The same of capped scores, with the margin for the keys of `large`. Rare: short rather than fast.
+template <typename T, class Seen>
+__device__ __forceinline__ float top_of_large(unsigned scores, const float* ks, const unsigned* large, float cap2, Seen seen_of) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int ch = 0; ch < 8; ++ch) {
+    unsigned r[16];
+    load16(scores + 16 * ch, r);
+    const unsigned see = seen_of(ch / 2) >> (16 * (ch & 1)), more = large[ch / 2] >> (16 * (ch & 1));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float x = __uint_as_float(r[j]) * ks[16 * ch + j];
+      if (cap2 > 0) x = cap2 * tanh_of<T>(x);
+      if ((more >> j) & 1) x += kLargeMargin;
+      if ((see >> j) & 1) top = fmaxf(top, x);
+    }
+  }
+  return top;
+}
+
 // Writes a row's 128 weights times the values' scales over its scores, 16 at a time as 8 columns of leading and 8 of
 // remaining parts, and returns the weights' sum.
 template <typename T, bool CAP, bool MASKED, class Seen>
@@ -542,14 +567,15 @@ __device__ __forceinline__ void weigh(const Cache& c, const Batch& b, const Args
         return s & ((halves & 1 ? 0xffffu : 0u) | (halves & 2 ? 0xffff0000u : 0u));
       };
       float top = -INFINITY;
+      const bool margin = word & 0x04040404u;
       if (inside) {
         top = top_of<false>(scores, ks, seen_of);
         seen = true;
       } else {
-        top = top_of<true>(scores, ks, seen_of);
+        top = margin ? top_of_large<T>(scores, ks, sh->large[g][turn & 1], cap2, seen_of) : top_of<true>(scores, ks, seen_of);
         seen = seen || seen_of(0) || seen_of(1) || seen_of(2) || seen_of(3);
       }
-      if (a.cap > 0) top = top == -INFINITY ? top : cap2 * tanh_of<T>(top);
+      if (a.cap > 0 && !margin) top = top == -INFINITY ? top : cap2 * tanh_of<T>(top);
       const bool grown = top > m + kGrowth || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grown)) {
         const float keep = grown ? exp2_fast(m - top) : 1.f;

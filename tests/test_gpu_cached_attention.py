@@ -425,3 +425,47 @@ def test_caps_beyond_float32_are_refused(cuda, cap):
     q, cache, table, s, o = make([100, 700], [1, 5], 4, 2, 64, 32, torch.float32)
     with pytest.raises(ConfigError, match="beyond float32"):
         attention.cached_attention(q, cache, table, s, o, cap=cap)
+
+
+@pytest.mark.parametrize("power", [-100, 60, 90, 115, 125])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE), (128, WIDE)])
+def test_values_of_every_magnitude(cuda, q_heads, room, dtype, power):
+    q, cache, table, s, o = make([300, 1900], [1, 5], q_heads, 2, 64, 32, dtype, seed=3, room=room)
+    cache.value_scales *= 2.0**power  # values up to 4.8 times that
+    check_relative(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+    check_relative(attention.cached_attention(q, cache, table, s, o, cap=10.0), q, cache, table, s, o, cap=10.0)
+    q.zero_()  # all weights one, all values of one sign: the largest sums
+    cache.values.clamp_(min=-127).abs_()
+    check_relative(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE), (128, WIDE)])
+@pytest.mark.parametrize("place", [0, 40, 200, 1001, 1004])
+def test_one_value_far_above_the_others(cuda, place, q_heads, room, dtype):
+    """Rows that see it, and rows that do not, whose own values are too small to be held beside it."""
+    q, cache, table, s, o = make([1000], [6], q_heads, 1, 64, 32, dtype, seed=4, room=room)
+    cache.value_scales *= 2.0**-90
+    at = table[0, place // 32], 0, place % 32
+    cache.value_scales[at] *= 2.0**105
+    cache.value_scales[at] *= 2.0**105
+    cache.values[at] += cache.values[at] == 0  # it has a part in every column
+    check_relative(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+    bits = tree_bits([6])
+    check_relative(attention.cached_attention(q, cache, table, s, o, visible=bits, cap=10.0), q, cache, table, s, o, bits, cap=10.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (64, WIDE), (128, WIDE)])
+@pytest.mark.parametrize("bits", [30, 95])
+def test_a_large_value_of_little_weight(cuda, bits, q_heads, room, dtype):
+    """2^120 at a weight 2^-30 or 2^-95 of the largest: it is most of the answer, and not all its weight may be taken from it."""
+    q, cache, table, s, o = make([500], [3], q_heads, 1, 64, 32, dtype, seed=5, room=room)
+    cache.keys.zero_()
+    cache.keys[table[0, 7], 0, 9] = 64
+    cache.key_scales.fill_(2.0**-6)
+    cache.value_scales[table[0, 7], 0, 9] *= 2.0**120
+    q.fill_(-1)  # 64 products of -1 with 1: a score of -64 scale, the others' 0
+    scale = bits * 0.6931471805599453 / 64
+    check_relative(attention.cached_attention(q, cache, table, s, o, scale=scale), q, cache, table, s, o, scale=scale)
