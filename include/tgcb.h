@@ -324,7 +324,7 @@ int tgcb_norm_rotate_backward(const tgcb_rotary_desc* d, void* stream);
 /* A paged cache: row (page p, head h, place r) of keys and of values is `width` int8 codes at
  * ((p * kv_heads + h) * page + r) * width and one float32 scale at (p * kv_heads + h) * page + r; the
  * row stands for code * scale. Codes are 16-byte aligned. `faults` counts rows that a call refused on the
- * device (see tgcb_batch). */
+ * device (see tgcb_batch) and is never reset by one. */
 typedef struct tgcb_cache {
   int8_t* keys;
   int8_t* values;

@@ -83,7 +83,8 @@ class QuantisedCache:
         self.keys, self.key_scales, self.values, self.value_scales = keys, key_scales, values, value_scales
         self.pages, self.kv_heads, self.page, self.width = pages, kv_heads, page, width
         self.device, self.index = keys.device, keys.get_device()
-        self.faults = torch.zeros(1, dtype=torch.int32, device=keys.device)
+        self.faults = torch.tensor([0], dtype=torch.int32, device=keys.device)  # there when this returns, for calls on any stream
+        self._reported = 0
         self.desc = _lib.CacheDesc(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
                                    self.faults.data_ptr(), pages, kv_heads, page, width)
 
@@ -151,8 +152,10 @@ class QuantisedCache:
         return keys, values
 
     def check(self) -> None:
-        """Synchronise and raise ``ConfigError`` if a call named positions or pages that are not there."""
-        count = int(self.faults.item())
+        """Synchronise the device and raise ``ConfigError`` if a call on any of its streams named positions or pages that are not
+        there, since this was last called."""
+        torch.cuda.synchronize(self.device)
+        counted = int(self.faults.item())
+        count, self._reported = (counted - self._reported) % (1 << 32), counted  # the device only ever adds to it
         if count:
-            self.faults.zero_()
             raise ConfigError(f"{count} accesses named a position outside the page table or a page outside the cache")

@@ -89,6 +89,32 @@ def test_attention_refuses(q_heads, scale, cap):
     assert rc == _lib.TGCB_E_INVALID
 
 
+class Faults:
+    """A counter of a device that goes on counting: one more after every read."""
+
+    def __init__(self):
+        self.value = 1
+
+    def item(self):
+        self.value += 1
+        return self.value - 1
+
+    def zero_(self):
+        self.value = 0
+
+
+def test_check_loses_no_count(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *_: None)
+    cache = kv_cache.QuantisedCache.__new__(kv_cache.QuantisedCache)
+    cache.faults, cache.device, cache.index, cache._reported = Faults(), torch.device("cuda:0"), 0, 0
+    for _ in range(3):
+        with pytest.raises(ConfigError, match="^1 accesses"):
+            cache.check()
+    cache.faults.value, cache._reported = -(1 << 31) + 5, (1 << 31) - 5  # the int32 has wrapped around
+    with pytest.raises(ConfigError, match="^10 accesses"):
+        cache.check()
+
+
 def test_host_tensors_are_refused():
     rows, gain = torch.randn(2, 2, 64), torch.ones(64)
     with pytest.raises(ConfigError):

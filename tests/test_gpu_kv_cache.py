@@ -235,3 +235,31 @@ def test_refusals(cuda):
         kv_cache.QuantisedCache.of(cache.keys, cache.key_scales, cache.values.float(), cache.value_scales)
     with pytest.raises(ConfigError):
         kv_cache.QuantisedCache.of(cache.keys, cache.key_scales[:2], cache.values, cache.value_scales)
+
+
+def test_check_waits_for_every_stream(cuda):
+    cache, _ = filled(4, 1, 16, 32)
+    rows, bad, starts, side = torch.randn(2, 1, 32, device="cuda"), vector([[7]]), vector([0]), torch.cuda.Stream()
+    cache.append(rows, rows, vector([[1]]), starts)  # its kernel is loaded before the streams differ
+    cache.check()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+    cache.append(rows, rows, bad, starts, stream=side)
+    with pytest.raises(ConfigError, match="2 accesses"):
+        cache.check()
+    cache.append(rows[:1], rows[:1], bad, starts)
+    with pytest.raises(ConfigError, match="1 accesses"):
+        cache.check()
+    cache.check()
+
+
+def test_a_new_cache_counts_on_every_stream(cuda):
+    parts = filled(4, 1, 16, 32)[1]
+    rows, bad, starts, side = torch.randn(2, 1, 32, device="cuda"), vector([[7]]), vector([0]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    cache = kv_cache.QuantisedCache.of(*parts)
+    cache.append(rows, rows, bad, starts, stream=side)
+    with pytest.raises(ConfigError, match="2 accesses"):
+        cache.check()
