@@ -369,7 +369,8 @@ int tgcb_cache_read(const tgcb_cache* cache, const tgcb_batch* batch, int dtype,
  * starts[b] + j for each set bit j (rows past the 64th are seen by none). The rows' own keys must
  * have been appended before. A token that sees nothing gets zeros. Weighted values are added up in float32 before they are
  * divided: scales from 2^-110 to 2^121 are held, and beside a scale above 2^80 that a token sees, scales from 2^-75 on;
- * weights below 2^-86 of the largest may count as 0. Scratch as
+ * weights below 2^-86 of the largest may count as 0. Waits inside a kernel are bounded (4 s): one that gives up records
+ * status 6 in the device status word (tgcb_status) and leaves `out` unfinished. Scratch as
  * tgcb_cached_attention_scratch_bytes says, 16-byte aligned, not shared by calls that may overlap. */
 size_t tgcb_cached_attention_scratch_bytes(const tgcb_cache* cache, const tgcb_batch* batch, int q_heads);
 int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int dtype, int q_heads,

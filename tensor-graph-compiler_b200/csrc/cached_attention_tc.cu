@@ -21,7 +21,7 @@
 // second in two parts, take 1.1). Loops are kept short for that reason. Measured: 2 x 509 tokens of 16 heads on 4 behind 4000
 // positions 122 us, 290 TFLOP/s; 32 trees of 1 to 31 nodes, 32 heads on 8, over 2000 to 8000 positions 255 to 268
 // us (calls in a row).
-// All waits are bounded (4 s); a CTA that gives up records status 2 and unwinds.
+// All waits are bounded (4 s); a CTA that gives up records status 6 and unwinds.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -45,7 +45,7 @@ static_assert(2 * kSoftmaxRegisters + 2 * kConverterRegisters + kProductRegister
 static_assert(kSoftmaxRegisters >= kLaunchRegisters && kConverterRegisters <= kLaunchRegisters && kProductRegisters <= kLaunchRegisters,
               "more_registers only goes up, fewer_registers only down");
 constexpr int kLeastTiles = 2;                           // one for each group
-constexpr int kStatusTimeout = 2;
+constexpr int kStatusTimeout = 6;                        // device status code (the kernels' TGCB_STATUS_* family)
 constexpr float kGrowth = 8.f;                           // of a maximum, in powers of two, before anything is rescaled
 
 template <int W>

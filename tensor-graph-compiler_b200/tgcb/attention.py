@@ -101,6 +101,7 @@ def cached_attention(queries: torch.Tensor, cache: kv_cache.QuantisedCache, tabl
 
     score = scale * q.k (``scale`` None: 1 / sqrt(width)), then with ``cap`` (at most 1e30) cap * tanh(score / cap).
     A token that sees nothing gets zeros. ``out`` (not the queries) receives the result; rows of no sequence are not written.
+    A kernel that waits in vain for 4 s gives up, with ``out`` unfinished; ``cache.check`` raises for it.
     """
     if not isinstance(cache, kv_cache.QuantisedCache):
         raise ConfigError("cached_attention reads a QuantisedCache")

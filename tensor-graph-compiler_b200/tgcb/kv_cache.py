@@ -10,15 +10,17 @@ every sequence has tokens / batch of them), ``starts`` [batch] how many position
 is position ``starts[b] + i``. All three are int32 on the device and are read when the kernels run: a
 captured call can be replayed with other lengths. Rows of no sequence are left as they
 were. Positions that the table does not hold and pages outside the cache are never accessed; they are
-counted, and ``check`` raises for them.
+counted, and ``check`` raises for them, as for a kernel that gave up waiting.
 """
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from tgcb import _lib, heads
-from tgcb.errors import ConfigError
+from tgcb.errors import ConfigError, DeviceError
 
 PAGES = (16, 32, 64, 128)
 WIDTHS = (32, 64, 128, 256)
@@ -153,8 +155,12 @@ class QuantisedCache:
 
     def check(self) -> None:
         """Synchronise the device and raise ``ConfigError`` if a call on any of its streams named positions or pages that are not
-        there, since this was last called."""
-        torch.cuda.synchronize(self.device)
+        there, since this was last called; ``DeviceError`` if a kernel gave up waiting, which leaves its call's output unfinished."""
+        status = ctypes.c_int(0)
+        with heads.on_device(self.index):
+            _lib.check(_lib.load().tgcb_status(1, ctypes.byref(status)), "reading the device status")  # synchronises the device
+        if status.value:
+            raise DeviceError(f"a kernel on {self.device} reported device status {status.value}: an output is not finished")
         counted = int(self.faults.item())
         count, self._reported = (counted - self._reported) % (1 << 32), counted  # the device only ever adds to it
         if count:

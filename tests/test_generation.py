@@ -2,13 +2,14 @@
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
 import torch
 
-from tgcb import _lib, attention, kv_cache, rotary
-from tgcb.errors import ConfigError
+from tgcb import _lib, attention, heads, kv_cache, rotary
+from tgcb.errors import ConfigError, DeviceError
 
 memory = (ctypes.c_char * 4096)()  # never read: every call here is refused for its arguments
 HERE = (ctypes.addressof(memory) + 255) & ~255
@@ -103,10 +104,40 @@ class Faults:
         self.value = 0
 
 
-def test_check_loses_no_count(monkeypatch):
+class Device:
+    """The library's status word, read and cleared as on a device."""
+
+    def __init__(self, status=0):
+        self.status = status
+
+    def tgcb_status(self, clear, to):
+        to._obj.value = self.status
+        if clear:
+            self.status = 0
+        return _lib.TGCB_OK
+
+
+def counting_cache(monkeypatch, device):
     monkeypatch.setattr(torch.cuda, "synchronize", lambda *_: None)
+    monkeypatch.setattr(heads, "on_device", lambda _: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "load", lambda: device)
     cache = kv_cache.QuantisedCache.__new__(kv_cache.QuantisedCache)
     cache.faults, cache.device, cache.index, cache._reported = Faults(), torch.device("cuda:0"), 0, 0
+    return cache
+
+
+def test_check_reports_a_kernel_that_gave_up(monkeypatch):
+    device = Device(6)
+    cache = counting_cache(monkeypatch, device)
+    with pytest.raises(DeviceError, match="status 6"):
+        cache.check()
+    with pytest.raises(ConfigError, match="^1 accesses"):  # not lost beside it
+        cache.check()
+    assert device.status == 0
+
+
+def test_check_loses_no_count(monkeypatch):
+    cache = counting_cache(monkeypatch, Device())
     for _ in range(3):
         with pytest.raises(ConfigError, match="^1 accesses"):
             cache.check()
