@@ -52,18 +52,28 @@ def _reach(t: torch.Tensor) -> tuple[int, int]:
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors of rows may share memory. Slices of the same wider rows, side by side, do not."""
+    """Whether two tensors of rows may share memory. Slices of the same wider rows, side by side, do not, nor do parts of each head."""
     if a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = _reach(a), _reach(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    for dim in (0, 1):  # both repeat with one stride, within which each has its own part
+    if a.dtype != b.dtype:
+        return True
+    # Where both repeat with one stride, within which one step of each has its place, only equal steps can meet: on to one step of
+    # both, from the larger of the two strides to the smaller.
+    for dim in sorted((0, 1), key=a.stride, reverse=True):
+        if a.shape[dim] == b.shape[dim] == 1:
+            continue
+        if min(a.shape[dim], b.shape[dim]) == 1 or a.stride(dim) != b.stride(dim):
+            return True
         step = a.stride(dim) * a.element_size()
-        if a.dtype == b.dtype and a.shape[dim] == b.shape[dim] and a.stride(dim) == b.stride(dim):
-            a_end, b_end = _reach(a.narrow(dim, 0, 1))[1], _reach(b.narrow(dim, 0, 1))[1]
-            if max(a_end, b_end) - min(a0, b0) <= step:
-                return not (a_end <= b0 or b_end <= a0)
+        a, b = a.narrow(dim, 0, 1), b.narrow(dim, 0, 1)
+        a1, b1 = _reach(a)[1], _reach(b)[1]
+        if max(a1, b1) - min(a0, b0) > step:
+            return True
+        if a1 <= b0 or b1 <= a0:
+            return False
     return True
 
 

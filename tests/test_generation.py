@@ -146,6 +146,36 @@ def test_check_loses_no_count(monkeypatch):
         cache.check()
 
 
+def test_parts_of_the_same_rows_are_apart():
+    halves, both = torch.zeros(5, 3, 128), torch.zeros(5, 3, 2, 64)
+    side_by_side, by_head = torch.zeros(5, 7, 64), torch.zeros(3, 5, 2, 64).transpose(0, 1)
+    for a, b in ((halves[..., :64], halves[..., 64:]), both.unbind(2), (side_by_side[:, :3], side_by_side[:, 3:6]), by_head.unbind(2),
+                 (side_by_side[:, :2], side_by_side[:, 2:]), (side_by_side[:, ::2], side_by_side[:, 1::2][:, :3]), (side_by_side[:2], side_by_side[2:])):
+        assert not heads.overlap(a, b) and not heads.overlap(b, a)
+    for a, b in ((halves[..., :65], halves[..., 64:]), (side_by_side[:, :4], side_by_side[:, 3:]), (by_head[:, :, 0], by_head[:, :, 0]),
+                 (side_by_side[:3], side_by_side[2:]), (halves, halves[1:2])):
+        assert heads.overlap(a, b) and heads.overlap(b, a)
+
+
+def test_rows_that_share_memory_are_never_taken_as_apart():
+    g = torch.Generator().manual_seed(0)
+    number = lambda low, high: int(torch.randint(low, high, (1,), generator=g))  # noqa: E731
+    memory, apart, shared = torch.arange(400), 0, 0
+    for _ in range(3000):
+        strides = number(0, 30), number(0, 30)
+        shape = number(1, 4), number(1, 4), number(1, 9)
+        a = memory.as_strided(shape, (*strides, 1), number(0, 60))
+        if number(0, 2):
+            shape = number(1, 4), number(1, 4), number(1, 9)
+        if not number(0, 3):
+            strides = number(0, 30), number(0, 30)
+        b = memory.as_strided(shape, (*strides, 1), number(0, 60))
+        meet = not set(a.reshape(-1).tolist()).isdisjoint(b.reshape(-1).tolist())
+        assert heads.overlap(a, b) or not meet
+        apart, shared = apart + (not heads.overlap(a, b)), shared + meet
+    assert apart > 500 and shared > 500
+
+
 def test_host_tensors_are_refused():
     rows, gain = torch.randn(2, 2, 64), torch.ones(64)
     with pytest.raises(ConfigError):

@@ -263,3 +263,14 @@ def test_a_new_cache_counts_on_every_stream(cuda):
     cache.append(rows, rows, bad, starts, stream=side)
     with pytest.raises(ConfigError, match="2 accesses"):
         cache.check()
+
+
+def test_read_into_parts_of_the_same_rows(cuda):
+    cache, _ = filled(4, 2, 16, 64)
+    rows, table, starts = torch.randn(5, 2, 64, device="cuda"), vector([[2]]), vector([1])
+    cache.append(rows, -rows, table, starts)
+    want = cache.read(5, table, starts)
+    for out in (torch.zeros(5, 2, 2, 64, device="cuda").unbind(2), torch.zeros(5, 2, 128, device="cuda").split(64, -1),
+                torch.zeros(2, 5, 2, 64, device="cuda").transpose(0, 1).unbind(2)):
+        cache.read_into(*out, table, starts)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])

@@ -219,3 +219,14 @@ def test_refusals(cuda):
     with pytest.raises(ConfigError):
         rotary.frequencies(7)
     assert heads.overlap(out, out[1:]) and not heads.overlap(q, k)
+
+
+def test_outputs_that_are_parts_of_the_same_heads(cuda):
+    rows = torch.randn(5, 3, 2, 64, device="cuda")
+    gain, positions, freqs = torch.ones(64, device="cuda"), torch.arange(5, device="cuda"), rotary.frequencies(64)
+    want = rotary.norm_rotate(rows[:, :, 0], rows[:, :, 1], gain, gain, positions, freqs)
+    out = torch.zeros_like(rows)
+    rotary.norm_rotate_into(rows[:, :, 0], rows[:, :, 1], gain, gain, positions, freqs, out[:, :, 0], out[:, :, 1])
+    assert torch.equal(out[:, :, 0], want[0]) and torch.equal(out[:, :, 1], want[1])
+    rotary.norm_rotate_into(rows[:, :, 0], rows[:, :, 1], gain, gain, positions, freqs, rows[:, :, 0], rows[:, :, 1])
+    assert torch.equal(rows, out)
