@@ -95,10 +95,19 @@ def rows(t: torch.Tensor) -> tuple[int, int, int]:
     return t.data_ptr(), token, head
 
 
+@contextlib.contextmanager
+def _elsewhere(index: int):
+    with torch.cuda.device(index):  # setting a device up leaves it current
+        _lib.ensure_device(index)
+        yield
+
+
 def on_device(index: int):
-    """A context in which CUDA device ``index`` is current, and set up."""
+    """A context in which CUDA device ``index`` is current, and set up. Afterwards the one that was is current again."""
+    if torch._C._cuda_getDevice() != index:
+        return _elsewhere(index)
     _lib.ensure_device(index)
-    return _here if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+    return _here
 
 
 def on_stream(index: int, stream):

@@ -176,6 +176,30 @@ def test_rows_that_share_memory_are_never_taken_as_apart():
     assert apart > 500 and shared > 500
 
 
+@pytest.mark.parametrize("index", [0, 1])
+def test_a_call_on_another_device_leaves_the_current_one(monkeypatch, index):
+    current, set_up = [0], []
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    def ensure(i):  # as tgcb_init: the first call on a device selects it
+        if i not in set_up:
+            set_up.append(i)
+            current[0] = i
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_lib, "ensure_device", ensure)
+    for _ in range(2):
+        with heads.on_device(index):
+            assert current[0] == index and set_up == [index]
+        assert current[0] == 0
+
+
 def test_host_tensors_are_refused():
     rows, gain = torch.randn(2, 2, 64), torch.ones(64)
     with pytest.raises(ConfigError):
