@@ -159,17 +159,39 @@ int tgcb_device_count(void) {
   return n;
 }
 
+// The status word's first value, on a stream of its own: the default stream may not be used while another, blocking one
+// is captured.
+static int clear_status(int* status) {
+  cudaStream_t s = nullptr;
+  CUDA_TRY(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking));
+  cudaError_t e = cudaMemsetAsync(status, 0, 256, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  cudaStreamDestroy(s);
+  CUDA_TRY(e);
+  return TGCB_OK;
+}
+
+// While it lives this thread may allocate and wait although a stream is being captured: setting a device up puts nothing
+// into the graph, and the first call on a device may be a captured one.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 int tgcb_init(int device) {
   std::lock_guard<std::mutex> lock(g_mutex);
   if (device < 0 || device >= kMaxDevices) return fail(TGCB_E_INVALID, "device %d out of range", device);
   CUDA_TRY(cudaSetDevice(device));
+  const RelaxedCapture relaxed;
   DeviceState& st = g_devices[device];
   // the allocation-free sum's scratch address, looked up here so its calls need no look-up
   int rc = tgcb_internal_noalloc_setup(device);
   if (rc != TGCB_OK) return rc;
   if (st.ready) return TGCB_OK;
   if (st.status == nullptr) CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&st.status), 256));  // kept if a later step fails
-  CUDA_TRY(cudaMemset(st.status, 0, 256));
+  rc = clear_status(st.status);
+  if (rc != TGCB_OK) return rc;
   void* fn = nullptr;
   cudaDriverEntryPointQueryResult q;
   CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));

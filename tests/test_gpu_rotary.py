@@ -10,6 +10,8 @@ rows' type: half of its eps of the value, and for float16 half its smallest subn
 
 from __future__ import annotations
 
+import os
+
 import pytest
 import torch
 from oracle import generation
@@ -230,3 +232,36 @@ def test_outputs_that_are_parts_of_the_same_heads(cuda):
     assert torch.equal(out[:, :, 0], want[0]) and torch.equal(out[:, :, 1], want[1])
     rotary.norm_rotate_into(rows[:, :, 0], rows[:, :, 1], gain, gain, positions, freqs, rows[:, :, 0], rows[:, :, 1])
     assert torch.equal(rows, out)
+
+
+FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tgcb import attention, kv_cache, rotary
+
+rows, gain, freqs = torch.randn(4, 3, 64, device="cuda"), torch.ones(64, device="cuda"), rotary.frequencies(64)
+positions, table, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1, 2, 3], [[2, 1]], [3]))
+cache = kv_cache.QuantisedCache(4, 1, 64, page=16)
+
+def step():
+    q, k = rotary.norm_rotate(rows[:, :2], rows[:, 2:], gain, gain, positions, freqs)
+    cache.append(k, rows[:, 2:], table, starts)
+    return attention.cached_attention(q, cache, table, starts)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+cache.check()
+assert bool(got.isfinite().all()) and torch.equal(got, step())
+"""
+
+
+def test_a_process_whose_first_call_is_captured(cuda):
+    import subprocess
+    import sys
+
+    package = os.path.dirname(os.path.dirname(heads.__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST, package], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
