@@ -665,7 +665,7 @@ int tgcb_cached_attention(const tgcb_cache* cache, const tgcb_batch* batch, int 
   a.visible = reinterpret_cast<const long long*>(visible);
   a.cuts = static_cast<int4*>(scratch);
   a.parts = need ? reinterpret_cast<float*>(static_cast<char*>(scratch) + cuts_bytes()) : nullptr;
-  a.q_heads = q_heads, a.group = q_heads / c.heads, a.scale = scale, a.cap = cap;
+  a.group = q_heads / c.heads, a.scale = scale, a.cap = cap;
   a.capacity = b.max_pages * c.page, a.whole = need == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype != TGCB_F32 && for_tensor(c, b, a.group)) return attend_tensor(c, b, a, dtype, s);

@@ -25,7 +25,7 @@ struct Args {
   const long long* visible;
   float* parts;   // [2 * CTAs][ROWS * (W + 2)]: weighted sums, then each row's maximum and sum of weights
   int4* cuts;     // [CTAs]: sequence (-1: none), head, row tile and last CTA of the unit that is cut at this CTA's end
-  int q_heads, group;
+  int group;      // query heads that share a key head
   float scale, cap;
   int capacity;   // positions a table row holds
   int whole;      // units are not cut

@@ -37,14 +37,6 @@ struct Vec {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_vec(const T* p, float* out) {
-  Vec<T> v;
-  v.raw = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-  for (int i = 0; i < Vec<T>::N; ++i) out[i] = to_float(v.e[i]);
-}
-
-template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float* in) {
   Vec<T> v;
 #pragma unroll
