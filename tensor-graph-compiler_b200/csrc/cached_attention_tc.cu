@@ -264,7 +264,7 @@ __device__ __forceinline__ void convert(const Cache& c, const Batch& b, const Ar
       auto pages_of = [&](int tile) {
         const int lane = tid & 31, position = (walk.from + tile) * kKeys + 16 * lane;
         if (lane >= kKeys / 16 || tile >= walk.tiles || position >= q.end) return kUnread;
-        return __ldg(b.table + walk.s * b.table_stride + (position >> c.page_bits));
+        return max(__ldg(b.table + walk.s * b.table_stride + (position >> c.page_bits)), -1);  // no entry is kUnread
       };
       auto rows_of = [&](int tile, int page) {
         const bool there = page >= 0 && page < c.pages;

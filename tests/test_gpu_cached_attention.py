@@ -469,3 +469,16 @@ def test_a_large_value_of_little_weight(cuda, bits, q_heads, room, dtype):
     q.fill_(-1)  # 64 products of -1 with 1: a score of -64 scale, the others' 0
     scale = bits * 0.6931471805599453 / 64
     check_relative(attention.cached_attention(q, cache, table, s, o, scale=scale), q, cache, table, s, o, scale=scale)
+
+
+@pytest.mark.parametrize("page", [-1, -2, -3, -(1 << 31), 10_000, (1 << 31) - 1])
+@pytest.mark.parametrize("q_heads,room", [(4, 0), (4, WIDE), (128, WIDE)])
+def test_every_page_that_is_not_there_is_counted(cuda, q_heads, room, page):
+    q, cache, table, s, o = make([300], [2], q_heads, 2, 64, 16, torch.bfloat16, room=room)
+    table[0, 3] = page
+    check(attention.cached_attention(q, cache, table, s, o), q, cache, table, s, o)
+    with pytest.raises(ConfigError):
+        cache.check()
+    cache.append(q[:, :2], q[:, :2], table, vector([47]), o)
+    with pytest.raises(ConfigError, match="^1 accesses"):
+        cache.check()
