@@ -23,6 +23,10 @@
 // equal pieces, one per CTA, whatever the sequences' lengths are (they are known on the device alone):
 // a unit that lies in one piece is finished there, one that is cut leaves its parts in scratch and
 // `combine` joins them in order, so results do not depend on timing.
+//
+// Four row tiles at width 128 spill (296 to 420 bytes of stores a thread, bfloat16 to float32), as do two at width 256 (164
+// to 244) and four at width 64 in bfloat16 and float32 (60 and 44). A row tile's steps end at its last row's position, but
+// the pieces are cut as if all tiles of a sequence had the last one's.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -37,7 +41,10 @@ using namespace tgcb_attend;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 32;       // keys a warp takes at once; pages hold 16 or more, so a step touches at most two
-constexpr int kMaxCtas = 444;   // three per SM, which fit at once; with 888 the long float32 case took 160 instead of 142 us
+// Three per SM, which fit at once with one row tile and widths up to 128 (with 888 the long float32 case took 160 instead of
+// 142 us). Two fit with more row tiles and one at width 256, for registers and shared memory: there the equal pieces run in one
+// and a half and in three rounds. Scratch is for this many.
+constexpr int kMaxCtas = 444;
 constexpr int kMinSteps = 8;    // steps a CTA takes at least: two per warp
 constexpr int kWholeBelow = 512;  // positions up to which units are not cut, which saves the second launch
 
@@ -559,7 +566,9 @@ int row_tiles(const Batch& b, int group, int width) {
 // 32 query rows a key head on average and the call may have four tiles of 128 keys for every SM. Measured there and
 // here: 2 x 509 tokens behind 4000 positions 132 and 367 us, 32 trees of 1 to 31 nodes over 2000 to 8000 positions 273
 // and 515 us; one tree of 13 nodes over 2047 positions, too little to fill the longer pipeline, 50 and 42 us (each
-// from a cold L2, a single call).
+// from a cold L2, a single call). Below 52 rows the two were not compared. Lengths are on the device, so the
+// choice goes by the call's average: 512 tokens beside 200 single ones (32 heads on 8 of 128, over 2000 positions) take
+// 456 us, and 89 + 151 us in two calls.
 bool for_tensor(const Cache& c, const Batch& b, int group) {
   if ((c.width != 64 && c.width != 128) || (b.tokens + b.batch - 1) / b.batch * group <= 32) return false;
   if ((long long)c.pages * c.heads * c.page > 0x7fffffffll) return false;  // it numbers rows in 32 bits

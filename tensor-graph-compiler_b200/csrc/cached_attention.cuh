@@ -33,7 +33,8 @@ struct Args {
 
 // Bytes 0 and 2 of a word of int8 codes as two bfloat16, each x / 64. With the sign bit flipped a byte is x + 128,
 // and the bfloat16 whose low byte it is and whose high byte is zero has the value (x + 128) 2^-133, subnormal
-// below 128 and normal from there; times 2^127, minus 2, is x 2^-6, exactly. `flip` and `mask` are
+// below 128 and normal from there; times 2^127, minus 2, is x 2^-6, exactly (the usual way to a float through its
+// exponent's bits, in multiply-add form). `flip` and `mask` are
 // 0x00800080 and 0x00ff00ff in registers, for with two constants in it the logic operation is issued twice.
 // Against cutting the byte into its sign and its other bits and subtracting the two as
 // bfloat16 numbers around 128: 1.5 arithmetic-logic instructions fewer for every two codes.

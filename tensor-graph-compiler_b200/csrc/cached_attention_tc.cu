@@ -18,9 +18,12 @@
 //
 // Bound by its 20 warps of three codes, which issue 0.53 instructions a cycle and scheduler and wait for one another,
 // tensor memory and instruction fetch (4.1 to 4.3 us for 128 rows x 128 keys at width 128, of which the products, the
-// second in two parts, take 1.1). Loops are kept short for that reason. Measured: 2 x 509 tokens of 16 heads on 4 behind 4000
-// positions 122 us, 290 TFLOP/s; 32 trees of 1 to 31 nodes, 32 heads on 8, over 2000 to 8000 positions 255 to 268
-// us (calls in a row).
+// second in two parts, take 1.1), with 320 to 454 bytes of spill stores and 548 to 580 of spill loads a thread under the
+// launch's 96 registers. Loops are kept short for that reason. Every tile of codes is converted for 128 rows alone, both
+// groups having the same ones, and a sequence's tiles of rows count alike in the division of the work although early rows
+// see fewer keys: one prompt of 8192 tokens behind nothing, 32 heads on 8, takes 2477 us (222 TFLOP/s; its busiest CTA has
+// 1.9 times the average's tiles). Measured: 2 x 509 tokens of 16 heads on 4 behind 4000 positions 122 us, 290 TFLOP/s; 32
+// trees of 1 to 31 nodes, 32 heads on 8, over 2000 to 8000 positions 242 to 270 us (calls in a row).
 // All waits are bounded (4 s); a CTA that gives up records status 6 and unwinds.
 #include <atomic>
 #include <cmath>

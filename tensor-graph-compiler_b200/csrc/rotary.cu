@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_rotate_rows(const Params 
 // shared memory that no other thread touches. Angles are computed for as many tiles of tokens at a time (a
 // batch) as gives every thread one, a batch ahead, so that there is one barrier a batch. Measured, 8192 tokens
 // of 32 + 8 bfloat16 heads of 128: forward 40 us (168 MB, 4.2 TB/s), backward 56 us (252 MB, 4.5 TB/s), held by
-// their instructions (some 350 a warp and step, for 16-bit elements twice the float32 ones' a byte); 4095 tokens
+// their instructions (some 350 a warp and step, for 16-bit elements twice the float32 ones' a byte; instructions on pairs of
+// float32 values are not used); 4095 tokens
 // of 16 + 4 float32 heads, backward: 20 us (126 MB, 6.2 TB/s).
 // Threads a CTA has at most, and the CTAs of that size that fit an SM's registers: 64 a thread forward, 102 backward.
 constexpr int kVecThreads[2] = {512, 320};
